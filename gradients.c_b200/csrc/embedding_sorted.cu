@@ -1,0 +1,483 @@
+// Embedding lookup with a scale, and its gradient summed in token order.
+//
+//   out[i] = s table[ids[i]];   d_table[v] = s * (sum over i with ids[i] = v, i ascending, of g[i])
+//
+// HBM-bound: the gradient reads g once and writes every table row once. The scatter with FP32 atomics next door (embedding_rope.cu)
+// needs a table of vocab x dim floats that is cleared before and rounded after, and its sums change from run to run; here the
+// positions are sorted by token first and a row is written once, when its sum is complete.
+//
+// 1. es_sort_kernel: a stable counting sort of the positions in one launch without communication between blocks. A block owns a slice
+//    of the vocabulary and reads ALL ids (they lie in L2: 4 bytes each against 2 dim for the gradient's row), so it knows by itself how
+//    many ids lie below its slice. It also clears the rows of its slice that no id names.
+// 2. es_reduce_kernel: equal pieces of the sorted list, whatever the frequencies: a warp adds a few dozen rows for 32 vectors of
+//    columns, runs that begin and end within a piece are written, the others go to FP32 partial sums.
+// 3. es_merge_kernel: adds the partial sums of the runs that cross pieces, in order.
+// Every sum is FP32 in an order that depends on the ids alone.
+#include "common.cuh"
+
+namespace {
+
+constexpr int ES_SORT_WARPS = 32;
+constexpr unsigned ES_MAX_WIDTH = 1536;      // tokens of a slice: 32 x 1536 counters fill 192 KB
+constexpr int ES_WARPS = 8;                  // of a reducing block
+
+template <typename T, int VE> struct es_vec {
+    T v[VE];
+};
+template <> struct __align__(16) es_vec<__half, 8> { __half v[8]; };
+template <> struct __align__(16) es_vec<__nv_bfloat16, 8> { __nv_bfloat16 v[8]; };
+template <> struct __align__(16) es_vec<float, 4> { float v[4]; };
+
+// ------------------------------------------------------------------ forward
+// LANES threads per row, ROWS rows each in flight.
+template <typename T, int VE, int LANES>
+__global__ void __launch_bounds__(256)
+es_lookup_kernel(const T *__restrict__ table, const int *__restrict__ ids, T *__restrict__ out, size_t n, size_t vocab, size_t dim, float scale)
+{
+    gdb_pdl_sync();
+    constexpr int ROWS = 4, PER = 256 / LANES;
+    typedef es_vec<T, VE> vec;
+    const unsigned t = threadIdx.x % LANES, r = threadIdx.x / LANES;
+    const size_t vecs = dim / VE;
+    for (size_t first = (size_t)blockIdx.x * PER * ROWS; first < n; first += (size_t)gridDim.x * PER * ROWS) {
+        int id[ROWS];
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+            const size_t row = first + u * PER + r;
+            id[u] = row < n ? __ldg(&ids[row]) : -1;
+        }
+        for (size_t v = t; v < vecs; v += LANES) {
+            vec a[ROWS];
+#pragma unroll
+            for (int u = 0; u < ROWS; ++u) {
+                if (id[u] >= 0 && (size_t)id[u] < vocab) a[u] = *reinterpret_cast<const vec *>(table + (size_t)id[u] * dim + v * VE);
+            }
+#pragma unroll
+            for (int u = 0; u < ROWS; ++u) {
+                const size_t row = first + u * PER + r;
+                if (row >= n) continue;
+                const bool in = id[u] >= 0 && (size_t)id[u] < vocab;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) gdb_io<T>::st(a[u].v, e, in ? gdb_io<T>::ld(a[u].v, e) * scale : __int_as_float(0x7fc00000));
+                *reinterpret_cast<vec *>(out + row * dim + v * VE) = a[u];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ sort
+// Block b owns tokens [b * width, (b + 1) * width). order[k] = position of the k-th id in token order, token[k] = that id; count[0] = ids
+// inside the table. `clear` != NULL: the gradient table, whose rows without an id are set to zero.
+template <typename V>
+__global__ void __launch_bounds__(ES_SORT_WARPS * 32)
+es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned width, unsigned *__restrict__ order, int *__restrict__ token,
+               unsigned *__restrict__ count, V *__restrict__ clear, size_t row_vecs)
+{
+    gdb_pdl_sync();
+    extern __shared__ unsigned counters[];   // [warps, width], then the slice's running sums
+    __shared__ unsigned warp_sum[ES_SORT_WARPS], below_sum[ES_SORT_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned v0 = blockIdx.x * width, w = min(width, vocab - v0);
+    unsigned *mine = counters + (size_t)warp * width;
+    for (unsigned k = threadIdx.x; k < ES_SORT_WARPS * width; k += blockDim.x) counters[k] = 0U;
+    __syncthreads();
+    // a warp reads a range of the ids, 32 at a time, twice: counts first
+    const unsigned per = ((n + ES_SORT_WARPS * 32U - 1U) / (ES_SORT_WARPS * 32U)) * 32U;
+    const unsigned i0 = min(n, warp * per), i1 = min(n, i0 + per);
+    unsigned below = 0U;
+#pragma unroll 4
+    for (unsigned i = i0 + lane; i < i1; i += 32U) {
+        const unsigned id = (unsigned)__ldg(&ids[i]);   // (a negative id lies above every vocabulary)
+        below += id < v0 ? 1U : 0U;
+        if (id - v0 < w) atomicAdd(&mine[id - v0], 1U);
+    }
+    below = __reduce_add_sync(0xffffffffU, below);
+    if (lane == 0) below_sum[warp] = below;
+    __syncthreads();
+    unsigned base = 0U;
+#pragma unroll
+    for (int k = 0; k < ES_SORT_WARPS; ++k) base += below_sum[k];
+    // place of the first id of (token, warp), tokens first: a thread per token, 1024 tokens at a time
+    for (unsigned k0 = 0; k0 < w; k0 += blockDim.x) {
+        const unsigned k = k0 + threadIdx.x;
+        unsigned total = 0U;
+        if (k < w) {
+#pragma unroll 8
+            for (int s = 0; s < ES_SORT_WARPS; ++s) total += counters[(size_t)s * width + k];
+        }
+        unsigned incl = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned up = __shfl_up_sync(0xffffffffU, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        unsigned before = base, all = 0U;
+#pragma unroll
+        for (int s = 0; s < ES_SORT_WARPS; ++s) {
+            before += s < warp ? warp_sum[s] : 0U;
+            all += warp_sum[s];
+        }
+        if (k < w) {
+            unsigned at = before + incl - total;
+#pragma unroll 8
+            for (int s = 0; s < ES_SORT_WARPS; ++s) {
+                const unsigned c = counters[(size_t)s * width + k];
+                counters[(size_t)s * width + k] = at;
+                at += c;
+            }
+        }
+        // rows that no id names
+        if (clear != nullptr) {
+            const V zero = {};
+            for (unsigned s = __ballot_sync(0xffffffffU, k < w && total == 0U); s != 0U; s &= s - 1U) {
+                V *row = clear + (size_t)(v0 + k0 + warp * 32U + (unsigned)__ffs(s) - 1U) * row_vecs;
+                for (size_t c = lane; c < row_vecs; c += 32U) row[c] = zero;
+            }
+        }
+        base += all;
+        __syncthreads();
+    }
+    if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) count[0] = base;
+    // the same ranges again: every id of the slice to its place, equal ids of a warp's 32 in lane order
+    for (unsigned i = i0; i < i1; i += 32U) {
+        const unsigned id = i + lane < i1 ? (unsigned)__ldg(&ids[i + lane]) : 0xffffffffU;
+        const bool in = id - v0 < w;
+        if (__ballot_sync(0xffffffffU, in) == 0U) continue;
+        const unsigned peers = __match_any_sync(0xffffffffU, in ? id - v0 : w + lane);
+        const unsigned before = __popc(peers & ((1U << lane) - 1U));
+        unsigned at = 0U;
+        if (in) at = mine[id - v0] + before;
+        __syncwarp();
+        if (in && before == 0U) mine[id - v0] = at + __popc(peers);
+        __syncwarp();
+        if (in) {
+            order[at] = i + lane;
+            token[at] = (int)id;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ sums
+template <typename T, int VE>
+__device__ __forceinline__ void es_store(T *p, const float *s, float scale, bool add)
+{
+    typedef es_vec<T, VE> vec;
+    vec v;
+    if (add) v = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        // accumulating: round, add, round, as gd_backend_accumulate after the plain call would
+        const float r = __fmul_rn(s[e], scale);   // (never fused with the addition)
+        gdb_io<T>::st(v.v, e, add ? gdb_io<T>::ld(v.v, e) + gdb_io<T>::rnd(r) : r);
+    }
+    *reinterpret_cast<vec *>(p) = v;
+}
+
+// Block (c, s): sorted entries [c * piece, (c + 1) * piece), a warp an eighth of them, columns [s * 32 * VE * NV, ...).
+// partial[c, 0] = sum of the run that began in an earlier piece, partial[c, 1] = of the one that begins here and goes on behind.
+template <typename T, int VE, int NV>
+__global__ void __launch_bounds__(ES_WARPS * 32)
+es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table,
+                 float *__restrict__ partial, unsigned piece, size_t dim, float scale, bool add)
+{
+    gdb_pdl_sync();
+    typedef es_vec<T, VE> vec;
+    constexpr int COLS = 32 * VE * NV, U = NV == 1 ? 8 : 2;
+    __shared__ float head[ES_WARPS][COLS], tail[ES_WARPS][COLS];
+    const unsigned total = count[0];
+    const unsigned e0 = blockIdx.x * piece;
+    if (e0 >= total) return;
+    const unsigned e1 = min(total, e0 + piece);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned per = piece / ES_WARPS, a = min(e1, e0 + warp * per), b = min(e1, a + per);
+    const size_t col0 = (size_t)blockIdx.y * COLS;
+    float acc[NV][VE];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
+    }
+    auto keep = [&](float *to) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                to[(lane + 32 * j) * VE + e] = acc[j][e];
+                acc[j][e] = 0.0f;
+            }
+        }
+    };
+    // runs that are not complete within the warp's entries
+    const int before = a > 0U && a < b ? token[a - 1] : -1, after = b < total && a < b ? token[b] : -1;
+    bool open_left = a < b && before == token[a];
+    int current = a < b ? token[a] : -1;
+    for (unsigned i = a; i < b; i += 32U) {
+        const unsigned mine = i + lane < b ? order[i + lane] : 0U;
+        const int mine_token = i + lane < b ? token[i + lane] : -1;
+        const int here = (int)min(32U, b - i);
+        for (int k = 0; k < here; k += U) {
+            vec v[U][NV];
+            int tok[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const unsigned pos = __shfl_sync(0xffffffffU, mine, (k + u) & 31);
+                tok[u] = __shfl_sync(0xffffffffU, mine_token, (k + u) & 31);
+                if (k + u < here) {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        const size_t c = col0 + (lane + 32 * j) * VE;
+                        if (c < dim) v[u][j] = *reinterpret_cast<const vec *>(g + (size_t)pos * dim + c);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k + u >= here) break;
+                if (tok[u] != current) {
+                    if (open_left) {
+                        keep(head[warp]);
+                        open_left = false;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NV; ++j) {
+                            const size_t c = col0 + (lane + 32 * j) * VE;
+                            if (c < dim) es_store<T, VE>(table + (size_t)current * dim + c, acc[j], scale, add);
+#pragma unroll
+                            for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
+                        }
+                    }
+                    current = tok[u];
+                }
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    if (col0 + (lane + 32 * j) * VE < dim) {
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) acc[j][e] += gdb_io<T>::ld(v[u][j].v, e);
+                    }
+                }
+            }
+        }
+    }
+    if (a < b) {
+        if (open_left) {
+            keep(head[warp]);
+        } else if (after == current) {
+            keep(tail[warp]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const size_t c = col0 + (lane + 32 * j) * VE;
+                if (c < dim) es_store<T, VE>(table + (size_t)current * dim + c, acc[j], scale, add);
+            }
+        }
+    }
+    __syncthreads();
+    // runs that cross the warps of the block, a thread per column, warps in order
+    for (int c = threadIdx.x; c < COLS; c += ES_WARPS * 32) {
+        if (col0 + c >= dim) break;
+        float sum = 0.0f;
+        bool from_before = true;   // the run being added began in an earlier piece
+        for (int k = 0; k < ES_WARPS; ++k) {
+            const unsigned ka = min(e1, e0 + k * per), kb = min(e1, ka + per);
+            if (ka >= kb) break;
+            const bool left = ka > 0U && token[ka - 1] == token[ka], right = kb < total && token[kb - 1] == token[kb];
+            const bool through = left && right && token[ka] == token[kb];
+            if (left) {
+                sum += head[k][c];
+                if (!through) {
+                    if (from_before) {
+                        partial[(size_t)blockIdx.x * 2U * dim + col0 + c] = sum;
+                    } else {
+                        es_store<T, 1>(table + (size_t)token[ka] * dim + col0 + c, &sum, scale, add);
+                    }
+                    sum = 0.0f;
+                    from_before = false;
+                }
+            } else {
+                from_before = false;
+            }
+            if (right && !through) {
+                sum = tail[k][c];
+                from_before = false;
+            }
+            if (kb == e1 && right) partial[((size_t)blockIdx.x * 2U + (from_before ? 0U : 1U)) * dim + col0 + c] = sum;
+        }
+    }
+}
+
+// Block (c, s): the run that begins in piece c and goes on in the next ones, if there is one; a warp adds every eighth of its parts.
+template <typename T>
+__global__ void __launch_bounds__(256)
+es_merge_kernel(const float *__restrict__ partial, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table, unsigned piece, size_t dim,
+                float scale, bool add)
+{
+    gdb_pdl_sync();
+    __shared__ float sh[8][33];
+    const unsigned total = count[0], c = blockIdx.x, e0 = c * piece, e1 = e0 + piece;
+    if (e1 >= total) return;
+    const int k = token[e1];
+    if (token[e1 - 1] != k || (e0 > 0U && token[e0 - 1] == k)) return;   // complete, or begun earlier
+    // last piece whose first entry has this token
+    unsigned lo = c + 1U, hi = (total - 1U) / piece;
+    while (lo < hi) {
+        const unsigned mid = (lo + hi + 1U) / 2U;
+        if (token[(size_t)mid * piece] == k) lo = mid; else hi = mid - 1U;
+    }
+    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+    for (size_t col0 = (size_t)blockIdx.y * 32U; col0 < dim; col0 += (size_t)gridDim.y * 32U) {
+        const size_t col = col0 + lane;
+        float s = 0.0f;
+        if (col < dim) {
+#pragma unroll 4
+            for (unsigned j = c + (unsigned)part; j <= lo; j += 8U) s += __ldcg(&partial[((size_t)j * 2U + (j == c ? 1U : 0U)) * dim + col]);
+        }
+        sh[part][lane] = s;
+        __syncthreads();
+        if (part == 0 && col < dim) {
+            float v = 0.0f;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) v += sh[p][lane];
+            es_store<T, 1>(table + (size_t)k * dim + col, &v, scale, add);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int VE>
+gd_status lookup(gd_backend *be, const void *table, const int *ids, void *out, const gd_backend_embedding_args *a, float scale)
+{
+    const size_t vecs = a->dim / VE;
+#define GO(LANES)                                                                                                                                             \
+    gdb_launch(es_lookup_kernel<T, VE, LANES>, gdb_grid_for((a->ids_count + 4U * (256 / LANES) - 1U) / (4U * (256 / LANES)), 1U, be, 32U), 256, 0, be->stream, \
+               (const T *)table, ids, (T *)out, a->ids_count, a->vocab, a->dim, scale)
+    if (vecs <= 16U) GO(16); else if (vecs <= 32U) GO(32); else if (vecs <= 64U) GO(64); else if (vecs <= 128U) GO(128); else GO(256);
+#undef GO
+    return gdb_launched(be, "embedding_scaled_forward");
+}
+
+template <typename T, int VE, int NV>
+gd_status reduce(gd_backend *be, const void *g, const unsigned *order, const int *token, const unsigned *count, void *table, float *partial, unsigned piece, unsigned pieces,
+                 size_t dim, float scale, bool add)
+{
+    const size_t slabs = (dim + 32U * VE * NV - 1U) / (32U * VE * NV);
+    if (slabs > 65535U) return GD_ERR_UNSUPPORTED;
+    gdb_launch(es_reduce_kernel<T, VE, NV>, dim3(pieces, (unsigned)slabs), ES_WARPS * 32, 0, be->stream, (const T *)g, order, token, count, (T *)table, partial, piece, dim, scale, add);
+    gd_status st = gdb_launched(be, "embedding_sorted_backward sums");
+    if (st != GD_OK || pieces == 1U) return st;
+    const size_t col_blocks = (dim + 31U) / 32U;
+    gdb_launch(es_merge_kernel<T>, dim3(pieces - 1U, (unsigned)(col_blocks < 64U ? col_blocks : 64U)), 256, 0, be->stream, (const float *)partial, token, count, (T *)table, piece, dim,
+               scale, add);
+    return gdb_launched(be, "embedding_sorted_backward merge");
+}
+
+template <typename T>
+gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, const gd_backend_embedding_args *a, float scale, bool add)
+{
+    constexpr int VE = sizeof(T) == 2 ? 8 : 4;
+    const unsigned n = (unsigned)a->ids_count, vocab = (unsigned)a->vocab;
+    const size_t dim = a->dim, row_bytes = dim * sizeof(T);
+    const bool vec = dim % VE == 0U && (((uintptr_t)g | (uintptr_t)table) % 16U) == 0U;
+    const size_t slabs = vec ? (dim + 32U * VE - 1U) / (32U * VE) : (dim + 255U) / 256U;
+    // order, token, count, partial sums
+    const size_t list = ((size_t)n * 4U + 255U) & ~(size_t)255U;
+    if (2U * list + 256U + 2U * dim * sizeof(float) > be->ws_bytes) return GD_ERR_OUT_OF_MEMORY;
+    unsigned *order = reinterpret_cast<unsigned *>(be->ws);
+    int *token = reinterpret_cast<int *>(be->ws + list);
+    unsigned *count = reinterpret_cast<unsigned *>(be->ws + 2U * list);
+    float *partial = reinterpret_cast<float *>(be->ws + 2U * list + 256U);
+    const size_t fit = (be->ws_bytes - 2U * list - 256U) / (2U * dim * sizeof(float));
+    // entries of a warp: 32, fewer while the blocks would not fill the GPU twice, more where the partial sums would not fit the workspace
+    size_t per = 32U;
+    while (per > 8U && ((size_t)n + per * ES_WARPS - 1U) / (per * ES_WARPS) * slabs < 2U * (size_t)be->sm_count) per /= 2U;
+    while (((size_t)n + per * ES_WARPS - 1U) / (per * ES_WARPS) > fit) per *= 2U;
+    const size_t piece = per * ES_WARPS, pieces = ((size_t)n + piece - 1U) / piece;
+    // a slice of the vocabulary per block, two blocks' worth of SMs at most where the counters allow it
+    unsigned width = (vocab + (unsigned)be->sm_count - 1U) / (unsigned)be->sm_count;
+    if (width > ES_MAX_WIDTH) width = ES_MAX_WIDTH;
+    const unsigned slices = (vocab + width - 1U) / width;
+    const int smem = (int)(width * ES_SORT_WARPS * sizeof(unsigned));
+    static bool ready = false;
+    if (!ready) {
+        const int most = (int)(ES_MAX_WIDTH * ES_SORT_WARPS * sizeof(unsigned));
+        cudaError_t e = cudaFuncSetAttribute(es_sort_kernel<uint4>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(es_sort_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return gdb_fail(be, e, "embedding_sorted_backward smem attribute");
+        ready = true;
+    }
+    if (vec) {
+        gdb_launch(es_sort_kernel<uint4>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, order, token, count, add ? (uint4 *)nullptr : (uint4 *)table, row_bytes / 16U);
+    } else {
+        gdb_launch(es_sort_kernel<T>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, order, token, count, add ? (T *)nullptr : (T *)table, dim);
+    }
+    gd_status st = gdb_launched(be, "embedding_sorted_backward sort");
+    if (st != GD_OK) return st;
+    return vec ? reduce<T, VE, 1>(be, g, order, token, count, table, partial, (unsigned)piece, (unsigned)pieces, dim, scale, add)
+               : reduce<T, 1, 8>(be, g, order, token, count, table, partial, (unsigned)piece, (unsigned)pieces, dim, scale, add);
+}
+
+bool es_args_ok(const gd_backend_tensor_view *rows, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *table, const gd_backend_embedding_args *a)
+{
+    return rows != NULL && ids != NULL && table != NULL && a != NULL && a->vocab > 0U && a->dim > 0U && a->vocab <= SIZE_MAX / 8U / a->dim &&
+           a->ids_count <= SIZE_MAX / 8U / a->dim && rows->dtype == table->dtype && table->count == a->vocab * a->dim && ids->count == a->ids_count &&
+           rows->count == a->ids_count * a->dim;
+}
+
+}  // namespace
+
+extern "C" {
+
+gd_status gdb200_embedding_scaled_forward(gd_backend *be, const gd_backend_tensor_view *table, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *out, float scale,
+                                          const gd_backend_embedding_args *args)
+{
+    if (be == NULL || !es_args_ok(out, ids, table, args)) {
+        return GD_ERR_INVALID_ARGUMENT;
+    }
+    const uint32_t dt = table->dtype;
+    if (!gdb_is_float_dtype(dt)) {
+        return GD_ERR_UNSUPPORTED;
+    }
+    const void *tp = gdb_tv_ptr(table, dt);
+    const int *ip = (const int *)gdb_tv_ptr(ids, GDB_DTYPE_I32);
+    void *op = gdb_tv_ptr(out, dt);
+    if (tp == NULL || ip == NULL || op == NULL) {
+        return GD_ERR_INVALID_ARGUMENT;
+    }
+    if (args->ids_count == 0U) {
+        return GD_OK;
+    }
+    const bool vec = args->dim % (16U / gdb_dtype_size(dt)) == 0U && (((uintptr_t)tp | (uintptr_t)op) % 16U) == 0U;
+    if (dt == GDB_DTYPE_F16) return vec ? lookup<__half, 8>(be, tp, ip, op, args, scale) : lookup<__half, 1>(be, tp, ip, op, args, scale);
+    if (dt == GDB_DTYPE_BF16) return vec ? lookup<__nv_bfloat16, 8>(be, tp, ip, op, args, scale) : lookup<__nv_bfloat16, 1>(be, tp, ip, op, args, scale);
+    return vec ? lookup<float, 4>(be, tp, ip, op, args, scale) : lookup<float, 1>(be, tp, ip, op, args, scale);
+}
+
+gd_status gdb200_embedding_sorted_backward(gd_backend *be, const gd_backend_tensor_view *grad_out, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *grad_table,
+                                           int32_t accumulate, float scale, const gd_backend_embedding_args *args)
+{
+    if (be == NULL || !es_args_ok(grad_out, ids, grad_table, args)) {
+        return GD_ERR_INVALID_ARGUMENT;
+    }
+    const uint32_t dt = grad_table->dtype;
+    if (!gdb_is_float_dtype(dt) || args->ids_count > 0x7fffffffU || args->vocab > 0x7fffffffU) {
+        return GD_ERR_UNSUPPORTED;
+    }
+    const void *gp = gdb_tv_ptr(grad_out, dt);
+    const int *ip = (const int *)gdb_tv_ptr(ids, GDB_DTYPE_I32);
+    void *tp = gdb_tv_ptr(grad_table, dt);
+    if (gp == NULL || ip == NULL || tp == NULL) {
+        return GD_ERR_INVALID_ARGUMENT;
+    }
+    if (args->ids_count == 0U) {
+        if (accumulate != 0) return GD_OK;
+        const cudaError_t e = cudaMemsetAsync(tp, 0, grad_table->count * gdb_dtype_size(dt), be->stream);
+        be->launches += 1U;
+        return e == cudaSuccess ? GD_OK : gdb_fail(be, e, "embedding_sorted_backward zero");
+    }
+    return dt == GDB_DTYPE_F16    ? backward<__half>(be, gp, ip, tp, args, scale, accumulate != 0)
+           : dt == GDB_DTYPE_BF16 ? backward<__nv_bfloat16>(be, gp, ip, tp, args, scale, accumulate != 0)
+                                  : backward<float>(be, gp, ip, tp, args, scale, accumulate != 0);
+}
+
+}  // extern "C"

@@ -121,6 +121,14 @@ class KvCacheAppendArgs(C.Structure):
     _fields_ = [("cache_pos", I32_T)]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [("rows", U64), ("cols", U64), ("eps", F), ("reserved0", U32)]
+
+
+class OrthogonalizeArgs(C.Structure):
+    _fields_ = [("batch", U64), ("rows", U64), ("cols", U64), ("steps", U32), ("a", F), ("b", F), ("c", F), ("eps", F)]
+
+
 GPT_MAX_LAYERS = 64
 GPT_MAX_PARAMS = 1 + 10 * GPT_MAX_LAYERS + 3
 
@@ -310,6 +318,12 @@ PROTOTYPES = {
     "gdb200_rms_norm_backward_with_weight_dropout": (_ST, [P, TV, TV, TV, TV, TV, I32_T, TV, TV, C.POINTER(RmsNormArgs), TV, TV, F, TV]),
     "gdb200_embedding_dropout_rms_norm": (_ST, [P, TV, TV, TV, TV, TV, TV, TV, F, F, U64]),
     "gdb200_lm_cross_entropy_fused_rows": (_ST, [P, TV, TV, TV, TV, TV, TV, F, F, I32_T]),
+    "gdb200_layer_norm_forward": (_ST, [P, TV, TV, TV, TV, TV, C.POINTER(LayerNormArgs)]),
+    "gdb200_layer_norm_backward": (_ST, [P, TV, TV, TV, TV, TV, I32_T, TV, TV, C.POINTER(LayerNormArgs)]),
+    "gdb200_embedding_scaled_forward": (_ST, [P, TV, TV, TV, F, C.POINTER(EmbeddingArgs)]),
+    "gdb200_embedding_sorted_backward": (_ST, [P, TV, TV, TV, I32_T, F, C.POINTER(EmbeddingArgs)]),
+    "gdb200_orthogonalize_scratch_bytes": (SZ, [C.POINTER(OrthogonalizeArgs)]),
+    "gdb200_orthogonalize": (_ST, [P, TV, TV, TV, C.POINTER(OrthogonalizeArgs)]),
     "gdb200_matmul_tn_colsum": (_ST, [P, MV, MV, MV, VV]),
     "gdb200_argmax_rows": (_ST, [P, TV, F, TV]),
     "gdb200_gpt_prefill": (_ST, [P, C.POINTER(GptSpec), C.POINTER(GptBatch), SZ, SZ, C.POINTER(GptDecodeState), C.POINTER(SZ)]),

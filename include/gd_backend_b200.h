@@ -536,6 +536,51 @@ gd_status gdb200_embedding_backward_static(void *stream, const void *grad_out, c
 const char *gdb200_embedding_backward_static_error(void);
 uint64_t gdb200_embedding_backward_static_max_elems(void);
 
+/* Layer norm (no counterpart in the reference, whose norm is the RMS norm of src/ops/rms_norm): out = (x - mean) / sqrt(var + eps) * weight
+ * + bias over the last dimension of x [rows, cols], var the mean of (x - mean)^2. weight and bias [cols] may be NULL (1 and 0); out may be x.
+ * stats F32 [rows, 2] = mean and 1 / sqrt(var + eps) of every row, NULL where no backward pass follows. F16, BF16 or F32 throughout (one
+ * type), any cols, sums FP32, one rounding. rows may be 0.
+ * Backward: grad_x (accumulate != 0: added into grad_x: round, add, round, as gd_backend_accumulate after the entry would), grad_weight =
+ * sum over rows of grad_out * (x - mean) / sqrt(var + eps), grad_bias = sum over rows of grad_out; each may be NULL, not all three. The two
+ * sums are FP32 in an order that depends on the shape alone, through partial sums in the backend's workspace (GD_ERR_UNSUPPORTED where one
+ * row of them, 8 * cols bytes, does not fit it). grad_x may be grad_out where it is not accumulated into. */
+typedef struct gdb200_layer_norm_args {
+    uint64_t rows, cols;
+    float eps;
+    uint32_t reserved0;
+} gdb200_layer_norm_args;
+gd_status gdb200_layer_norm_forward(gd_backend *backend, const gd_backend_tensor_view *x, const gd_backend_tensor_view *weight, const gd_backend_tensor_view *bias,
+                                    const gd_backend_tensor_view *out, const gd_backend_tensor_view *stats, const gdb200_layer_norm_args *args);
+gd_status gdb200_layer_norm_backward(gd_backend *backend, const gd_backend_tensor_view *x, const gd_backend_tensor_view *weight, const gd_backend_tensor_view *stats,
+                                     const gd_backend_tensor_view *grad_out, const gd_backend_tensor_view *grad_x, int32_t accumulate,
+                                     const gd_backend_tensor_view *grad_weight, const gd_backend_tensor_view *grad_bias, const gdb200_layer_norm_args *args);
+
+/* Embedding lookup with a scale, out[i] = round(scale * table[ids[i]]), NaN rows for ids outside the table as gd_backend_embedding_forward
+ * gives; and its gradient grad_table[v] = round(scale * sum of grad_out[i] over the i with ids[i] = v), ids outside the table skipped.
+ * Against gd_backend_embedding_backward: the rows are summed in FP32 in the order of the ids, so a call repeats bit for bit, no FP32
+ * table is lent, and accumulate != 0 adds into grad_table (round, add, round, as gd_backend_accumulate after the plain call would)
+ * touching only the rows that the ids name (a tied head's gradient). F16, BF16, F32, any dim; up to 2^31 - 1 ids and table rows. The sorted
+ * order (8 bytes an id) and partial sums lie in the backend's workspace; GD_ERR_OUT_OF_MEMORY where they do not fit. */
+gd_status gdb200_embedding_scaled_forward(gd_backend *backend, const gd_backend_tensor_view *table, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *out, float scale,
+                                          const gd_backend_embedding_args *args);
+gd_status gdb200_embedding_sorted_backward(gd_backend *backend, const gd_backend_tensor_view *grad_out, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *grad_table,
+                                           int32_t accumulate, float scale, const gd_backend_embedding_args *args);
+
+/* Orthogonalisation of `batch` matrices [rows, cols] by Newton-Schulz products (what the Muon optimizer steps along; the reference has
+ * AdamW only, src/optim/adamw.c): X = x / (|x|_F + eps), then `steps` times A = X X^T (on the smaller side), X <- a X + (b A + c A^2) X,
+ * out = X. x F16, BF16 or F32, out F16 or BF16 (the products' operands are FP16 with FP32 sums, the iterate is carried in two FP16 numbers:
+ * the result is within 0.2 % of 64-bit arithmetic in the 2-norm); out may be x. The iterates have to stay below 64 in magnitude, as they do
+ * for coefficients whose polynomial maps [0, 1.3] into itself. A matrix of zeros gives zeros (eps > 0). `scratch`: U8, 256-byte aligned, of
+ * gdb200_orthogonalize_scratch_bytes(args) bytes (0: a shape that is not taken), not to be shared with a call on another stream. */
+typedef struct gdb200_orthogonalize_args {
+    uint64_t batch, rows, cols;
+    uint32_t steps;
+    float a, b, c, eps;
+} gdb200_orthogonalize_args;
+size_t gdb200_orthogonalize_scratch_bytes(const gdb200_orthogonalize_args *args);
+gd_status gdb200_orthogonalize(gd_backend *backend, const gd_backend_tensor_view *x, const gd_backend_tensor_view *out, const gd_backend_tensor_view *scratch,
+                               const gdb200_orthogonalize_args *args);
+
 /* Native sequencing of one gpt_lm training step (no counterpart in the reference's backend ABI; it
  * replays the call sequence of the reference's host: src/train/trainer.c:75-223,
  * examples/gpt_lm/gpt_lm_shared.c:602-823, src/optim/adamw.c:2163-2270). The caller lays out
