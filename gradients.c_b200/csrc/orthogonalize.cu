@@ -19,99 +19,216 @@ constexpr float NS_UP = 1024.0f, NS_DOWN = 1.0f / 1024.0f;
 constexpr int NS_NORM_BLOCKS = 64;   // partial sums of a matrix's squares, at most
 
 // ------------------------------------------------------------------ |G|_F and the first iterate
-// Sums of squares are FP64: neither 1e38 nor 1e-38 leaves the range, and the order of the sum does not show.
+// eight consecutive elements of a row, zeros behind its end
+template <typename T>
+__device__ __forceinline__ void ns_load8(const T *p, unsigned left, bool vec, float (&f)[8])
+{
+    if (vec) {
+        if constexpr (sizeof(T) == 2) {
+            gdb_vec8<T> v;
+            v.raw = __ldg(reinterpret_cast<const uint4 *>(p));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = v.get(e);
+        } else {
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (unsigned)e < left ? gdb_io<T>::ld(p, e) : 0.0f;
+    }
+}
+// Sums of squares are FP64: neither 1e38 nor 1e-38 leaves the range. The matrix is taken as one row of `count` elements.
 template <typename T>
 __global__ void __launch_bounds__(256)
-ns_norm_kernel(const T *__restrict__ g, double *__restrict__ partial, size_t count)
+ns_norm_kernel(const T *__restrict__ g, double *__restrict__ partial, size_t count, bool vec)
 {
     gdb_pdl_sync();
     __shared__ double sh[8];
     const T *m = g + (size_t)blockIdx.y * count;
-    double s = 0.0;
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (size_t)gridDim.x * blockDim.x) {
-        const double v = (double)gdb_io<T>::ld(m, i);
-        s += v * v;
-    }
+    double s[2] = {0.0, 0.0};
+    const size_t stride = (size_t)gridDim.x * blockDim.x * 8U;
+#pragma unroll 4
+    for (size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 8U; i < count; i += stride) {
+        float f[8];
+        ns_load8(m + i, (unsigned)min((size_t)8U, count - i), vec && i + 8U <= count, f);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffU, s, o);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+        for (int e = 0; e < 8; ++e) s[e & 1] += (double)f[e] * (double)f[e];
+    }
+    double t = s[0] + s[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = t;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) s += sh[w];
-        partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + blockIdx.x] = s;
+        for (int w = 1; w < 8; ++w) t += sh[w];
+        partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + blockIdx.x] = t;
     }
 }
 template <typename T>
 __global__ void __launch_bounds__(256)
-ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int parts, __half *__restrict__ hi, __half *__restrict__ lo, size_t rows, size_t cols, size_t pitch,
-                float eps)
+ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int parts, __half *__restrict__ hi, __half *__restrict__ lo, unsigned rows, unsigned cols,
+                unsigned octets, float eps, bool vec)
 {
     gdb_pdl_sync();
-    double s = 0.0;
-    for (int k = 0; k < parts; ++k) s += __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + k]);
+    // (every warp adds the partial sums in the same order)
+    const int lane = threadIdx.x & 31;
+    double s = (lane < parts ? __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + lane]) : 0.0) +
+               (lane + 32 < parts ? __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + lane + 32]) : 0.0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffU, s, o);
     const double f = (double)NS_UP / (sqrt(s) + (double)eps);
+    const bool small = f < 3.0e38 && f > 1.2e-38;   // the factor is a normal FP32 number
+    const float ff = (float)f;
     const T *m = g + (size_t)blockIdx.y * rows * cols;
-    __half *h = hi + (size_t)blockIdx.y * rows * pitch, *l = lo + (size_t)blockIdx.y * rows * pitch;
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * cols; i += (size_t)gridDim.x * blockDim.x) {
-        const size_t r = i / cols, c = i - r * cols;
-        const float v = (float)((double)gdb_io<T>::ld(m, i) * f);
-        const __half a = __float2half_rn(v);
-        h[r * pitch + c] = a;
-        l[r * pitch + c] = __float2half_rn(v - __half2float(a));
+    uint4 *h = reinterpret_cast<uint4 *>(hi) + (size_t)blockIdx.y * rows * octets, *l = reinterpret_cast<uint4 *>(lo) + (size_t)blockIdx.y * rows * octets;
+    const size_t n = (size_t)rows * octets;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+        const unsigned r = n < 0xffffffffU ? (unsigned)i / octets : (unsigned)(i / octets), c = (unsigned)(i - (size_t)r * octets) * 8U;
+        float v[8];
+        ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
+        gdb_vec8<__half> a, b;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float w = small ? v[e] * ff : (float)((double)v[e] * f);
+            a.set(e, w);
+            b.set(e, w - a.get(e));
+        }
+        h[i] = a.raw;
+        l[i] = b.raw;
     }
 }
 
 // ------------------------------------------------------------------ products
+// GRAM: A = 2^-20 X X^T. POLY: P = b A + c A A. UPDATE: X <- a (hi + lo) + P hi. LAST: the same into the caller's tensor.
+// A and P are symmetric (and commute with A), so the tiles on and above the diagonal are formed and those above it stored twice, and
+// either order of the product's operands does.
 enum { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
 
-struct ns_epilogue {
-    __half *out, *out_lo;            // GRAM / POLY: the symmetric product; UPDATE: the next iterate
-    const __half *in, *in_lo;        // POLY: A; UPDATE / LAST: this iterate
-    void *final_out;                 // LAST
-    size_t out_batch, out_pitch;     // elements
-    size_t in_batch, in_pitch;
-    float alpha, beta;               // alpha * product + beta * in
+// What the epilogue reads and writes, in tiles of 32 x 64 (a warp's rows, 128 bytes a row, swizzled).
+struct ns_maps {
+    CUtensorMap a, b;        // operands
+    CUtensorMap in, lo;      // POLY: A; UPDATE, LAST: hi, and lo in and out
+    CUtensorMap out;         // A, P, the next hi, or the caller's tensor
+    CUtensorMap mirror;      // GRAM, POLY: out again, in tiles of 64 x 32 without a swizzle
+};
+struct ns_shape {
+    uint32_t M, N, K, tiles_m, tiles_n, batch;
+    float alpha, beta;
+    void *plain;             // LAST into a tensor that TMA cannot address (odd rows): its address, else NULL
 };
 
-constexpr int NS_STAGES = 4, NS_BN = 128;
-constexpr int NS_STAGE_BYTES = (BM + NS_BN) * BK * 2;
-constexpr int NS_SMEM = NS_STAGES * NS_STAGE_BYTES + 256 + 1024;
+// One warp's 32 x 64 piece of the result: v0 / v1 hold its accumulators (lane = row). `st` is the warp's staging, two 4 KB tiles: the
+// inputs arrived there and the results leave from there. Mirrored pieces are written transposed into the second tile.
+template <int MODE, typename TOUT>
+__device__ __forceinline__ void ns_finish_piece(const ns_maps &maps, const ns_shape &sh, unsigned char *st, const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t row0,
+                                                uint32_t col0, uint32_t z, bool mirror, int lane)
+{
+    unsigned char *r0 = st + lane * 128, *r1 = r0 + 4096;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int chunk = (j ^ (lane & 7)) << 4;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = sh.alpha * __uint_as_float(j < 4 ? v0[(j & 3) * 8 + e] : v1[(j & 3) * 8 + e]);
+        if (MODE != NS_GRAM) {
+            gdb_vec8<__half> a, l;
+            a.raw = *reinterpret_cast<const uint4 *>(r0 + chunk);
+            if (MODE != NS_POLY) l.raw = *reinterpret_cast<const uint4 *>(r1 + chunk);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = fmaf(sh.beta, MODE == NS_POLY ? a.get(e) : a.get(e) + l.get(e), f[e]);
+        }
+        if (MODE == NS_LAST) {
+            uint4 o;
+            o.x = half_pack<TOUT>::pack(f[0] * NS_DOWN, f[1] * NS_DOWN);
+            o.y = half_pack<TOUT>::pack(f[2] * NS_DOWN, f[3] * NS_DOWN);
+            o.z = half_pack<TOUT>::pack(f[4] * NS_DOWN, f[5] * NS_DOWN);
+            o.w = half_pack<TOUT>::pack(f[6] * NS_DOWN, f[7] * NS_DOWN);
+            *reinterpret_cast<uint4 *>(r0 + chunk) = o;
+            continue;
+        }
+        gdb_vec8<__half> o;
+        o.raw = make_uint4(half_pack<__half>::pack(f[0], f[1]), half_pack<__half>::pack(f[2], f[3]), half_pack<__half>::pack(f[4], f[5]), half_pack<__half>::pack(f[6], f[7]));
+        *reinterpret_cast<uint4 *>(r0 + chunk) = o.raw;
+        if (MODE == NS_UPDATE) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] -= o.get(e);
+            *reinterpret_cast<uint4 *>(r1 + chunk) = make_uint4(half_pack<__half>::pack(f[0], f[1]), half_pack<__half>::pack(f[2], f[3]), half_pack<__half>::pack(f[4], f[5]),
+                                                                half_pack<__half>::pack(f[6], f[7]));
+        } else if (mirror) {
+            // row j * 8 + e of the transposed piece, 64 bytes: the lanes' elements side by side
+            unsigned short *t = reinterpret_cast<unsigned short *>(st + 4096) + j * 8 * 32 + lane;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e * 32] = (unsigned short)((&o.raw.x)[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+    if (MODE == NS_LAST && sh.plain != nullptr) {
+        __syncwarp();
+        unsigned short *out = reinterpret_cast<unsigned short *>(sh.plain) + ((size_t)z * sh.M + row0) * sh.N + col0;
+        const uint32_t rows = min(32U, sh.M - row0), cols = min(64U, sh.N - col0);
+        for (uint32_t r = 0; r < rows; ++r) {
+#pragma unroll
+            for (uint32_t c = lane; c < 64U; c += 32U) {
+                if (c < cols) out[(size_t)r * sh.N + c] = *reinterpret_cast<const unsigned short *>(st + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+            }
+        }
+        fence_proxy_async_smem();   // the next inputs arrive here
+        __syncwarp();
+        return;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_3d(&maps.out, (int)col0, (int)row0, (int)z, smem_u32(st));
+        if (MODE == NS_UPDATE) tma_store_3d(&maps.lo, (int)col0, (int)row0, (int)z, smem_u32(st + 4096));
+        if ((MODE == NS_GRAM || MODE == NS_POLY) && mirror) tma_store_3d(&maps.mirror, (int)row0, (int)col0, (int)z, smem_u32(st + 4096));
+        bulk_commit_group();
+    }
+}
+// the inputs of a piece on their way to the warp's staging (one lane)
+template <int MODE>
+__device__ __forceinline__ void ns_fetch_piece(const ns_maps &maps, unsigned char *st, uint32_t bar, uint32_t row0, uint32_t col0, uint32_t z)
+{
+    mbar_expect_tx(bar, MODE == NS_POLY ? 4096 : 8192);
+    tma_load_3d(smem_u32(st), &maps.in, (int)col0, (int)row0, (int)z, bar);
+    if (MODE != NS_POLY) tma_load_3d(smem_u32(st + 4096), &maps.lo, (int)col0, (int)row0, (int)z, bar);
+}
 
-// One 128 x 128 tile per CTA. GRAM and POLY are symmetric: tiles on and above the diagonal are formed, those above it written twice.
-template <bool A_MN, bool B_MN, int MODE, typename TOUT>
-__global__ void __launch_bounds__(192, 1)
-ns_product_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, ns_epilogue ep, uint32_t M, uint32_t N, uint32_t K, uint32_t tiles_n,
-                  int *err_flag)
+// ---- one CTA, one 128 x 64 tile: small matrices, where the number of SMs at work counts ----
+constexpr int NS1_BN = 64, NS1_STAGE_BYTES = (BM + NS1_BN) * BK * 2;
+template <int STAGES> constexpr int ns1_smem() { return STAGES * NS1_STAGE_BYTES + 4 * 8192 + 256 + 1024; }
+
+template <bool A_MN, bool B_MN, int MODE, typename TOUT, int STAGES>
+__global__ void __launch_bounds__(192)
+ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err_flag)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + NS_STAGES * NS_STAGE_BYTES);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS_STAGES + 1);
+    unsigned char *staging = smem + STAGES * NS1_STAGE_BYTES;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 4 * 8192);   // full, empty, accumulator, inputs of the four epilogue warps
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 5);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t z = blockIdx.y;
     uint32_t tm, tn;
     if (SYM) {
-        // row tm of the upper triangle holds tiles_n - tm tiles
+        // of row tile tm the column tiles from the diagonal on
         uint32_t u = blockIdx.x;
-        for (tm = 0; u >= tiles_n - tm; ++tm) u -= tiles_n - tm;
-        tn = tm + u;
+        for (tm = 0; u >= sh.tiles_n - 2U * tm; ++tm) u -= sh.tiles_n - 2U * tm;
+        tn = 2U * tm + u;
     } else {
-        tm = blockIdx.x / tiles_n;
-        tn = blockIdx.x - tm * tiles_n;
+        tm = blockIdx.x / sh.tiles_n;
+        tn = blockIdx.x - tm * sh.tiles_n;
     }
-    const uint32_t m0 = tm * BM, n0 = tn * NS_BN, n_iters = (K + BK - 1) / BK;
-    const int z = (int)blockIdx.y;
-    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[NS_STAGES]), accum_bar = smem_u32(&bars[2 * NS_STAGES]);
+    const uint32_t m0 = tm * BM, n0 = tn * NS1_BN, n_iters = (sh.K + BK - 1) / BK;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]), accum_bar = smem_u32(&bars[2 * STAGES]), in0 = smem_u32(&bars[2 * STAGES + 1]);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NS_STAGES; ++s) {
-            mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 1);
-        }
-        mbar_init(accum_bar, 1);
+        for (int s = 0; s < 2 * STAGES + 5; ++s) mbar_init(full0 + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)NS_BN) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)NS1_BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tcgen05_fence_before();
@@ -123,39 +240,34 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
     if (warp == 0) {
         if (lane == 0) {
             for (uint32_t it = 0; it < n_iters; ++it) {
-                const uint32_t s = it % NS_STAGES, ph = (it / NS_STAGES) & 1U, bar = full0 + 8 * s;
+                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1U, bar = full0 + 8 * s;
                 if (!mbar_wait(empty0 + 8 * s, ph ^ 1U)) {
                     atomicExch(err_flag, 701);
                     break;
                 }
-                const uint32_t a_dst = smem_u32(smem + s * NS_STAGE_BYTES), b_dst = a_dst + BM * BK * 2;
+                const uint32_t a_dst = smem_u32(smem + s * NS1_STAGE_BYTES), b_dst = a_dst + BM * BK * 2;
                 const int k0 = (int)(it * BK);
-                mbar_expect_tx(bar, NS_STAGE_BYTES);
+                mbar_expect_tx(bar, NS1_STAGE_BYTES);
                 if (A_MN) {
-                    tma_load_3d(a_dst, &tma_a, (int)m0, k0, z, bar);
-                    tma_load_3d(a_dst + BK * 128, &tma_a, (int)m0 + 64, k0, z, bar);
+                    tma_load_3d(a_dst, &maps.a, (int)m0, k0, (int)z, bar);
+                    tma_load_3d(a_dst + BK * 128, &maps.a, (int)m0 + 64, k0, (int)z, bar);
                 } else {
-                    tma_load_3d(a_dst, &tma_a, k0, (int)m0, z, bar);
+                    tma_load_3d(a_dst, &maps.a, k0, (int)m0, (int)z, bar);
                 }
-                if (B_MN) {
-                    tma_load_3d(b_dst, &tma_b, (int)n0, k0, z, bar);
-                    tma_load_3d(b_dst + BK * 128, &tma_b, (int)n0 + 64, k0, z, bar);
-                } else {
-                    tma_load_3d(b_dst, &tma_b, k0, (int)n0, z, bar);
-                }
+                if (B_MN) tma_load_3d(b_dst, &maps.b, (int)n0, k0, (int)z, bar); else tma_load_3d(b_dst, &maps.b, k0, (int)n0, (int)z, bar);
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t IDESC = (1U << 4) | ((A_MN ? 1U : 0U) << 15) | ((B_MN ? 1U : 0U) << 16) | ((uint32_t)(NS_BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            constexpr uint32_t IDESC = (1U << 4) | ((A_MN ? 1U : 0U) << 15) | ((B_MN ? 1U : 0U) << 16) | ((uint32_t)(NS1_BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
             for (uint32_t it = 0; it < n_iters; ++it) {
-                const uint32_t s = it % NS_STAGES, ph = (it / NS_STAGES) & 1U;
+                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1U;
                 if (!mbar_wait(full0 + 8 * s, ph)) {
                     atomicExch(err_flag, 702);
                     break;
                 }
                 tcgen05_fence_after();
-                const uint32_t a_base = smem_u32(smem + s * NS_STAGE_BYTES), b_base = a_base + BM * BK * 2;
+                const uint32_t a_base = smem_u32(smem + s * NS1_STAGE_BYTES), b_base = a_base + BM * BK * 2;
 #pragma unroll
                 for (int kk = 0; kk < BK / UMMA_K; ++kk) {
                     const uint64_t adesc = A_MN ? make_smem_desc(a_base + kk * 2048, BK * 128, 1024) : make_smem_desc(a_base + kk * 32, 16, 1024);
@@ -168,86 +280,324 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
         }
     } else {
         const int quad = warp & 3;
-        const uint32_t row = m0 + quad * 32 + lane;
-        const bool ok = mbar_wait(accum_bar, 0);
+        unsigned char *st = staging + quad * 8192;
+        const uint32_t row0 = m0 + quad * 32, bar = in0 + 8 * quad;
+        const bool live = row0 < sh.M;   // (the tile's first column always lies inside)
+        if (MODE != NS_GRAM && live && lane == 0) ns_fetch_piece<MODE>(maps, st, bar, row0, n0, z);
+        bool ok = mbar_wait(accum_bar, 0);
+        if (MODE != NS_GRAM && live) ok = mbar_wait(bar, 0) && ok;
+        ok = __all_sync(0xffffffffU, ok);
         if (!ok && lane == 0) atomicExch(err_flag, 703);
         tcgen05_fence_after();
-        if (ok) {
-#pragma unroll 1
-            for (int cb = 0; cb < NS_BN / 32; ++cb) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(cb * 32), v);
-                const uint32_t col0 = n0 + cb * 32;
-#pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    if (row >= M || col0 + j >= N) continue;
-                    float f[8];
-                    gdb_vec8<__half> a, o;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = ep.alpha * __uint_as_float(v[j + e]);
-                    if (MODE != NS_GRAM) {
-                        const size_t at = (size_t)z * ep.in_batch + (size_t)row * ep.in_pitch + col0 + j;
-                        a.raw = *reinterpret_cast<const uint4 *>(ep.in + at);
-                        if (MODE == NS_POLY) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] += ep.beta * a.get(e);
-                        } else {
-                            gdb_vec8<__half> l;
-                            l.raw = *reinterpret_cast<const uint4 *>(ep.in_lo + at);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] += ep.beta * (a.get(e) + l.get(e));
-                        }
-                    }
-                    if (MODE == NS_LAST) {
-                        TOUT *dst = reinterpret_cast<TOUT *>(ep.final_out) + (size_t)z * ep.out_batch + (size_t)row * ep.out_pitch + col0 + j;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (col0 + j + e < N) gdb_io<TOUT>::st(dst, e, f[e] * NS_DOWN);
-                        }
-                        continue;
-                    }
-                    const size_t at = (size_t)z * ep.out_batch + (size_t)row * ep.out_pitch + col0 + j;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o.set(e, f[e]);
-                    *reinterpret_cast<uint4 *>(ep.out + at) = o.raw;
-                    if (MODE == NS_UPDATE) {
-                        gdb_vec8<__half> l;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) l.set(e, f[e] - o.get(e));
-                        *reinterpret_cast<uint4 *>(ep.out_lo + at) = l.raw;
-                    }
-                    if (SYM && tn != tm) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (col0 + j + e < N) ep.out[(size_t)z * ep.out_batch + (size_t)(col0 + j + e) * ep.out_pitch + row] = __ushort_as_half((unsigned short)((&o.raw.x)[e >> 1] >> (16 * (e & 1))));
-                        }
-                    }
-                }
-                __syncwarp();   // (the next load from tensor memory is the whole warp's)
-            }
+        if (ok && live) {
+            uint32_t v0[32], v1[32];
+            tmem_ld_32x32b_x32_nowait(tmem_base + ((uint32_t)(quad * 32) << 16), v0);
+            tmem_ld_32x32b_x32_nowait(tmem_base + ((uint32_t)(quad * 32) << 16) + 32U, v1);
+            tmem_ld_wait();
+            ns_finish_piece<MODE, TOUT>(maps, sh, st, v0, v1, row0, n0, z, tn / 2U != tm, lane);
         }
+        if (lane == 0) bulk_wait_all();
     }
+    __syncwarp();
     tcgen05_fence_before();
     __syncthreads();
     if (warp == 1) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)NS_BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)NS1_BN) : "memory");
     }
 }
 
+// ---- a pair of CTAs, 256 x 256 tiles, persistent: tiles to fill the GPU. The roles and the two accumulators are those of
+// gemm_tcgen05_pair.cu: each CTA fetches its own halves of the operands, the leader issues the products for both, the epilogue
+// of one tile runs under the products of the next. ----
+constexpr int NS2_BN = 256, NS2_STAGES = 5, NS2_WARPS = 8;
+constexpr int NS2_STAGE_BYTES = (BM + NS2_BN / 2) * BK * 2;
+constexpr int NS2_SMEM = NS2_STAGES * NS2_STAGE_BYTES + NS2_WARPS * 8192 + 256 + 1024;
+
 template <bool A_MN, bool B_MN, int MODE, typename TOUT>
-gd_status product(gd_backend *be, const CUtensorMap &ma, const CUtensorMap &mb, const ns_epilogue &ep, uint32_t M, uint32_t N, uint32_t K, uint32_t batch)
+__global__ void __launch_bounds__(32 * (2 + NS2_WARPS), 1)
+ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err_flag)
 {
-    auto kern = ns_product_kernel<A_MN, B_MN, MODE, TOUT>;
+    constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
+    unsigned char *staging = smem + NS2_STAGES * NS2_STAGE_BYTES;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + NS2_WARPS * 8192);
+    // full, empty, accumulator full [2], accumulator empty [2], inputs of the epilogue warps
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS2_STAGES + 4 + NS2_WARPS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+    const uint32_t n_iters = (sh.K + BK - 1) / BK;
+    const uint32_t per = SYM ? sh.tiles_n * (sh.tiles_n + 1U) / 2U : sh.tiles_m * sh.tiles_n, units = per * sh.batch;
+    auto tile_of = [&](uint32_t u, uint32_t &z, uint32_t &tm, uint32_t &tn) {
+        z = u / per;
+        u -= z * per;
+        if (SYM) {
+            for (tm = 0; u >= sh.tiles_n - tm; ++tm) u -= sh.tiles_n - tm;
+            tn = tm + u;
+        } else {
+            tm = u / sh.tiles_n;
+            tn = u - tm * sh.tiles_n;
+        }
+    };
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[NS2_STAGES]);
+    const uint32_t tfull0 = smem_u32(&bars[2 * NS2_STAGES]), tempty0 = smem_u32(&bars[2 * NS2_STAGES + 2]);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2 * NS2_STAGES + 2; ++s) mbar_init(full0 + 8 * s, 1);
+        for (int b = 0; b < 2; ++b) mbar_init(tempty0 + 8 * b, 2 * NS2_WARPS);   // the epilogue warps of both CTAs
+        for (int w = 0; w < NS2_WARPS; ++w) mbar_init(smem_u32(&bars[2 * NS2_STAGES + 4 + w]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * NS2_BN)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    cluster_sync_all();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    gdb_pdl_sync();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t full_leader = mapa_shared(full0, 0);
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t u = cluster_id; u < units && ok; u += n_clusters) {
+                uint32_t z, tm, tn;
+                tile_of(u, z, tm, tn);
+                const int am = (int)(tm * 2 * BM + rank * BM), bn = (int)(tn * NS2_BN + rank * (NS2_BN / 2));
+                for (uint32_t kb = 0; kb < n_iters; ++kb, ++it) {
+                    const uint32_t s = it % NS2_STAGES, ph = (it / NS2_STAGES) & 1U;
+                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1U)) {
+                        atomicExch(err_flag, 711);
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * NS2_STAGE_BYTES);
+                    const uint32_t a_dst = smem_u32(smem + s * NS2_STAGE_BYTES), b_dst = a_dst + BM * BK * 2, bar = full_leader + 8 * s;
+                    const int k0 = (int)(kb * BK);
+                    if (A_MN) {
+                        tma_load_3d_pair(a_dst, &maps.a, am, k0, (int)z, bar);
+                        tma_load_3d_pair(a_dst + BK * 128, &maps.a, am + 64, k0, (int)z, bar);
+                    } else {
+                        tma_load_3d_pair(a_dst, &maps.a, k0, am, (int)z, bar);
+                    }
+                    if (B_MN) {
+                        tma_load_3d_pair(b_dst, &maps.b, bn, k0, (int)z, bar);
+                        tma_load_3d_pair(b_dst + BK * 128, &maps.b, bn + 64, k0, (int)z, bar);
+                    } else {
+                        tma_load_3d_pair(b_dst, &maps.b, k0, bn, (int)z, bar);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t IDESC = (1U << 4) | ((A_MN ? 1U : 0U) << 15) | ((B_MN ? 1U : 0U) << 16) | ((uint32_t)(NS2_BN >> 3) << 17) | ((uint32_t)((2 * BM) >> 4) << 24);
+            uint32_t it = 0, idx = 0;
+            bool ok = true;
+            for (uint32_t u = cluster_id; u < units && ok; u += n_clusters, ++idx) {
+                const uint32_t buf = idx & 1U;
+                if (!mbar_wait(tempty0 + 8 * buf, ((idx >> 1) & 1U) ^ 1U)) {
+                    atomicExch(err_flag, 712);
+                    break;
+                }
+                tcgen05_fence_after();
+                const uint32_t d_tmem = tmem_base + buf * NS2_BN;
+                for (uint32_t kb = 0; kb < n_iters; ++kb, ++it) {
+                    const uint32_t s = it % NS2_STAGES, ph = (it / NS2_STAGES) & 1U;
+                    if (!mbar_wait(full0 + 8 * s, ph)) {
+                        atomicExch(err_flag, 713);
+                        ok = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+                    const uint32_t a_base = smem_u32(smem + s * NS2_STAGE_BYTES), b_base = a_base + BM * BK * 2;
+#pragma unroll
+                    for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                        const uint64_t adesc = A_MN ? make_smem_desc(a_base + kk * 2048, BK * 128, 1024) : make_smem_desc(a_base + kk * 32, 16, 1024);
+                        const uint64_t bdesc = B_MN ? make_smem_desc(b_base + kk * 2048, BK * 128, 1024) : make_smem_desc(b_base + kk * 32, 16, 1024);
+                        tcgen05_mma_f16_pair(d_tmem, adesc, bdesc, IDESC, (kb != 0 || kk != 0) ? 1U : 0U);
+                    }
+                    tcgen05_commit_pair(empty0 + 8 * s, 3);
+                }
+                if (ok) tcgen05_commit_pair(tfull0 + 8 * buf, 3);
+            }
+        }
+    } else {
+        // warps w and w + 4 share a tensor-memory quadrant and take two of the tile's four 64-column pieces each
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        unsigned char *st = staging + (warp - 2) * 8192;
+        const uint32_t in_bar = smem_u32(&bars[2 * NS2_STAGES + 4 + (warp - 2)]), tempty_leader = mapa_shared(tempty0, 0);
+        uint32_t idx = 0, in_phase = 0;
+        auto fetch = [&](uint32_t u, int c) {
+            if (u >= units) return;
+            uint32_t z, tm, tn;
+            tile_of(u, z, tm, tn);
+            const uint32_t row0 = tm * 2 * BM + rank * BM + quad * 32, col0 = tn * NS2_BN + c * 64;
+            if (row0 < sh.M && col0 < sh.N) ns_fetch_piece<MODE>(maps, st, in_bar, row0, col0, z);
+        };
+        if (MODE != NS_GRAM && lane == 0) fetch(cluster_id, half * 2);
+        bool ok = true;
+        for (uint32_t u = cluster_id; u < units && ok; u += n_clusters, ++idx) {
+            uint32_t z, tm, tn;
+            tile_of(u, z, tm, tn);
+            const uint32_t buf = idx & 1U;
+            ok = __all_sync(0xffffffffU, mbar_wait(tfull0 + 8 * buf, (idx >> 1) & 1U));
+            if (!ok) {
+                if (lane == 0) atomicExch(err_flag, 714);
+                break;
+            }
+            tcgen05_fence_after();
+            const uint32_t row0 = tm * 2 * BM + rank * BM + quad * 32, tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + buf * NS2_BN;
+#pragma unroll 1
+            for (int c = half * 2; c < half * 2 + 2; ++c) {
+                const uint32_t col0 = tn * NS2_BN + c * 64;
+                const bool live = row0 < sh.M && col0 < sh.N;
+                uint32_t v0[32], v1[32];
+                tmem_ld_32x32b_x32_nowait(tbase + c * 64, v0);
+                tmem_ld_32x32b_x32_nowait(tbase + c * 64 + 32, v1);
+                tmem_ld_wait();
+                if (c == half * 2 + 1) {
+                    // the accumulator has been copied out
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
+                }
+                if (live && MODE != NS_GRAM) {
+                    ok = __all_sync(0xffffffffU, mbar_wait(in_bar, in_phase++ & 1U));
+                    if (!ok) {
+                        if (lane == 0) atomicExch(err_flag, 715);
+                        break;
+                    }
+                }
+                if (live) {
+                    if (MODE == NS_GRAM) {
+                        if (lane == 0) bulk_wait_group_read<0>();
+                        __syncwarp();
+                    }
+                    ns_finish_piece<MODE, TOUT>(maps, sh, st, v0, v1, row0, col0, z, tn != tm, lane);
+                }
+                if (MODE != NS_GRAM && lane == 0) {
+                    bulk_wait_group_read<0>();
+                    if (c == half * 2) fetch(u, c + 1); else fetch(u + n_clusters, c - 1);
+                }
+                __syncwarp();
+            }
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    cluster_sync_all();   // neither CTA releases tensor memory while its peer may still use it
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * NS2_BN)) : "memory");
+    }
+}
+
+// [batch, rows, cols] of 16-bit elements, boxes of box_rows x box_cols; `swizzle`: 128 bytes, else dense rows
+bool ns_map(CUtensorMap *m, uint32_t dtype, const void *base, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows, uint32_t box_cols, bool swizzle)
+{
+    encode_tiled_fn fn = get_encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {cols, rows, batch}, strides[2] = {pitch * 2U, rows * pitch * 2U};
+    const cuuint32_t box[3] = {box_cols, box_rows, 1}, estr[3] = {1, 1, 1};
+    return fn(m, dtype == GDB_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct ns_tensor {       // a matrix of the scratch, as an operand and in the epilogue
+    __half *p;
+    uint64_t rows, cols, pitch;
+};
+bool ns_operand(CUtensorMap *m, const ns_tensor &t, uint64_t batch, bool mn, uint32_t tile)
+{
+    return mn ? ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, BK, 64, true) : ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, tile, BK, true);
+}
+bool ns_pieces(CUtensorMap *m, const ns_tensor &t, uint64_t batch) { return ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, 32, 64, true); }
+
+template <bool A_MN, bool B_MN, int MODE, typename TOUT>
+gd_status ns_launch_single(gd_backend *be, const ns_maps &maps, const ns_shape &sh, uint32_t tiles)
+{
+    // UPDATE and LAST have more tiles than SMs as a rule and run two CTAs per SM, the others one with a deeper ring
+    constexpr int STAGES = MODE == NS_GRAM || MODE == NS_POLY ? 6 : 3, SMEM = ns1_smem<STAGES>();
+    auto kern = ns_single_kernel<A_MN, B_MN, MODE, TOUT, STAGES>;
     static bool ready = false;
     if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return gdb_fail(be, e, "orthogonalize smem attribute");
         ready = true;
     }
-    const uint32_t tiles_m = (M + BM - 1) / BM, tiles_n = (N + NS_BN - 1) / NS_BN;
-    const uint32_t tiles = MODE == NS_GRAM || MODE == NS_POLY ? tiles_n * (tiles_n + 1) / 2 : tiles_m * tiles_n;
-    gdb_launch(kern, dim3(tiles, batch), 192, NS_SMEM, be->stream, ma, mb, ep, M, N, K, tiles_n, be->err_flag);
+    gdb_launch(kern, dim3(tiles, sh.batch), 192, SMEM, be->stream, maps, sh, be->err_flag);
     return gdb_launched(be, "orthogonalize product");
+}
+
+template <bool A_MN, bool B_MN, int MODE, typename TOUT>
+gd_status ns_launch_pair(gd_backend *be, const ns_maps &maps, const ns_shape &sh, uint32_t units)
+{
+    auto kern = ns_pair_kernel<A_MN, B_MN, MODE, TOUT>;
+    static bool ready = false;
+    if (!ready) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS2_SMEM);
+        if (e != cudaSuccess) return gdb_fail(be, e, "orthogonalize smem attribute");
+        ready = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    const uint32_t most = (uint32_t)be->sm_count / 2U;
+    cfg.gridDim = dim3(2U * (units < most ? units : most));
+    cfg.blockDim = dim3(32 * (2 + NS2_WARPS));
+    cfg.dynamicSmemBytes = NS2_SMEM;
+    cfg.stream = be->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps, sh, be->err_flag);
+    if (e != cudaSuccess) {
+        be->launches += 1U;
+        return gdb_fail(be, e, "orthogonalize product");
+    }
+    return gdb_launched(be, "orthogonalize product");
+}
+
+// One product of a step: operands xa, xb, epilogue tensors as the mode needs them.
+template <bool A_MN, bool B_MN, int MODE, typename TOUT = __half>
+gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, const ns_tensor *in, const ns_tensor *lo, const ns_tensor *out, void *final_out, ns_shape sh)
+{
+    constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    const uint32_t p_m = (sh.M + 255U) / 256U, p_n = (sh.N + 255U) / 256U, s_m = (sh.M + 127U) / 128U, s_n = (sh.N + 63U) / 64U;
+    uint32_t singles = s_m * s_n;
+    const uint32_t pairs = (SYM ? p_n * (p_n + 1U) / 2U : p_m * p_n) * sh.batch;
+    if (SYM) {
+        singles = 0;
+        for (uint32_t i = 0; 2U * i < s_n; ++i) singles += s_n - 2U * i;
+    }
+    // Both kernels wait for their operands: a k step of 64 takes a pair's CTA 32 KB, a single CTA 24 KB at some 55 bytes per cycle and
+    // SM, so rounds of tiles count 4 : 3.
+    const uint64_t sms = (uint64_t)be->sm_count, clusters = sms / 2U;
+    const bool pair = 4U * ((pairs + clusters - 1U) / clusters) <= 3U * (((uint64_t)singles * sh.batch + sms - 1U) / sms);
+    sh.tiles_m = pair ? p_m : s_m;
+    sh.tiles_n = pair ? p_n : s_n;
+    ns_maps maps;
+    bool ok = ns_operand(&maps.a, xa, sh.batch, A_MN, 128) && ns_operand(&maps.b, xb, sh.batch, B_MN, pair ? 128 : 64);
+    maps.in = maps.lo = maps.out = maps.mirror = maps.a;   // (those that a mode does not use)
+    if (in != nullptr) ok = ok && ns_pieces(&maps.in, *in, sh.batch);
+    if (lo != nullptr) ok = ok && ns_pieces(&maps.lo, *lo, sh.batch);
+    if (out != nullptr) ok = ok && ns_pieces(&maps.out, *out, sh.batch);
+    if (SYM) ok = ok && ns_map(&maps.mirror, GDB_DTYPE_F16, out->p, sh.batch, out->rows, out->cols, out->pitch, 64, 32, false);
+    if (MODE == NS_LAST) {
+        sh.plain = nullptr;
+        if (sh.N % 8U != 0U || (uintptr_t)final_out % 16U != 0U) sh.plain = final_out;
+        else ok = ok && ns_map(&maps.out, std::is_same<TOUT, __half>::value ? GDB_DTYPE_F16 : GDB_DTYPE_BF16, final_out, sh.batch, sh.M, sh.N, sh.N, 32, 64, true);
+    }
+    if (!ok) return GD_ERR_UNSUPPORTED;
+    return pair ? ns_launch_pair<A_MN, B_MN, MODE, TOUT>(be, maps, sh, pairs) : ns_launch_single<A_MN, B_MN, MODE, TOUT>(be, maps, sh, singles);
 }
 
 // Where the parts of the scratch lie: the iterate's high halves (two, used in turn), its low halves, A, P, the sums of squares.
@@ -261,7 +611,8 @@ bool ns_plan(const gdb200_orthogonalize_args *a, ns_layout *l)
     l->small = a->rows < a->cols ? a->rows : a->cols;
     l->pitch = (a->cols + 7U) & ~(uint64_t)7U;
     l->small_pitch = (l->small + 7U) & ~(size_t)7U;
-    if (l->pitch != 0U && a->rows * l->pitch > (SIZE_MAX >> 8) / (a->batch + 1U)) return false;
+    // (the products count tiles of a batch in 32 bits)
+    if ((a->rows / 128U + 1U) * (a->cols / 64U + 1U) * (a->batch + 1U) > 0x7fffffffU) return false;
     const size_t x = (a->batch * a->rows * l->pitch * 2U + 255U) & ~(size_t)255U, s = (a->batch * l->small * l->small_pitch * 2U + 255U) & ~(size_t)255U;
     l->hi[0] = 0U;
     l->hi[1] = x;
@@ -277,12 +628,15 @@ template <typename T>
 gd_status first_iterate(gd_backend *be, const void *g, double *partial, __half *hi, __half *lo, const gdb200_orthogonalize_args *a, size_t pitch)
 {
     const size_t count = a->rows * a->cols;
-    unsigned parts = (unsigned)((count + 8191U) / 8192U < NS_NORM_BLOCKS ? (count + 8191U) / 8192U : NS_NORM_BLOCKS);
-    gdb_launch(ns_norm_kernel<T>, dim3(parts, (unsigned)a->batch), 256, 0, be->stream, (const T *)g, partial, count);
+    const bool even = (uintptr_t)g % 16U == 0U;
+    const size_t want = (count + 4095U) / 4096U, most = (size_t)be->sm_count * 8U / a->batch + 1U;
+    size_t parts = want < most ? want : most;
+    if (parts > NS_NORM_BLOCKS) parts = NS_NORM_BLOCKS;
+    gdb_launch(ns_norm_kernel<T>, dim3((unsigned)parts, (unsigned)a->batch), 256, 0, be->stream, (const T *)g, partial, count, even && (a->batch == 1U || count % 8U == 0U));
     gd_status st = gdb_launched(be, "orthogonalize norm");
     if (st != GD_OK) return st;
-    gdb_launch(ns_split_kernel<T>, dim3(gdb_grid_for(count, 1024, be, 4), (unsigned)a->batch), 256, 0, be->stream, (const T *)g, (const double *)partial, (int)parts, hi, lo,
-               (size_t)a->rows, (size_t)a->cols, pitch, a->eps);
+    gdb_launch(ns_split_kernel<T>, dim3(gdb_grid_for(a->rows * (pitch / 8U), 256, be, 8), (unsigned)a->batch), 256, 0, be->stream, (const T *)g, (const double *)partial, (int)parts, hi, lo,
+               (unsigned)a->rows, (unsigned)a->cols, (unsigned)(pitch / 8U), a->eps, even && a->cols % 8U == 0U);
     return gdb_launched(be, "orthogonalize split");
 }
 
@@ -316,58 +670,41 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
     if (count == 0U) {
         return GD_OK;
     }
-    const uint32_t rows = (uint32_t)a->rows, cols = (uint32_t)a->cols, m = (uint32_t)l.small, batch = (uint32_t)a->batch;
+    const uint64_t rows = a->rows, cols = a->cols, m = l.small;
     const bool tall = rows > cols;
-    __half *hi[2] = {(__half *)(sp + l.hi[0]), (__half *)(sp + l.hi[1])}, *lo = (__half *)(sp + l.lo), *gram = (__half *)(sp + l.gram), *poly = (__half *)(sp + l.poly);
-    // operand tiles: [k contiguous] boxes of 128 rows, [k strided] boxes of 64 columns
-    CUtensorMap xk[2], xm[2], gk, pk;
-    bool ok = make_tmap_batched(&gk, GDB_DTYPE_F16, gram, batch, m, m, l.small_pitch * 2U, m * l.small_pitch * 2U, BK, 128) &&
-              make_tmap_batched(&pk, GDB_DTYPE_F16, poly, batch, m, m, l.small_pitch * 2U, m * l.small_pitch * 2U, BK, 128);
-    for (int i = 0; i < 2; ++i) {
-        ok = ok && make_tmap_batched(&xk[i], GDB_DTYPE_F16, hi[i], batch, rows, cols, l.pitch * 2U, rows * l.pitch * 2U, BK, 128) &&
-             make_tmap_batched(&xm[i], GDB_DTYPE_F16, hi[i], batch, rows, cols, l.pitch * 2U, rows * l.pitch * 2U, 64, BK);
-    }
-    if (!ok) {
-        return GD_ERR_UNSUPPORTED;
-    }
+    const ns_tensor hi[2] = {{(__half *)(sp + l.hi[0]), rows, cols, l.pitch}, {(__half *)(sp + l.hi[1]), rows, cols, l.pitch}};
+    const ns_tensor lo = {(__half *)(sp + l.lo), rows, cols, l.pitch}, gram = {(__half *)(sp + l.gram), m, m, l.small_pitch}, poly = {(__half *)(sp + l.poly), m, m, l.small_pitch};
     double *norm = (double *)(sp + l.norm);
-    gd_status st = x->dtype == GDB_DTYPE_F16    ? first_iterate<__half>(be, xp, norm, hi[0], lo, a, l.pitch)
-                   : x->dtype == GDB_DTYPE_BF16 ? first_iterate<__nv_bfloat16>(be, xp, norm, hi[0], lo, a, l.pitch)
-                                                : first_iterate<float>(be, xp, norm, hi[0], lo, a, l.pitch);
-    ns_epilogue square = {};
-    square.out_batch = square.in_batch = m * l.small_pitch;
-    square.out_pitch = square.in_pitch = l.small_pitch;
+    gd_status st = x->dtype == GDB_DTYPE_F16    ? first_iterate<__half>(be, xp, norm, hi[0].p, lo.p, a, l.pitch)
+                   : x->dtype == GDB_DTYPE_BF16 ? first_iterate<__nv_bfloat16>(be, xp, norm, hi[0].p, lo.p, a, l.pitch)
+                                                : first_iterate<float>(be, xp, norm, hi[0].p, lo.p, a, l.pitch);
     for (uint32_t k = 0; k < a->steps && st == GD_OK; ++k) {
-        const int cur = (int)(k & 1U);
-        ns_epilogue e = square;
-        e.out = gram;
-        e.alpha = NS_DOWN * NS_DOWN;
-        st = tall ? product<true, true, NS_GRAM, __half>(be, xm[cur], xm[cur], e, m, m, rows, batch) : product<false, false, NS_GRAM, __half>(be, xk[cur], xk[cur], e, m, m, cols, batch);
+        const ns_tensor &x0 = hi[k & 1U], &x1 = hi[(k & 1U) ^ 1U];
+        ns_shape square = {};
+        square.M = square.N = (uint32_t)m;
+        square.K = (uint32_t)(tall ? rows : cols);
+        square.batch = (uint32_t)a->batch;
+        square.alpha = NS_DOWN * NS_DOWN;
+        st = tall ? ns_product<true, true, NS_GRAM>(be, x0, x0, nullptr, nullptr, &gram, nullptr, square)
+                  : ns_product<false, false, NS_GRAM>(be, x0, x0, nullptr, nullptr, &gram, nullptr, square);
         if (st != GD_OK) break;
-        e.in = gram;
-        e.out = poly;
-        e.alpha = a->c;
-        e.beta = a->b;
-        st = product<false, false, NS_POLY, __half>(be, gk, gk, e, m, m, m, batch);
+        square.K = (uint32_t)m;
+        square.alpha = a->c;
+        square.beta = a->b;
+        st = ns_product<false, false, NS_POLY>(be, gram, gram, &gram, nullptr, &poly, nullptr, square);
         if (st != GD_OK) break;
-        e = ns_epilogue();
-        e.in = hi[cur];
-        e.in_lo = lo;
-        e.in_batch = e.out_batch = rows * l.pitch;
-        e.in_pitch = e.out_pitch = l.pitch;
-        e.alpha = 1.0f;
-        e.beta = a->a;
+        ns_shape full = square;
+        full.M = (uint32_t)rows;
+        full.N = (uint32_t)cols;
+        full.alpha = 1.0f;
+        full.beta = a->a;
         if (k + 1U < a->steps) {
-            e.out = hi[cur ^ 1];
-            e.out_lo = lo;
-            st = tall ? product<false, false, NS_UPDATE, __half>(be, xk[cur], pk, e, rows, cols, m, batch) : product<false, true, NS_UPDATE, __half>(be, pk, xm[cur], e, rows, cols, m, batch);
+            st = tall ? ns_product<false, false, NS_UPDATE>(be, x0, poly, &x0, &lo, &x1, nullptr, full) : ns_product<false, true, NS_UPDATE>(be, poly, x0, &x0, &lo, &x1, nullptr, full);
+        } else if (out->dtype == GDB_DTYPE_F16) {
+            st = tall ? ns_product<false, false, NS_LAST, __half>(be, x0, poly, &x0, &lo, nullptr, op, full) : ns_product<false, true, NS_LAST, __half>(be, poly, x0, &x0, &lo, nullptr, op, full);
         } else {
-            e.final_out = op;
-            e.out_batch = (size_t)rows * cols;
-            e.out_pitch = cols;
-#define GO(T) (tall ? product<false, false, NS_LAST, T>(be, xk[cur], pk, e, rows, cols, m, batch) : product<false, true, NS_LAST, T>(be, pk, xm[cur], e, rows, cols, m, batch))
-            st = out->dtype == GDB_DTYPE_F16 ? GO(__half) : GO(__nv_bfloat16);
-#undef GO
+            st = tall ? ns_product<false, false, NS_LAST, __nv_bfloat16>(be, x0, poly, &x0, &lo, nullptr, op, full)
+                      : ns_product<false, true, NS_LAST, __nv_bfloat16>(be, poly, x0, &x0, &lo, nullptr, op, full);
         }
     }
     return st;
