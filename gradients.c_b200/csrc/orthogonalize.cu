@@ -106,98 +106,142 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
 // either order of the product's operands does.
 enum { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
 
-// What the epilogue reads and writes, in tiles of 32 x 64 (a warp's rows, 128 bytes a row, swizzled).
 struct ns_maps {
     CUtensorMap a, b;        // operands
-    CUtensorMap in, lo;      // POLY: A; UPDATE, LAST: hi, and lo in and out
-    CUtensorMap out;         // A, P, the next hi, or the caller's tensor
-    CUtensorMap mirror;      // GRAM, POLY: out again, in tiles of 64 x 32 without a swizzle
 };
+// What the epilogue reads and writes, [batch, M, pitch] with rows of a multiple of 32 bytes (LAST's output: dense, any alignment).
 struct ns_shape {
-    uint32_t M, N, K, tiles_m, tiles_n, batch;
+    uint32_t M, N, K, tiles_m, tiles_n, batch, pitch;
     float alpha, beta;
-    void *plain;             // LAST into a tensor that TMA cannot address (odd rows): its address, else NULL
+    const __half *in;        // POLY: A; UPDATE, LAST: hi
+    __half *lo;              // UPDATE: in and out; LAST: in
+    void *out;               // A, P, the next hi, or the caller's tensor
+    bool wide_out;           // LAST: the caller's rows take 32-byte stores
 };
 
-// One warp's 32 x 64 piece of the result: v0 / v1 hold its accumulators (lane = row). `st` is the warp's staging, two 4 KB tiles: the
-// inputs arrived there and the results leave from there. Mirrored pieces are written transposed into the second tile.
-template <int MODE, typename TOUT>
-__device__ __forceinline__ void ns_finish_piece(const ns_maps &maps, const ns_shape &sh, unsigned char *st, const uint32_t (&v0)[32], const uint32_t (&v1)[32], uint32_t row0,
-                                                uint32_t col0, uint32_t z, bool mirror, int lane)
+// One warp's 32 x 64 piece of the result, a lane per row. Inputs and results go between registers and memory directly, 32 bytes a lane
+// and access: the products alone take 125 of the 128 bytes that shared memory moves in a cycle (operands written, read, and read by
+// the peer), so staging tiles there for TMA costs the products their time (four 5632 x 2048 matrices: a step's UPDATE 170 us with staged
+// tiles, 128 us without any epilogue traffic).
+struct ns_row {
+    uint32_t w[32];          // 64 elements
+};
+__device__ __forceinline__ void ns_load_row(ns_row &r, const __half *p, uint32_t left)
 {
-    unsigned char *r0 = st + lane * 128, *r1 = r0 + 4096;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int chunk = (j ^ (lane & 7)) << 4;
-        float f[8];
+    for (int k = 0; k < 4; ++k) {
+        uint32_t *w = r.w + 8 * k;
+        if (16U * k < left) {
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p + 16 * k)
+                         : "memory");
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = sh.alpha * __uint_as_float(j < 4 ? v0[(j & 3) * 8 + e] : v1[(j & 3) * 8 + e]);
-        if (MODE != NS_GRAM) {
-            gdb_vec8<__half> a, l;
-            a.raw = *reinterpret_cast<const uint4 *>(r0 + chunk);
-            if (MODE != NS_POLY) l.raw = *reinterpret_cast<const uint4 *>(r1 + chunk);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = fmaf(sh.beta, MODE == NS_POLY ? a.get(e) : a.get(e) + l.get(e), f[e]);
+            for (int e = 0; e < 8; ++e) w[e] = 0U;
         }
-        if (MODE == NS_LAST) {
-            uint4 o;
-            o.x = half_pack<TOUT>::pack(f[0] * NS_DOWN, f[1] * NS_DOWN);
-            o.y = half_pack<TOUT>::pack(f[2] * NS_DOWN, f[3] * NS_DOWN);
-            o.z = half_pack<TOUT>::pack(f[4] * NS_DOWN, f[5] * NS_DOWN);
-            o.w = half_pack<TOUT>::pack(f[6] * NS_DOWN, f[7] * NS_DOWN);
-            *reinterpret_cast<uint4 *>(r0 + chunk) = o;
-            continue;
-        }
-        gdb_vec8<__half> o;
-        o.raw = make_uint4(half_pack<__half>::pack(f[0], f[1]), half_pack<__half>::pack(f[2], f[3]), half_pack<__half>::pack(f[4], f[5]), half_pack<__half>::pack(f[6], f[7]));
-        *reinterpret_cast<uint4 *>(r0 + chunk) = o.raw;
-        if (MODE == NS_UPDATE) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] -= o.get(e);
-            *reinterpret_cast<uint4 *>(r1 + chunk) = make_uint4(half_pack<__half>::pack(f[0], f[1]), half_pack<__half>::pack(f[2], f[3]), half_pack<__half>::pack(f[4], f[5]),
-                                                                half_pack<__half>::pack(f[6], f[7]));
-        } else if (mirror) {
-            // row j * 8 + e of the transposed piece, 64 bytes: the lanes' elements side by side
-            unsigned short *t = reinterpret_cast<unsigned short *>(st + 4096) + j * 8 * 32 + lane;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e * 32] = (unsigned short)((&o.raw.x)[e >> 1] >> (16 * (e & 1)));
-        }
-    }
-    if (MODE == NS_LAST && sh.plain != nullptr) {
-        __syncwarp();
-        unsigned short *out = reinterpret_cast<unsigned short *>(sh.plain) + ((size_t)z * sh.M + row0) * sh.N + col0;
-        const uint32_t rows = min(32U, sh.M - row0), cols = min(64U, sh.N - col0);
-        for (uint32_t r = 0; r < rows; ++r) {
-#pragma unroll
-            for (uint32_t c = lane; c < 64U; c += 32U) {
-                if (c < cols) out[(size_t)r * sh.N + c] = *reinterpret_cast<const unsigned short *>(st + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
-            }
-        }
-        fence_proxy_async_smem();   // the next inputs arrive here
-        __syncwarp();
-        return;
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-        tma_store_3d(&maps.out, (int)col0, (int)row0, (int)z, smem_u32(st));
-        if (MODE == NS_UPDATE) tma_store_3d(&maps.lo, (int)col0, (int)row0, (int)z, smem_u32(st + 4096));
-        if ((MODE == NS_GRAM || MODE == NS_POLY) && mirror) tma_store_3d(&maps.mirror, (int)row0, (int)col0, (int)z, smem_u32(st + 4096));
-        bulk_commit_group();
     }
 }
-// the inputs of a piece on their way to the warp's staging (one lane)
-template <int MODE>
-__device__ __forceinline__ void ns_fetch_piece(const ns_maps &maps, unsigned char *st, uint32_t bar, uint32_t row0, uint32_t col0, uint32_t z)
+__device__ __forceinline__ void ns_store_row(void *base, const uint32_t *w, uint32_t left)
 {
-    mbar_expect_tx(bar, MODE == NS_POLY ? 4096 : 8192);
-    tma_load_3d(smem_u32(st), &maps.in, (int)col0, (int)row0, (int)z, bar);
-    if (MODE != NS_POLY) tma_load_3d(smem_u32(st + 4096), &maps.lo, (int)col0, (int)row0, (int)z, bar);
+    __half *p = reinterpret_cast<__half *>(base);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t *v = w + 8 * k;
+        if (16U * k < left) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 16 * k), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                         "r"(v[6]), "r"(v[7])
+                         : "memory");
+        }
+    }
+}
+__device__ __forceinline__ float2 ns_two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+
+// the inputs of a piece, on their way while its products are formed
+template <int MODE>
+__device__ __forceinline__ void ns_load_piece(ns_row &in, ns_row &lo, const ns_shape &sh, uint32_t row, uint32_t col0, uint32_t z)
+{
+    if (MODE == NS_GRAM) return;
+    const uint32_t left = row < sh.M && col0 < sh.N ? sh.N - col0 : 0U;
+    const size_t at = ((size_t)z * sh.M + (left != 0U ? row : 0U)) * sh.pitch + (left != 0U ? col0 : 0U);
+    ns_load_row(in, sh.in + at, left);
+    if (MODE != NS_POLY) ns_load_row(lo, sh.lo + at, left);
+}
+// v: the piece's accumulators. `stage` (4 KB, this warp's): rows that take no 32-byte stores are put together there.
+template <int MODE, typename TOUT>
+__device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row &in, ns_row &lo, uint32_t (&v)[64], uint32_t row0, uint32_t col0, uint32_t z, bool mirror,
+                                                unsigned char *stage, int lane)
+{
+    const uint32_t row = row0 + lane;
+    const bool live = row < sh.M && col0 < sh.N;
+    const uint32_t left = live ? sh.N - col0 : 0U;
+    const size_t at = ((size_t)z * sh.M + row) * sh.pitch + col0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        float f0 = sh.alpha * __uint_as_float(v[2 * e]), f1 = sh.alpha * __uint_as_float(v[2 * e + 1]);
+        if (MODE != NS_GRAM) {
+            float2 a = ns_two(in.w[e]);
+            if (MODE != NS_POLY) {
+                const float2 l = ns_two(lo.w[e]);
+                a.x += l.x;
+                a.y += l.y;
+            }
+            f0 = fmaf(sh.beta, a.x, f0);
+            f1 = fmaf(sh.beta, a.y, f1);
+        }
+        if (MODE == NS_LAST) {
+            v[e] = half_pack<TOUT>::pack(f0 * NS_DOWN, f1 * NS_DOWN);
+        } else {
+            v[e] = half_pack<__half>::pack(f0, f1);
+            if (MODE == NS_UPDATE) {
+                const float2 r = ns_two(v[e]);
+                lo.w[e] = half_pack<__half>::pack(f0 - r.x, f1 - r.y);
+            }
+        }
+    }
+    if (MODE == NS_LAST) {
+        unsigned short *out = reinterpret_cast<unsigned short *>(sh.out) + ((size_t)z * sh.M + row0) * sh.N + col0;
+        if (sh.wide_out) {
+            ns_store_row(out + (size_t)lane * sh.N, v, left);
+        } else {
+            const uint32_t rows = row0 < sh.M ? min(32U, sh.M - row0) : 0U, cols = col0 < sh.N ? min(64U, sh.N - col0) : 0U;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            __syncwarp();
+            for (uint32_t r = 0; r < rows; ++r) {
+#pragma unroll
+                for (uint32_t c = lane; c < 64U; c += 32U) {
+                    if (c < cols) out[(size_t)r * sh.N + c] = *reinterpret_cast<const unsigned short *>(stage + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+                }
+            }
+            __syncwarp();
+        }
+        return;
+    }
+    __half *out = reinterpret_cast<__half *>(sh.out);
+    ns_store_row(out + at, v, left);
+    if (MODE == NS_UPDATE) {
+        ns_store_row(sh.lo + at, lo.w, left);
+    } else if (mirror && live) {
+        // the transposed piece: the lanes' elements of a column lie side by side
+        unsigned short *t = reinterpret_cast<unsigned short *>(out) + ((size_t)z * sh.M + col0) * sh.pitch + row;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+            if ((uint32_t)e < left) t[(size_t)e * sh.pitch] = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+}
+__device__ __forceinline__ void ns_accumulators(uint32_t (&v)[64], uint32_t taddr)
+{
+    uint32_t(&a)[32] = *reinterpret_cast<uint32_t(*)[32]>(v), (&b)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 32);
+    tmem_ld_32x32b_x32_nowait(taddr, a);
+    tmem_ld_32x32b_x32_nowait(taddr + 32U, b);
+    tmem_ld_wait();
 }
 
 // ---- one CTA, one 128 x 64 tile: small matrices, where the number of SMs at work counts ----
 constexpr int NS1_BN = 64, NS1_STAGE_BYTES = (BM + NS1_BN) * BK * 2;
-template <int STAGES> constexpr int ns1_smem() { return STAGES * NS1_STAGE_BYTES + 4 * 8192 + 256 + 1024; }
+template <int STAGES> constexpr int ns1_smem() { return STAGES * NS1_STAGE_BYTES + 4 * 4096 + 256 + 1024; }
 
 template <bool A_MN, bool B_MN, int MODE, typename TOUT, int STAGES>
 __global__ void __launch_bounds__(192)
@@ -207,8 +251,8 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
     unsigned char *staging = smem + STAGES * NS1_STAGE_BYTES;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 4 * 8192);   // full, empty, accumulator, inputs of the four epilogue warps
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 5);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 4 * 4096);   // full, empty, accumulator
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t z = blockIdx.y;
     uint32_t tm, tn;
@@ -222,9 +266,9 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
         tn = blockIdx.x - tm * sh.tiles_n;
     }
     const uint32_t m0 = tm * BM, n0 = tn * NS1_BN, n_iters = (sh.K + BK - 1) / BK;
-    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]), accum_bar = smem_u32(&bars[2 * STAGES]), in0 = smem_u32(&bars[2 * STAGES + 1]);
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]), accum_bar = smem_u32(&bars[2 * STAGES]);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 2 * STAGES + 5; ++s) mbar_init(full0 + 8 * s, 1);
+        for (int s = 0; s < 2 * STAGES + 1; ++s) mbar_init(full0 + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -280,23 +324,17 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
         }
     } else {
         const int quad = warp & 3;
-        unsigned char *st = staging + quad * 8192;
-        const uint32_t row0 = m0 + quad * 32, bar = in0 + 8 * quad;
-        const bool live = row0 < sh.M;   // (the tile's first column always lies inside)
-        if (MODE != NS_GRAM && live && lane == 0) ns_fetch_piece<MODE>(maps, st, bar, row0, n0, z);
-        bool ok = mbar_wait(accum_bar, 0);
-        if (MODE != NS_GRAM && live) ok = mbar_wait(bar, 0) && ok;
-        ok = __all_sync(0xffffffffU, ok);
+        const uint32_t row0 = m0 + quad * 32;
+        ns_row in, lo;
+        ns_load_piece<MODE>(in, lo, sh, row0 + lane, n0, z);
+        const bool ok = __all_sync(0xffffffffU, mbar_wait(accum_bar, 0));
         if (!ok && lane == 0) atomicExch(err_flag, 703);
         tcgen05_fence_after();
-        if (ok && live) {
-            uint32_t v0[32], v1[32];
-            tmem_ld_32x32b_x32_nowait(tmem_base + ((uint32_t)(quad * 32) << 16), v0);
-            tmem_ld_32x32b_x32_nowait(tmem_base + ((uint32_t)(quad * 32) << 16) + 32U, v1);
-            tmem_ld_wait();
-            ns_finish_piece<MODE, TOUT>(maps, sh, st, v0, v1, row0, n0, z, tn / 2U != tm, lane);
+        if (ok) {
+            uint32_t v[64];
+            ns_accumulators(v, tmem_base + ((uint32_t)(quad * 32) << 16));
+            ns_finish_piece<MODE, TOUT>(sh, in, lo, v, row0, n0, z, tn / 2U != tm, staging + quad * 4096, lane);
         }
-        if (lane == 0) bulk_wait_all();
     }
     __syncwarp();
     tcgen05_fence_before();
@@ -309,9 +347,9 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
 // ---- a pair of CTAs, 256 x 256 tiles, persistent: tiles to fill the GPU. The roles and the two accumulators are those of
 // gemm_tcgen05_pair.cu: each CTA fetches its own halves of the operands, the leader issues the products for both, the epilogue
 // of one tile runs under the products of the next. ----
-constexpr int NS2_BN = 256, NS2_STAGES = 5, NS2_WARPS = 8;
+constexpr int NS2_BN = 256, NS2_STAGES = 5, NS2_WARPS = 8, NS2_STAGING = 4096;
 constexpr int NS2_STAGE_BYTES = (BM + NS2_BN / 2) * BK * 2;
-constexpr int NS2_SMEM = NS2_STAGES * NS2_STAGE_BYTES + NS2_WARPS * 8192 + 256 + 1024;
+constexpr int NS2_SMEM = NS2_STAGES * NS2_STAGE_BYTES + NS2_WARPS * NS2_STAGING + 512 + 1024;
 
 template <bool A_MN, bool B_MN, int MODE, typename TOUT>
 __global__ void __launch_bounds__(32 * (2 + NS2_WARPS), 1)
@@ -321,9 +359,9 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
     unsigned char *staging = smem + NS2_STAGES * NS2_STAGE_BYTES;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + NS2_WARPS * 8192);
-    // full, empty, accumulator full [2], accumulator empty [2], inputs of the epilogue warps
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS2_STAGES + 4 + NS2_WARPS);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + NS2_WARPS * NS2_STAGING);
+    // full, empty, accumulator full [2], accumulator empty [2]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS2_STAGES + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
     const uint32_t n_iters = (sh.K + BK - 1) / BK;
@@ -344,7 +382,6 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2 * NS2_STAGES + 2; ++s) mbar_init(full0 + 8 * s, 1);
         for (int b = 0; b < 2; ++b) mbar_init(tempty0 + 8 * b, 2 * NS2_WARPS);   // the epilogue warps of both CTAs
-        for (int w = 0; w < NS2_WARPS; ++w) mbar_init(smem_u32(&bars[2 * NS2_STAGES + 4 + w]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -427,65 +464,35 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
     } else {
         // warps w and w + 4 share a tensor-memory quadrant and take two of the tile's four 64-column pieces each
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        unsigned char *st = staging + (warp - 2) * 8192;
-        const uint32_t in_bar = smem_u32(&bars[2 * NS2_STAGES + 4 + (warp - 2)]), tempty_leader = mapa_shared(tempty0, 0);
-        uint32_t idx = 0, in_phase = 0;
-        auto fetch = [&](uint32_t u, int c) {
-            if (u >= units) return;
+        const uint32_t tempty_leader = mapa_shared(tempty0, 0);
+        uint32_t idx = 0;
+        for (uint32_t u = cluster_id; u < units; u += n_clusters, ++idx) {
             uint32_t z, tm, tn;
             tile_of(u, z, tm, tn);
-            const uint32_t row0 = tm * 2 * BM + rank * BM + quad * 32, col0 = tn * NS2_BN + c * 64;
-            if (row0 < sh.M && col0 < sh.N) ns_fetch_piece<MODE>(maps, st, in_bar, row0, col0, z);
-        };
-        if (MODE != NS_GRAM && lane == 0) fetch(cluster_id, half * 2);
-        bool ok = true;
-        for (uint32_t u = cluster_id; u < units && ok; u += n_clusters, ++idx) {
-            uint32_t z, tm, tn;
-            tile_of(u, z, tm, tn);
-            const uint32_t buf = idx & 1U;
-            ok = __all_sync(0xffffffffU, mbar_wait(tfull0 + 8 * buf, (idx >> 1) & 1U));
-            if (!ok) {
+            const uint32_t buf = idx & 1U, row0 = tm * 2 * BM + rank * BM + quad * 32, tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + buf * NS2_BN + half * 128;
+            ns_row in, lo;
+            ns_load_piece<MODE>(in, lo, sh, row0 + lane, tn * NS2_BN + half * 128, z);
+            if (!__all_sync(0xffffffffU, mbar_wait(tfull0 + 8 * buf, (idx >> 1) & 1U))) {
                 if (lane == 0) atomicExch(err_flag, 714);
                 break;
             }
             tcgen05_fence_after();
-            const uint32_t row0 = tm * 2 * BM + rank * BM + quad * 32, tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + buf * NS2_BN;
 #pragma unroll 1
-            for (int c = half * 2; c < half * 2 + 2; ++c) {
-                const uint32_t col0 = tn * NS2_BN + c * 64;
-                const bool live = row0 < sh.M && col0 < sh.N;
-                uint32_t v0[32], v1[32];
-                tmem_ld_32x32b_x32_nowait(tbase + c * 64, v0);
-                tmem_ld_32x32b_x32_nowait(tbase + c * 64 + 32, v1);
-                tmem_ld_wait();
-                if (c == half * 2 + 1) {
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t col0 = tn * NS2_BN + half * 128 + 64U * p;
+                if (p == 1) ns_load_piece<MODE>(in, lo, sh, row0 + lane, col0, z);
+                uint32_t v[64];
+                ns_accumulators(v, tbase + 64U * p);
+                if (p == 1) {
                     // the accumulator has been copied out
                     tcgen05_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
                 }
-                if (live && MODE != NS_GRAM) {
-                    ok = __all_sync(0xffffffffU, mbar_wait(in_bar, in_phase++ & 1U));
-                    if (!ok) {
-                        if (lane == 0) atomicExch(err_flag, 715);
-                        break;
-                    }
-                }
-                if (live) {
-                    if (MODE == NS_GRAM) {
-                        if (lane == 0) bulk_wait_group_read<0>();
-                        __syncwarp();
-                    }
-                    ns_finish_piece<MODE, TOUT>(maps, sh, st, v0, v1, row0, col0, z, tn != tm, lane);
-                }
-                if (MODE != NS_GRAM && lane == 0) {
-                    bulk_wait_group_read<0>();
-                    if (c == half * 2) fetch(u, c + 1); else fetch(u + n_clusters, c - 1);
-                }
+                ns_finish_piece<MODE, TOUT>(sh, in, lo, v, row0, col0, z, tn != tm, staging + (warp - 2) * NS2_STAGING, lane);
                 __syncwarp();
             }
         }
-        if (lane == 0) bulk_wait_all();
     }
     __syncwarp();
     tcgen05_fence_before();
@@ -515,7 +522,6 @@ bool ns_operand(CUtensorMap *m, const ns_tensor &t, uint64_t batch, bool mn, uin
 {
     return mn ? ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, BK, 64, true) : ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, tile, BK, true);
 }
-bool ns_pieces(CUtensorMap *m, const ns_tensor &t, uint64_t batch) { return ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, 32, 64, true); }
 
 template <bool A_MN, bool B_MN, int MODE, typename TOUT>
 gd_status ns_launch_single(gd_backend *be, const ns_maps &maps, const ns_shape &sh, uint32_t tiles)
@@ -566,9 +572,9 @@ gd_status ns_launch_pair(gd_backend *be, const ns_maps &maps, const ns_shape &sh
     return gdb_launched(be, "orthogonalize product");
 }
 
-// One product of a step: operands xa, xb, epilogue tensors as the mode needs them.
+// One product of a step: operands xa and xb; sh has what the epilogue needs.
 template <bool A_MN, bool B_MN, int MODE, typename TOUT = __half>
-gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, const ns_tensor *in, const ns_tensor *lo, const ns_tensor *out, void *final_out, ns_shape sh)
+gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, ns_shape sh)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
     const uint32_t p_m = (sh.M + 255U) / 256U, p_n = (sh.N + 255U) / 256U, s_m = (sh.M + 127U) / 128U, s_n = (sh.N + 63U) / 64U;
@@ -586,16 +592,6 @@ gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, c
     sh.tiles_n = pair ? p_n : s_n;
     ns_maps maps;
     bool ok = ns_operand(&maps.a, xa, sh.batch, A_MN, 128) && ns_operand(&maps.b, xb, sh.batch, B_MN, pair ? 128 : 64);
-    maps.in = maps.lo = maps.out = maps.mirror = maps.a;   // (those that a mode does not use)
-    if (in != nullptr) ok = ok && ns_pieces(&maps.in, *in, sh.batch);
-    if (lo != nullptr) ok = ok && ns_pieces(&maps.lo, *lo, sh.batch);
-    if (out != nullptr) ok = ok && ns_pieces(&maps.out, *out, sh.batch);
-    if (SYM) ok = ok && ns_map(&maps.mirror, GDB_DTYPE_F16, out->p, sh.batch, out->rows, out->cols, out->pitch, 64, 32, false);
-    if (MODE == NS_LAST) {
-        sh.plain = nullptr;
-        if (sh.N % 8U != 0U || (uintptr_t)final_out % 16U != 0U) sh.plain = final_out;
-        else ok = ok && ns_map(&maps.out, std::is_same<TOUT, __half>::value ? GDB_DTYPE_F16 : GDB_DTYPE_BF16, final_out, sh.batch, sh.M, sh.N, sh.N, 32, 64, true);
-    }
     if (!ok) return GD_ERR_UNSUPPORTED;
     return pair ? ns_launch_pair<A_MN, B_MN, MODE, TOUT>(be, maps, sh, pairs) : ns_launch_single<A_MN, B_MN, MODE, TOUT>(be, maps, sh, singles);
 }
@@ -609,8 +605,8 @@ bool ns_plan(const gdb200_orthogonalize_args *a, ns_layout *l)
 {
     if (a == NULL || a->rows >= (1U << 24) || a->cols >= (1U << 24) || a->batch > 65535U) return false;
     l->small = a->rows < a->cols ? a->rows : a->cols;
-    l->pitch = (a->cols + 7U) & ~(uint64_t)7U;
-    l->small_pitch = (l->small + 7U) & ~(size_t)7U;
+    l->pitch = (a->cols + 15U) & ~(uint64_t)15U;   // (32 bytes: one access of the epilogue)
+    l->small_pitch = (l->small + 15U) & ~(size_t)15U;
     // (the products count tiles of a batch in 32 bits)
     if ((a->rows / 128U + 1U) * (a->cols / 64U + 1U) * (a->batch + 1U) > 0x7fffffffU) return false;
     const size_t x = (a->batch * a->rows * l->pitch * 2U + 255U) & ~(size_t)255U, s = (a->batch * l->small * l->small_pitch * 2U + 255U) & ~(size_t)255U;
@@ -685,26 +681,33 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
         square.K = (uint32_t)(tall ? rows : cols);
         square.batch = (uint32_t)a->batch;
         square.alpha = NS_DOWN * NS_DOWN;
-        st = tall ? ns_product<true, true, NS_GRAM>(be, x0, x0, nullptr, nullptr, &gram, nullptr, square)
-                  : ns_product<false, false, NS_GRAM>(be, x0, x0, nullptr, nullptr, &gram, nullptr, square);
+        square.pitch = (uint32_t)l.small_pitch;
+        square.out = gram.p;
+        st = tall ? ns_product<true, true, NS_GRAM>(be, x0, x0, square) : ns_product<false, false, NS_GRAM>(be, x0, x0, square);
         if (st != GD_OK) break;
         square.K = (uint32_t)m;
         square.alpha = a->c;
         square.beta = a->b;
-        st = ns_product<false, false, NS_POLY>(be, gram, gram, &gram, nullptr, &poly, nullptr, square);
+        square.in = gram.p;
+        square.out = poly.p;
+        st = ns_product<false, false, NS_POLY>(be, gram, gram, square);
         if (st != GD_OK) break;
         ns_shape full = square;
         full.M = (uint32_t)rows;
         full.N = (uint32_t)cols;
+        full.pitch = (uint32_t)l.pitch;
         full.alpha = 1.0f;
         full.beta = a->a;
+        full.in = x0.p;
+        full.lo = lo.p;
         if (k + 1U < a->steps) {
-            st = tall ? ns_product<false, false, NS_UPDATE>(be, x0, poly, &x0, &lo, &x1, nullptr, full) : ns_product<false, true, NS_UPDATE>(be, poly, x0, &x0, &lo, &x1, nullptr, full);
-        } else if (out->dtype == GDB_DTYPE_F16) {
-            st = tall ? ns_product<false, false, NS_LAST, __half>(be, x0, poly, &x0, &lo, nullptr, op, full) : ns_product<false, true, NS_LAST, __half>(be, poly, x0, &x0, &lo, nullptr, op, full);
+            full.out = x1.p;
+            st = tall ? ns_product<false, false, NS_UPDATE>(be, x0, poly, full) : ns_product<false, true, NS_UPDATE>(be, poly, x0, full);
         } else {
-            st = tall ? ns_product<false, false, NS_LAST, __nv_bfloat16>(be, x0, poly, &x0, &lo, nullptr, op, full)
-                      : ns_product<false, true, NS_LAST, __nv_bfloat16>(be, poly, x0, &x0, &lo, nullptr, op, full);
+            full.out = op;
+            full.wide_out = cols % 16U == 0U && (uintptr_t)op % 32U == 0U;
+            if (out->dtype == GDB_DTYPE_F16) st = tall ? ns_product<false, false, NS_LAST, __half>(be, x0, poly, full) : ns_product<false, true, NS_LAST, __half>(be, poly, x0, full);
+            else st = tall ? ns_product<false, false, NS_LAST, __nv_bfloat16>(be, x0, poly, full) : ns_product<false, true, NS_LAST, __nv_bfloat16>(be, poly, x0, full);
         }
     }
     return st;
