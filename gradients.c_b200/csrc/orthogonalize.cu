@@ -12,11 +12,13 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 
+#include <algorithm>
+
 namespace {
 using namespace gdb_t5;
 
 constexpr float NS_UP = 1024.0f, NS_DOWN = 1.0f / 1024.0f;
-constexpr int NS_NORM_BLOCKS = 64;   // partial sums of a matrix's squares, at most
+constexpr int NS_NORM_BLOCKS = 256;   // partial sums of a matrix's squares, at most
 
 // ------------------------------------------------------------------ |G|_F and the first iterate
 // eight consecutive elements of a row, zeros behind its end
@@ -39,7 +41,8 @@ __device__ __forceinline__ void ns_load8(const T *p, unsigned left, bool vec, fl
         for (int e = 0; e < 8; ++e) f[e] = (unsigned)e < left ? gdb_io<T>::ld(p, e) : 0.0f;
     }
 }
-// Sums of squares are FP64: neither 1e38 nor 1e-38 leaves the range. The matrix is taken as one row of `count` elements.
+// Sums of squares are FP64, so that neither 1e38 nor 1e-38 leaves the range; eight squares are added in FP32 first where that holds them
+// (one conversion in place of eight: four 5632 x 2048 BF16 matrices 60 -> 2x us). The matrix is taken as one row of `count` elements.
 template <typename T>
 __global__ void __launch_bounds__(256)
 ns_norm_kernel(const T *__restrict__ g, double *__restrict__ partial, size_t count, bool vec)
@@ -47,16 +50,25 @@ ns_norm_kernel(const T *__restrict__ g, double *__restrict__ partial, size_t cou
     gdb_pdl_sync();
     __shared__ double sh[8];
     const T *m = g + (size_t)blockIdx.y * count;
-    double s[2] = {0.0, 0.0};
+    double t = 0.0;
     const size_t stride = (size_t)gridDim.x * blockDim.x * 8U;
 #pragma unroll 4
     for (size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 8U; i < count; i += stride) {
         float f[8];
         ns_load8(m + i, (unsigned)min((size_t)8U, count - i), vec && i + 8U <= count, f);
+        float most = 0.0f, s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e & 1] += (double)f[e] * (double)f[e];
+        for (int e = 0; e < 8; ++e) {
+            most = fmaxf(most, fabsf(f[e]));
+            s = fmaf(f[e], f[e], s);
+        }
+        if (most == 0.0f || (most > 1.0e-12f && most < 1.0e18f)) {
+            t += (double)s;   // (NaN among the elements: in s)
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t += (double)f[e] * (double)f[e];
+        }
     }
-    double t = s[0] + s[1];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = t;
@@ -74,8 +86,8 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
     gdb_pdl_sync();
     // (every warp adds the partial sums in the same order)
     const int lane = threadIdx.x & 31;
-    double s = (lane < parts ? __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + lane]) : 0.0) +
-               (lane + 32 < parts ? __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + lane + 32]) : 0.0);
+    double s = 0.0;
+    for (int k = lane; k < parts; k += 32) s += __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + k]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffU, s, o);
     const double f = (double)NS_UP / (sqrt(s) + (double)eps);
@@ -84,6 +96,7 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
     const T *m = g + (size_t)blockIdx.y * rows * cols;
     uint4 *h = reinterpret_cast<uint4 *>(hi) + (size_t)blockIdx.y * rows * octets, *l = reinterpret_cast<uint4 *>(lo) + (size_t)blockIdx.y * rows * octets;
     const size_t n = (size_t)rows * octets;
+#pragma unroll 2
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
         const unsigned r = n < 0xffffffffU ? (unsigned)i / octets : (unsigned)(i / octets), c = (unsigned)(i - (size_t)r * octets) * 8U;
         float v[8];
@@ -119,17 +132,19 @@ struct ns_shape {
     bool wide_out;           // LAST: the caller's rows take 32-byte stores
 };
 
-// One warp's 32 x 64 piece of the result, a lane per row. Inputs and results go between registers and memory directly, 32 bytes a lane
+// One warp's piece of the result, 32 rows (a lane each) x COLS columns. Inputs and results go between registers and memory directly, 32 bytes a lane
 // and access: the products alone take 125 of the 128 bytes that shared memory moves in a cycle (operands written, read, and read by
 // the peer), so staging tiles there for TMA costs the products their time (four 5632 x 2048 matrices: a step's UPDATE 170 us with staged
 // tiles, 128 us without any epilogue traffic).
-struct ns_row {
-    uint32_t w[32];          // 64 elements
+constexpr int NS_PIECE = 32, NS_STAGE_ROW = 80, NS_WARP_STAGE = NS_PIECE * NS_STAGE_ROW;   // rows of 64 bytes, 16 apart in the banks
+template <int COLS> struct ns_row {
+    uint32_t w[COLS / 2];
 };
-__device__ __forceinline__ void ns_load_row(ns_row &r, const __half *p, uint32_t left)
+template <int COLS>
+__device__ __forceinline__ void ns_load_row(ns_row<COLS> &r, const __half *p, uint32_t left)
 {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < COLS / 16; ++k) {
         uint32_t *w = r.w + 8 * k;
         if (16U * k < left) {
             asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -142,11 +157,12 @@ __device__ __forceinline__ void ns_load_row(ns_row &r, const __half *p, uint32_t
         }
     }
 }
+template <int COLS>
 __device__ __forceinline__ void ns_store_row(void *base, const uint32_t *w, uint32_t left)
 {
     __half *p = reinterpret_cast<__half *>(base);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < COLS / 16; ++k) {
         const uint32_t *v = w + 8 * k;
         if (16U * k < left) {
             asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 16 * k), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
@@ -158,8 +174,8 @@ __device__ __forceinline__ void ns_store_row(void *base, const uint32_t *w, uint
 __device__ __forceinline__ float2 ns_two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 
 // the inputs of a piece, on their way while its products are formed
-template <int MODE>
-__device__ __forceinline__ void ns_load_piece(ns_row &in, ns_row &lo, const ns_shape &sh, uint32_t row, uint32_t col0, uint32_t z)
+template <int MODE, int COLS>
+__device__ __forceinline__ void ns_load_piece(ns_row<COLS> &in, ns_row<COLS> &lo, const ns_shape &sh, uint32_t row, uint32_t col0, uint32_t z)
 {
     if (MODE == NS_GRAM) return;
     const uint32_t left = row < sh.M && col0 < sh.N ? sh.N - col0 : 0U;
@@ -167,9 +183,9 @@ __device__ __forceinline__ void ns_load_piece(ns_row &in, ns_row &lo, const ns_s
     ns_load_row(in, sh.in + at, left);
     if (MODE != NS_POLY) ns_load_row(lo, sh.lo + at, left);
 }
-// v: the piece's accumulators. `stage` (4 KB, this warp's): rows that take no 32-byte stores are put together there.
-template <int MODE, typename TOUT>
-__device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row &in, ns_row &lo, uint32_t (&v)[64], uint32_t row0, uint32_t col0, uint32_t z, bool mirror,
+// v: the piece's accumulators. `stage` (this warp's): where a piece is transposed, or rows that take no 32-byte stores are put together.
+template <int MODE, typename TOUT, int COLS>
+__device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row<COLS> &in, ns_row<COLS> &lo, uint32_t (&v)[COLS], uint32_t row0, uint32_t col0, uint32_t z, bool mirror,
                                                 unsigned char *stage, int lane)
 {
     const uint32_t row = row0 + lane;
@@ -177,7 +193,7 @@ __device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row
     const uint32_t left = live ? sh.N - col0 : 0U;
     const size_t at = ((size_t)z * sh.M + row) * sh.pitch + col0;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
+    for (int e = 0; e < COLS / 2; ++e) {
         float f0 = sh.alpha * __uint_as_float(v[2 * e]), f1 = sh.alpha * __uint_as_float(v[2 * e + 1]);
         if (MODE != NS_GRAM) {
             float2 a = ns_two(in.w[e]);
@@ -202,108 +218,156 @@ __device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row
     if (MODE == NS_LAST) {
         unsigned short *out = reinterpret_cast<unsigned short *>(sh.out) + ((size_t)z * sh.M + row0) * sh.N + col0;
         if (sh.wide_out) {
-            ns_store_row(out + (size_t)lane * sh.N, v, left);
+            ns_store_row<COLS>(out + (size_t)lane * sh.N, v, left);
         } else {
-            const uint32_t rows = row0 < sh.M ? min(32U, sh.M - row0) : 0U, cols = col0 < sh.N ? min(64U, sh.N - col0) : 0U;
+            const uint32_t rows = row0 < sh.M ? min(32U, sh.M - row0) : 0U;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            __syncwarp();
-            for (uint32_t r = 0; r < rows; ++r) {
+            for (int h = 0; h < COLS / NS_PIECE; ++h) {
 #pragma unroll
-                for (uint32_t c = lane; c < 64U; c += 32U) {
-                    if (c < cols) out[(size_t)r * sh.N + c] = *reinterpret_cast<const unsigned short *>(stage + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t *w = v + h * (NS_PIECE / 2) + 4 * j;
+                    *reinterpret_cast<uint4 *>(stage + lane * NS_STAGE_ROW + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                __syncwarp();
+                const uint32_t c = h * NS_PIECE + lane;
+                if (col0 + c < sh.N) {
+#pragma unroll 8
+                    for (uint32_t r = 0; r < rows; ++r) out[(size_t)r * sh.N + c] = *reinterpret_cast<const unsigned short *>(stage + r * NS_STAGE_ROW + lane * 2);
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
         return;
     }
     __half *out = reinterpret_cast<__half *>(sh.out);
-    ns_store_row(out + at, v, left);
+    ns_store_row<COLS>(out + at, v, left);
     if (MODE == NS_UPDATE) {
-        ns_store_row(sh.lo + at, lo.w, left);
-    } else if (mirror && live) {
-        // the transposed piece: the lanes' elements of a column lie side by side
-        unsigned short *t = reinterpret_cast<unsigned short *>(out) + ((size_t)z * sh.M + col0) * sh.pitch + row;
+        ns_store_row<COLS>(sh.lo + at, lo.w, left);
+    } else if (COLS == NS_PIECE && mirror) {
+        // the transposed piece: row e of it are the lanes' elements e
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-            if ((uint32_t)e < left) t[(size_t)e * sh.pitch] = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+        for (int e = 0; e < NS_PIECE; ++e) *reinterpret_cast<unsigned short *>(stage + e * NS_STAGE_ROW + lane * 2) = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint4 t = *reinterpret_cast<const uint4 *>(stage + lane * NS_STAGE_ROW + j * 16);
+            v[4 * j] = t.x;
+            v[4 * j + 1] = t.y;
+            v[4 * j + 2] = t.z;
+            v[4 * j + 3] = t.w;
         }
+        const uint32_t row_t = col0 + lane, left_t = row_t < sh.M && row0 < sh.N ? sh.N - row0 : 0U;
+        ns_store_row<COLS>(out + ((size_t)z * sh.M + row_t) * sh.pitch + row0, v, left_t);
+        __syncwarp();
     }
 }
-__device__ __forceinline__ void ns_accumulators(uint32_t (&v)[64], uint32_t taddr)
-{
-    uint32_t(&a)[32] = *reinterpret_cast<uint32_t(*)[32]>(v), (&b)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 32);
-    tmem_ld_32x32b_x32_nowait(taddr, a);
-    tmem_ld_32x32b_x32_nowait(taddr + 32U, b);
-    tmem_ld_wait();
-}
 
-// ---- one CTA, one 128 x 64 tile: small matrices, where the number of SMs at work counts ----
-constexpr int NS1_BN = 64, NS1_STAGE_BYTES = (BM + NS1_BN) * BK * 2;
-template <int STAGES> constexpr int ns1_smem() { return STAGES * NS1_STAGE_BYTES + 4 * 4096 + 256 + 1024; }
+// ---- one CTA, one tile of 128 x BN: small matrices, where the number of SMs at work counts ----
+// SPLIT: two CTAs of a cluster take half of the contraction each and send each other the sums of half of the tile's columns (GRAM of long
+// matrices: few tiles, each a long chain of products).
+constexpr int NS1_SENT_ROW = 144, NS1_SENT = BM * NS1_SENT_ROW;   // 32 FP32 sums of a row, rows 16 bytes apart in the banks
+template <int BN, int STAGES, bool SPLIT> struct ns1_plan {
+    static constexpr int STAGE_BYTES = (BM + BN) * BK * 2, WARPS = 4 * BN / NS_PIECE, THREADS = 64 + 32 * WARPS;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + WARPS * NS_WARP_STAGE + (SPLIT ? NS1_SENT : 0) + 256 + 1024;
+    static_assert(BN == 32 || BN == 64, "columns of the operand's box");
+};
 
-template <bool A_MN, bool B_MN, int MODE, typename TOUT, int STAGES>
-__global__ void __launch_bounds__(192)
+template <bool A_MN, bool B_MN, int MODE, typename TOUT, int BN, int STAGES, bool SPLIT>
+__global__ void __launch_bounds__(ns1_plan<BN, STAGES, SPLIT>::THREADS)
 ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err_flag)
 {
+    typedef ns1_plan<BN, STAGES, SPLIT> plan;
+    static_assert(!SPLIT || (MODE == NS_GRAM && BN == 64), "halves of 32 columns");
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    // UPDATE and LAST read X and its low half, which the launches before the preceding one wrote: their loads need not wait for it. The
+    // operand that does is P.
+    constexpr bool EARLY = !SYM, A_IS_X = !B_MN;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
-    unsigned char *staging = smem + STAGES * NS1_STAGE_BYTES;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + 4 * 4096);   // full, empty, accumulator
+    unsigned char *staging = smem + STAGES * plan::STAGE_BYTES;
+    unsigned char *sent = staging + plan::WARPS * NS_WARP_STAGE;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sent + (SPLIT ? NS1_SENT : 0));   // full, empty, accumulator
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t z = blockIdx.y;
     uint32_t tm, tn;
     if (SYM) {
         // of row tile tm the column tiles from the diagonal on
-        uint32_t u = blockIdx.x;
-        for (tm = 0; u >= sh.tiles_n - 2U * tm; ++tm) u -= sh.tiles_n - 2U * tm;
-        tn = 2U * tm + u;
+        constexpr uint32_t STEP = BM / BN;
+        uint32_t u = SPLIT ? blockIdx.x >> 1 : blockIdx.x;
+        for (tm = 0; u >= sh.tiles_n - STEP * tm; ++tm) u -= sh.tiles_n - STEP * tm;
+        tn = STEP * tm + u;
     } else {
         tm = blockIdx.x / sh.tiles_n;
         tn = blockIdx.x - tm * sh.tiles_n;
     }
-    const uint32_t m0 = tm * BM, n0 = tn * NS1_BN, n_iters = (sh.K + BK - 1) / BK;
+    const uint32_t rank = SPLIT ? cluster_ctarank() : 0U, all_iters = (sh.K + BK - 1) / BK;
+    const uint32_t first = rank * ((all_iters + 1U) / 2U), n_iters = SPLIT ? (rank == 0U ? (all_iters + 1U) / 2U : all_iters - first) : all_iters;
+    const uint32_t m0 = tm * BM, n0 = tn * BN;
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]), accum_bar = smem_u32(&bars[2 * STAGES]);
+    auto load_a = [&](uint32_t it) {
+        const uint32_t s = it % STAGES, dst = smem_u32(smem + s * plan::STAGE_BYTES), bar = full0 + 8 * s;
+        if (A_MN) {
+            tma_load_3d(dst, &maps.a, (int)m0, (int)((first + it) * BK), (int)z, bar);
+            tma_load_3d(dst + BK * 128, &maps.a, (int)m0 + 64, (int)((first + it) * BK), (int)z, bar);
+        } else {
+            tma_load_3d(dst, &maps.a, (int)((first + it) * BK), (int)m0, (int)z, bar);
+        }
+    };
+    auto load_b = [&](uint32_t it) {
+        const uint32_t s = it % STAGES, dst = smem_u32(smem + s * plan::STAGE_BYTES) + BM * BK * 2, bar = full0 + 8 * s;
+        if (B_MN) tma_load_3d(dst, &maps.b, (int)n0, (int)((first + it) * BK), (int)z, bar); else tma_load_3d(dst, &maps.b, (int)((first + it) * BK), (int)n0, (int)z, bar);
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2 * STAGES + 1; ++s) mbar_init(full0 + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)NS1_BN) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    const int quad = warp & 3, part = (warp - 2) >> 2;   // (epilogue warps: tensor-memory quadrant, columns)
+    const uint32_t row0 = m0 + quad * 32, col0 = n0 + part * NS_PIECE;
+    ns_row<NS_PIECE> in, lo;
+    uint32_t v[NS_PIECE];
+    bool ok = true;
+    if (EARLY) {
+        if (threadIdx.x == 0) {
+            for (uint32_t it = 0; it < n_iters && it < STAGES; ++it) {
+                mbar_expect_tx(full0 + 8 * it, plan::STAGE_BYTES);
+                if (A_IS_X) load_a(it); else load_b(it);
+            }
+        } else if (warp >= 2) {
+            ns_load_piece<MODE>(in, lo, sh, row0 + lane, col0, z);
+        }
+    }
     gdb_pdl_sync();
 
     if (warp == 0) {
         if (lane == 0) {
             for (uint32_t it = 0; it < n_iters; ++it) {
-                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1U, bar = full0 + 8 * s;
-                if (!mbar_wait(empty0 + 8 * s, ph ^ 1U)) {
-                    atomicExch(err_flag, 701);
-                    break;
+                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1U;
+                const bool begun = EARLY && it < STAGES;
+                if (!begun) {
+                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1U)) {
+                        atomicExch(err_flag, 701);
+                        break;
+                    }
+                    mbar_expect_tx(full0 + 8 * s, plan::STAGE_BYTES);
                 }
-                const uint32_t a_dst = smem_u32(smem + s * NS1_STAGE_BYTES), b_dst = a_dst + BM * BK * 2;
-                const int k0 = (int)(it * BK);
-                mbar_expect_tx(bar, NS1_STAGE_BYTES);
-                if (A_MN) {
-                    tma_load_3d(a_dst, &maps.a, (int)m0, k0, (int)z, bar);
-                    tma_load_3d(a_dst + BK * 128, &maps.a, (int)m0 + 64, k0, (int)z, bar);
-                } else {
-                    tma_load_3d(a_dst, &maps.a, k0, (int)m0, (int)z, bar);
-                }
-                if (B_MN) tma_load_3d(b_dst, &maps.b, (int)n0, k0, (int)z, bar); else tma_load_3d(b_dst, &maps.b, k0, (int)n0, (int)z, bar);
+                if (!begun || !A_IS_X) load_a(it);
+                if (!begun || A_IS_X) load_b(it);
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t IDESC = (1U << 4) | ((A_MN ? 1U : 0U) << 15) | ((B_MN ? 1U : 0U) << 16) | ((uint32_t)(NS1_BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            constexpr uint32_t IDESC = (1U << 4) | ((A_MN ? 1U : 0U) << 15) | ((B_MN ? 1U : 0U) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
             for (uint32_t it = 0; it < n_iters; ++it) {
                 const uint32_t s = it % STAGES, ph = (it / STAGES) & 1U;
                 if (!mbar_wait(full0 + 8 * s, ph)) {
@@ -311,7 +375,7 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
                     break;
                 }
                 tcgen05_fence_after();
-                const uint32_t a_base = smem_u32(smem + s * NS1_STAGE_BYTES), b_base = a_base + BM * BK * 2;
+                const uint32_t a_base = smem_u32(smem + s * plan::STAGE_BYTES), b_base = a_base + BM * BK * 2;
 #pragma unroll
                 for (int kk = 0; kk < BK / UMMA_K; ++kk) {
                     const uint64_t adesc = A_MN ? make_smem_desc(a_base + kk * 2048, BK * 128, 1024) : make_smem_desc(a_base + kk * 32, 16, 1024);
@@ -323,33 +387,52 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
             tcgen05_commit(accum_bar);
         }
     } else {
-        const int quad = warp & 3;
-        const uint32_t row0 = m0 + quad * 32;
-        ns_row in, lo;
-        ns_load_piece<MODE>(in, lo, sh, row0 + lane, n0, z);
-        const bool ok = __all_sync(0xffffffffU, mbar_wait(accum_bar, 0));
+        if (!EARLY) ns_load_piece<MODE>(in, lo, sh, row0 + lane, col0, z);
+        ok = __all_sync(0xffffffffU, mbar_wait(accum_bar, 0));
         if (!ok && lane == 0) atomicExch(err_flag, 703);
         tcgen05_fence_after();
         if (ok) {
-            uint32_t v[64];
-            ns_accumulators(v, tmem_base + ((uint32_t)(quad * 32) << 16));
-            ns_finish_piece<MODE, TOUT>(sh, in, lo, v, row0, n0, z, tn / 2U != tm, staging + quad * 4096, lane);
+            tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(quad * 32) << 16) + part * NS_PIECE, v);
+            if (SPLIT && part != (int)rank) {
+                const uint32_t to = mapa_shared(smem_u32(sent) + (quad * 32 + lane) * NS1_SENT_ROW, rank ^ 1U);
+#pragma unroll
+                for (int k = 0; k < NS_PIECE; k += 4) {
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 4 * k), "r"(v[k]), "r"(v[k + 1]), "r"(v[k + 2]), "r"(v[k + 3]) : "memory");
+                }
+            }
         }
+    }
+    if (SPLIT) {
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= 2 && part == (int)rank) {
+#pragma unroll
+            for (int k = 0; k < NS_PIECE; k += 4) {
+                const float4 o = *reinterpret_cast<const float4 *>(sent + (quad * 32 + lane) * NS1_SENT_ROW + 4 * k);
+                v[k] = __float_as_uint(__uint_as_float(v[k]) + o.x);
+                v[k + 1] = __float_as_uint(__uint_as_float(v[k + 1]) + o.y);
+                v[k + 2] = __float_as_uint(__uint_as_float(v[k + 2]) + o.z);
+                v[k + 3] = __float_as_uint(__uint_as_float(v[k + 3]) + o.w);
+            }
+        }
+    }
+    if (warp >= 2 && ok && (!SPLIT || part == (int)rank)) {
+        ns_finish_piece<MODE, TOUT>(sh, in, lo, v, row0, col0, z, tn / (BM / BN) != tm, staging + (warp - 2) * NS_WARP_STAGE, lane);
     }
     __syncwarp();
     tcgen05_fence_before();
     __syncthreads();
     if (warp == 1) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)NS1_BN) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)BN) : "memory");
     }
 }
 
 // ---- a pair of CTAs, 256 x 256 tiles, persistent: tiles to fill the GPU. The roles and the two accumulators are those of
 // gemm_tcgen05_pair.cu: each CTA fetches its own halves of the operands, the leader issues the products for both, the epilogue
 // of one tile runs under the products of the next. ----
-constexpr int NS2_BN = 256, NS2_STAGES = 5, NS2_WARPS = 8, NS2_STAGING = 4096;
+constexpr int NS2_BN = 256, NS2_STAGES = 5, NS2_WARPS = 8;
 constexpr int NS2_STAGE_BYTES = (BM + NS2_BN / 2) * BK * 2;
-constexpr int NS2_SMEM = NS2_STAGES * NS2_STAGE_BYTES + NS2_WARPS * NS2_STAGING + 512 + 1024;
+constexpr int NS2_SMEM = NS2_STAGES * NS2_STAGE_BYTES + NS2_WARPS * NS_WARP_STAGE + 256 + 1024;
 
 template <bool A_MN, bool B_MN, int MODE, typename TOUT>
 __global__ void __launch_bounds__(32 * (2 + NS2_WARPS), 1)
@@ -359,7 +442,7 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
     unsigned char *staging = smem + NS2_STAGES * NS2_STAGE_BYTES;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + NS2_WARPS * NS2_STAGING);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + NS2_WARPS * NS_WARP_STAGE);
     // full, empty, accumulator full [2], accumulator empty [2]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS2_STAGES + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -462,7 +545,9 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
             }
         }
     } else {
-        // warps w and w + 4 share a tensor-memory quadrant and take two of the tile's four 64-column pieces each
+        // warps w and w + 4 share a tensor-memory quadrant and take half of the tile's columns each: in two pieces where whole lines of 128
+        // bytes go to memory, in four square ones where they are transposed
+        constexpr int COLS = SYM ? NS_PIECE : 64;
         const int quad = warp & 3, half = (warp - 2) >> 2;
         const uint32_t tempty_leader = mapa_shared(tempty0, 0);
         uint32_t idx = 0;
@@ -470,26 +555,28 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
             uint32_t z, tm, tn;
             tile_of(u, z, tm, tn);
             const uint32_t buf = idx & 1U, row0 = tm * 2 * BM + rank * BM + quad * 32, tbase = tmem_base + ((uint32_t)(quad * 32) << 16) + buf * NS2_BN + half * 128;
-            ns_row in, lo;
-            ns_load_piece<MODE>(in, lo, sh, row0 + lane, tn * NS2_BN + half * 128, z);
+            const uint32_t first = tn * NS2_BN + half * 128;
+            ns_row<COLS> in, lo;
+            ns_load_piece<MODE>(in, lo, sh, row0 + lane, first, z);
             if (!__all_sync(0xffffffffU, mbar_wait(tfull0 + 8 * buf, (idx >> 1) & 1U))) {
                 if (lane == 0) atomicExch(err_flag, 714);
                 break;
             }
             tcgen05_fence_after();
-#pragma unroll 1
-            for (int p = 0; p < 2; ++p) {
-                const uint32_t col0 = tn * NS2_BN + half * 128 + 64U * p;
-                if (p == 1) ns_load_piece<MODE>(in, lo, sh, row0 + lane, col0, z);
-                uint32_t v[64];
-                ns_accumulators(v, tbase + 64U * p);
-                if (p == 1) {
+#pragma unroll
+            for (int p = 0; p < 128 / COLS; ++p) {
+                if (p > 0) ns_load_piece<MODE>(in, lo, sh, row0 + lane, first + p * COLS, z);   // (two sets of registers, loaded a piece ahead, gained nothing)
+                uint32_t v[COLS];
+#pragma unroll
+                for (int k = 0; k < COLS; k += 32) tmem_ld_32x32b_x32_nowait(tbase + p * COLS + k, *reinterpret_cast<uint32_t(*)[32]>(v + k));
+                tmem_ld_wait();
+                if ((p + 1) * COLS == 128) {
                     // the accumulator has been copied out
                     tcgen05_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * buf);
                 }
-                ns_finish_piece<MODE, TOUT>(sh, in, lo, v, row0, col0, z, tn != tm, staging + (warp - 2) * NS2_STAGING, lane);
+                ns_finish_piece<MODE, TOUT>(sh, in, lo, v, row0, first + p * COLS, z, tn != tm, staging + (warp - 2) * NS_WARP_STAGE, lane);
                 __syncwarp();
             }
         }
@@ -523,19 +610,47 @@ bool ns_operand(CUtensorMap *m, const ns_tensor &t, uint64_t batch, bool mn, uin
     return mn ? ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, BK, 64, true) : ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, tile, BK, true);
 }
 
-template <bool A_MN, bool B_MN, int MODE, typename TOUT>
+// a launch of clusters of two
+template <typename K>
+gd_status ns_launch_clusters(gd_backend *be, K kern, dim3 grid, unsigned threads, int smem, const ns_maps &maps, const ns_shape &sh)
+{
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see gdb_pdl_sync()
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = be->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps, sh, be->err_flag);
+    if (e != cudaSuccess) {
+        be->launches += 1U;
+        return gdb_fail(be, e, "orthogonalize product");
+    }
+    return gdb_launched(be, "orthogonalize product");
+}
+
+template <bool A_MN, bool B_MN, int MODE, typename TOUT, int BN, bool SPLIT = false>
 gd_status ns_launch_single(gd_backend *be, const ns_maps &maps, const ns_shape &sh, uint32_t tiles)
 {
-    // UPDATE and LAST have more tiles than SMs as a rule and run two CTAs per SM, the others one with a deeper ring
-    constexpr int STAGES = MODE == NS_GRAM || MODE == NS_POLY ? 6 : 3, SMEM = ns1_smem<STAGES>();
-    auto kern = ns_single_kernel<A_MN, B_MN, MODE, TOUT, STAGES>;
+    // UPDATE and LAST: two CTAs fit an SM, or one beside a CTA of the preceding POLY
+    constexpr int STAGES = MODE == NS_GRAM || MODE == NS_POLY ? (BN == 32 ? 5 : 4) : (BN == 32 ? 4 : 3);
+    typedef ns1_plan<BN, STAGES, SPLIT> plan;
+    auto kern = ns_single_kernel<A_MN, B_MN, MODE, TOUT, BN, STAGES, SPLIT>;
     static bool ready = false;
     if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan::SMEM);
         if (e != cudaSuccess) return gdb_fail(be, e, "orthogonalize smem attribute");
         ready = true;
     }
-    gdb_launch(kern, dim3(tiles, sh.batch), 192, SMEM, be->stream, maps, sh, be->err_flag);
+    if (SPLIT) return ns_launch_clusters(be, kern, dim3(2U * tiles, sh.batch), plan::THREADS, plan::SMEM, maps, sh);
+    gdb_launch(kern, dim3(tiles, sh.batch), plan::THREADS, plan::SMEM, be->stream, maps, sh, be->err_flag);
     return gdb_launched(be, "orthogonalize product");
 }
 
@@ -549,27 +664,8 @@ gd_status ns_launch_pair(gd_backend *be, const ns_maps &maps, const ns_shape &sh
         if (e != cudaSuccess) return gdb_fail(be, e, "orthogonalize smem attribute");
         ready = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
     const uint32_t most = (uint32_t)be->sm_count / 2U;
-    cfg.gridDim = dim3(2U * (units < most ? units : most));
-    cfg.blockDim = dim3(32 * (2 + NS2_WARPS));
-    cfg.dynamicSmemBytes = NS2_SMEM;
-    cfg.stream = be->stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps, sh, be->err_flag);
-    if (e != cudaSuccess) {
-        be->launches += 1U;
-        return gdb_fail(be, e, "orthogonalize product");
-    }
-    return gdb_launched(be, "orthogonalize product");
+    return ns_launch_clusters(be, kern, dim3(2U * (units < most ? units : most)), 32U * (2 + NS2_WARPS), NS2_SMEM, maps, sh);
 }
 
 // One product of a step: operands xa and xb; sh has what the epilogue needs.
@@ -577,23 +673,45 @@ template <bool A_MN, bool B_MN, int MODE, typename TOUT = __half>
 gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, ns_shape sh)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    const uint32_t p_m = (sh.M + 255U) / 256U, p_n = (sh.N + 255U) / 256U, s_m = (sh.M + 127U) / 128U, s_n = (sh.N + 63U) / 64U;
-    uint32_t singles = s_m * s_n;
-    const uint32_t pairs = (SYM ? p_n * (p_n + 1U) / 2U : p_m * p_n) * sh.batch;
-    if (SYM) {
-        singles = 0;
-        for (uint32_t i = 0; 2U * i < s_n; ++i) singles += s_n - 2U * i;
-    }
-    // Both kernels wait for their operands: a k step of 64 takes a pair's CTA 32 KB, a single CTA 24 KB at some 55 bytes per cycle and
-    // SM, so rounds of tiles count 4 : 3.
     const uint64_t sms = (uint64_t)be->sm_count, clusters = sms / 2U;
-    const bool pair = 4U * ((pairs + clusters - 1U) / clusters) <= 3U * (((uint64_t)singles * sh.batch + sms - 1U) / sms);
+    const uint32_t p_m = (sh.M + 255U) / 256U, p_n = (sh.N + 255U) / 256U, s_m = (sh.M + 127U) / 128U;
+    const uint32_t pairs = (SYM ? p_n * (p_n + 1U) / 2U : p_m * p_n) * sh.batch;
+    auto singles = [&](uint32_t bn) {
+        const uint32_t s_n = (sh.N + bn - 1U) / bn, step = 128U / bn;
+        uint32_t n = s_m * s_n;
+        if (SYM) {
+            n = 0;
+            for (uint32_t i = 0; step * i < s_n; ++i) n += s_n - step * i;
+        }
+        return n;
+    };
+    // Time of a launch in units of 10 ns, as measured: a fixed part (dependency on the launch before, first operands, epilogue), one per
+    // k step of 64 and round of tiles (the operands' way into shared memory), and what a further round adds where one CTA per SM starts
+    // anew. One call on a 512 x 512, 1024 x 1024, 2048 x 2048 matrix: pair 182, 221, 322 us, 128 x 64 tiles 91, 134, 411 us, 128 x 32
+    // tiles 83, 123, 413 us.
+    const uint32_t wide = singles(64), narrow = B_MN ? 0U : singles(32), iters = (sh.K + BK - 1U) / BK;
+    auto cost = [&](uint64_t fixed, uint64_t again, uint64_t step, uint64_t tiles, uint64_t places, uint64_t its) {
+        const uint64_t rounds = (tiles + places - 1U) / places;
+        return fixed + again * (rounds - 1U) + step * its * rounds;
+    };
+    const uint64_t none = UINT64_MAX, again = SYM ? 250U : 80U, c_pair = cost(900, 100, 39, pairs, clusters, iters),
+                   c_wide = cost(320, again, 35, (uint64_t)wide * sh.batch, sms, iters), c_narrow = B_MN ? none : cost(285, again, 33, (uint64_t)narrow * sh.batch, sms, iters),
+                   c_split = MODE == NS_GRAM && iters > 1U ? cost(530, again, 35, 2U * (uint64_t)wide * sh.batch, sms, (iters + 1U) / 2U) : none;
+    const uint64_t least = std::min(std::min(c_pair, c_wide), std::min(c_narrow, c_split));
+    const bool pair = c_pair == least, split = !pair && c_split == least, slim = !pair && !split && c_narrow == least;
+    const uint32_t bn = pair ? 256U : (slim ? 32U : 64U);
     sh.tiles_m = pair ? p_m : s_m;
-    sh.tiles_n = pair ? p_n : s_n;
+    sh.tiles_n = (sh.N + bn - 1U) / bn;
     ns_maps maps;
-    bool ok = ns_operand(&maps.a, xa, sh.batch, A_MN, 128) && ns_operand(&maps.b, xb, sh.batch, B_MN, pair ? 128 : 64);
-    if (!ok) return GD_ERR_UNSUPPORTED;
-    return pair ? ns_launch_pair<A_MN, B_MN, MODE, TOUT>(be, maps, sh, pairs) : ns_launch_single<A_MN, B_MN, MODE, TOUT>(be, maps, sh, singles);
+    if (!ns_operand(&maps.a, xa, sh.batch, A_MN, 128) || !ns_operand(&maps.b, xb, sh.batch, B_MN, pair ? 128 : bn)) return GD_ERR_UNSUPPORTED;
+    if (pair) return ns_launch_pair<A_MN, B_MN, MODE, TOUT>(be, maps, sh, pairs);
+    if constexpr (!B_MN) {
+        if (slim) return ns_launch_single<A_MN, B_MN, MODE, TOUT, 32>(be, maps, sh, narrow);
+    }
+    if constexpr (MODE == NS_GRAM) {
+        if (split) return ns_launch_single<A_MN, B_MN, MODE, TOUT, 64, true>(be, maps, sh, wide);
+    }
+    return ns_launch_single<A_MN, B_MN, MODE, TOUT, 64>(be, maps, sh, wide);
 }
 
 // Where the parts of the scratch lie: the iterate's high halves (two, used in turn), its low halves, A, P, the sums of squares.
