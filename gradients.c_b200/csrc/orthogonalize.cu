@@ -42,7 +42,34 @@ __device__ __forceinline__ void ns_load8(const T *p, unsigned left, bool vec, fl
     }
 }
 // Sums of squares are FP64, so that neither 1e38 nor 1e-38 leaves the range; eight squares are added in FP32 first where that holds them
-// (one conversion in place of eight: four 5632 x 2048 BF16 matrices 60 -> 2x us). The matrix is taken as one row of `count` elements.
+// (one conversion in place of eight: four 5632 x 2048 BF16 matrices 60 -> 25 us).
+__device__ __forceinline__ double ns_squares(const float (&f)[8])
+{
+    float most = 0.0f, s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        most = fmaxf(most, fabsf(f[e]));
+        s = fmaf(f[e], f[e], s);
+    }
+    if (most == 0.0f || (most > 1.0e-12f && most < 1.0e18f)) return (double)s;   // (NaN among the elements: in s)
+    double t = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t += (double)f[e] * (double)f[e];
+    return t;
+}
+// f times the factor as the sum of two FP16 numbers
+__device__ __forceinline__ void ns_halves(const float (&f)[8], double factor, gdb_vec8<__half> &hi, gdb_vec8<__half> &lo)
+{
+    const bool normal = factor < 3.0e38 && factor > 1.2e-38;   // the factor is a normal FP32 number
+    const float ff = (float)factor;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float w = normal ? f[e] * ff : (float)((double)f[e] * factor);
+        hi.set(e, w);
+        lo.set(e, w - hi.get(e));
+    }
+}
+// The matrix is taken as one row of `count` elements.
 template <typename T>
 __global__ void __launch_bounds__(256)
 ns_norm_kernel(const T *__restrict__ g, double *__restrict__ partial, size_t count, bool vec)
@@ -56,18 +83,7 @@ ns_norm_kernel(const T *__restrict__ g, double *__restrict__ partial, size_t cou
     for (size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 8U; i < count; i += stride) {
         float f[8];
         ns_load8(m + i, (unsigned)min((size_t)8U, count - i), vec && i + 8U <= count, f);
-        float most = 0.0f, s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            most = fmaxf(most, fabsf(f[e]));
-            s = fmaf(f[e], f[e], s);
-        }
-        if (most == 0.0f || (most > 1.0e-12f && most < 1.0e18f)) {
-            t += (double)s;   // (NaN among the elements: in s)
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t += (double)f[e] * (double)f[e];
-        }
+        t += ns_squares(f);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
@@ -91,8 +107,6 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffU, s, o);
     const double f = (double)NS_UP / (sqrt(s) + (double)eps);
-    const bool small = f < 3.0e38 && f > 1.2e-38;   // the factor is a normal FP32 number
-    const float ff = (float)f;
     const T *m = g + (size_t)blockIdx.y * rows * cols;
     uint4 *h = reinterpret_cast<uint4 *>(hi) + (size_t)blockIdx.y * rows * octets, *l = reinterpret_cast<uint4 *>(lo) + (size_t)blockIdx.y * rows * octets;
     const size_t n = (size_t)rows * octets;
@@ -102,12 +116,7 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
         float v[8];
         ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
         gdb_vec8<__half> a, b;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float w = small ? v[e] * ff : (float)((double)v[e] * f);
-            a.set(e, w);
-            b.set(e, w - a.get(e));
-        }
+        ns_halves(v, f, a, b);
         h[i] = a.raw;
         l[i] = b.raw;
     }
@@ -610,6 +619,287 @@ bool ns_operand(CUtensorMap *m, const ns_tensor &t, uint64_t batch, bool mn, uin
     return mn ? ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, BK, 64, true) : ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, tile, BK, true);
 }
 
+// ---- matrices whose smaller side is at most 128: all steps in one launch, a cluster of up to 16 CTAs per matrix ----
+// A and P are one tile. Each CTA keeps up to 256 columns of X (rows for a tall matrix: X is taken transposed then) in shared memory, both
+// halves, and forms its part of A; the parts are added over distributed shared memory (every CTA a share of the rows, then the sum to
+// all), P is formed by every CTA for itself, and the CTA's columns are updated in place. Two exchanges a step in place of three launches
+// that would each occupy a handful of SMs: 17 launches take the host 57 us alone.
+constexpr int NT_M = 128, NT_W = 256, NT_THREADS = 256, NT_MAX_CTAS = 16;
+constexpr int NT_X_BYTES = NT_M * NT_W * 2, NT_A_BYTES = NT_M * NT_M * 2, NT_PARTS = NT_M * NT_M * 4;   // (P takes the place of the parts)
+constexpr int NT_SMEM = 2 * NT_X_BYTES + NT_A_BYTES + NT_PARTS + 512 + 1024;
+
+// element (row, col) of a tile of 128 rows in blocks of 64 columns, 128-byte swizzle: the 16 bytes that hold columns 8 * octet ...
+__device__ __forceinline__ uint32_t nt_at(uint32_t row, uint32_t octet) { return (octet >> 3) * (NT_M * 128U) + row * 128U + (((octet & 7U) ^ (row & 7U)) << 4); }
+__device__ __forceinline__ void nt_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+template <typename T, typename TOUT>
+__global__ void __launch_bounds__(NT_THREADS, 1)
+ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols, uint32_t steps, float ca, float cb, float cc, float eps, bool vec, int *err_flag)
+{
+    gdb_pdl_sync();
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
+    unsigned char *xh = smem, *xl = xh + NT_X_BYTES, *sa = xl + NT_X_BYTES, *parts = sa + NT_A_BYTES;   // hi, lo, A, parts of A (then P)
+    double *sums = reinterpret_cast<double *>(parts + NT_PARTS);                                        // [CTAs], then the warps' sums
+    uint64_t *bar = reinterpret_cast<uint64_t *>(sums + NT_MAX_CTAS + 8);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), ctas = gridDim.x, z = blockIdx.y;   // (one cluster per matrix: grid.x is its size)
+    const bool tall = rows > cols;
+    const uint32_t m = tall ? cols : rows, n = tall ? rows : cols;
+    const uint32_t width = ((n + ctas - 1U) / ctas + 63U) & ~63U, j0 = rank * width;   // columns of X here (multiples of 64)
+    const uint32_t done = smem_u32(bar);
+    if (threadIdx.x == 0) {
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512U) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    const T *x = g + (size_t)z * rows * cols;
+    // eight columns of a row: contiguous in memory, or one from each of eight rows of a tall matrix (neighbouring threads take
+    // neighbouring elements of those)
+    const uint32_t octets = width / 8U;
+    auto place = [&](uint32_t i, uint32_t &row, uint32_t &octet) {
+        row = tall ? i % NT_M : i / octets;
+        octet = tall ? i / NT_M : i % octets;
+    };
+    auto load = [&](uint32_t row, uint32_t octet, float (&f)[8]) {
+        const uint32_t j = j0 + octet * 8U;
+        if (row >= m || j >= n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+        } else if (tall) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = j + e < n ? gdb_io<T>::ld(x, (size_t)(j + e) * cols + row) : 0.0f;
+        } else {
+            ns_load8(x + (size_t)row * cols + j, n - j, vec, f);
+        }
+    };
+    double t = 0.0;
+#pragma unroll 2
+    for (uint32_t i = threadIdx.x; i < NT_M * octets; i += NT_THREADS) {
+        uint32_t row, octet;
+        place(i, row, octet);
+        float f[8];
+        load(row, octet, f);
+        t += ns_squares(f);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
+    if (lane == 0) sums[NT_MAX_CTAS + warp] = t;
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_slot;   // columns 0..255: X, 256..383: A, 384..511: A A
+    cluster_sync_all();                 // (every CTA of the cluster runs before its memory is written)
+    if (threadIdx.x < ctas) {
+        double s = 0.0;
+        for (int w = 0; w < 8; ++w) s += sums[NT_MAX_CTAS + w];
+        asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_shared(smem_u32(sums + rank), threadIdx.x)), "l"(__double_as_longlong(s)) : "memory");
+    }
+    __syncwarp();
+    cluster_sync_all();
+    double norm = 0.0;
+    for (uint32_t r = 0; r < ctas; ++r) norm += sums[r];
+    const double factor = (double)NS_UP / (sqrt(norm) + (double)eps);
+#pragma unroll 2
+    for (uint32_t i = threadIdx.x; i < NT_M * octets; i += NT_THREADS) {
+        uint32_t row, octet;
+        place(i, row, octet);
+        float f[8];
+        load(row, octet, f);
+        gdb_vec8<__half> h, l;
+        ns_halves(f, factor, h, l);
+        *reinterpret_cast<uint4 *>(xh + nt_at(row, octet)) = h.raw;
+        *reinterpret_cast<uint4 *>(xl + nt_at(row, octet)) = l.raw;
+    }
+
+    const int quad = warp & 3, half = warp >> 2;
+    const uint32_t row = quad * 32 + lane, tlane = (uint32_t)(quad * 32) << 16;
+    const uint32_t share = NT_M / ctas;   // rows of A that this CTA adds up
+    uint32_t phase = 0;
+    bool ok = true;
+    // the products of a phase, by one thread, and the wait for them by all
+    auto products = [&](uint32_t d, uint32_t a, uint32_t b, bool b_mn, uint32_t n_cols, uint32_t blocks, uint32_t block_bytes) {
+        nt_fence();
+        tcgen05_fence_before();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            tcgen05_fence_after();
+            const uint32_t idesc = (1U << 4) | ((b_mn ? 1U : 0U) << 16) | ((n_cols >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            for (uint32_t k = 0; k < blocks; ++k) {
+                for (uint32_t kk = 0; kk < BK / UMMA_K; ++kk) {
+                    const uint64_t ad = make_smem_desc(a + k * (NT_M * 128U) + kk * 32, 16, 1024);
+                    const uint64_t bd = b_mn ? make_smem_desc(b + k * block_bytes + kk * 2048, NT_M * 128U, 1024) : make_smem_desc(b + k * block_bytes + kk * 32, 16, 1024);
+                    tcgen05_mma_f16(d, ad, bd, idesc, (k != 0 || kk != 0) ? 1U : 0U);
+                }
+            }
+            tcgen05_commit(done);
+        }
+        if (ok && !mbar_wait(done, phase)) {
+            ok = false;
+            atomicExch(err_flag, 721);
+        }
+        phase ^= 1U;
+        __syncwarp();
+        tcgen05_fence_after();
+    };
+    for (uint32_t step = 0; step < steps; ++step) {
+        // this CTA's part of A = X X^T
+        products(tmem + 256U, smem_u32(xh), smem_u32(xh), false, NT_M, width / BK, NT_M * 128U);
+        if (ctas > 1U) {
+            // no CTA of the cluster still reads its P, which lies where the parts go
+            cluster_sync_all();
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem + tlane + 256U + half * 64 + c * 32, v);
+                const uint32_t to = mapa_shared(smem_u32(parts) + (rank * share + row % share) * 512U, row / share);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t at = to + (((uint32_t)(half * 16 + c * 8 + k) ^ (row & 7U)) << 4);
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[4 * k]), "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3]) : "memory");
+                }
+            }
+            cluster_sync_all();
+            for (uint32_t i = threadIdx.x; i < share * 32U; i += NT_THREADS) {
+                const uint32_t r = i / 32U, c4 = i % 32U, to_row = rank * share + r;
+                float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (uint32_t k = 0; k < ctas; ++k) {
+                    const float4 p = *reinterpret_cast<const float4 *>(parts + (k * share + r) * 512U + ((c4 ^ (r & 7U)) << 4));
+                    s.x += p.x;
+                    s.y += p.y;
+                    s.z += p.z;
+                    s.w += p.w;
+                }
+                constexpr float DOWN2 = NS_DOWN * NS_DOWN;
+                const uint32_t w0 = half_pack<__half>::pack(s.x * DOWN2, s.y * DOWN2), w1 = half_pack<__half>::pack(s.z * DOWN2, s.w * DOWN2);
+                const uint32_t at = smem_u32(sa) + nt_at(to_row, c4 >> 1) + (c4 & 1U) * 8U;
+                for (uint32_t k = 0; k < ctas; ++k) {
+                    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(at, (rank + k) % ctas)), "r"(w0), "r"(w1) : "memory");
+                }
+            }
+            nt_fence();
+            __syncwarp();
+            cluster_sync_all();
+        } else {
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem + tlane + 256U + half * 64 + c * 32, v);
+                constexpr float DOWN2 = NS_DOWN * NS_DOWN;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = half_pack<__half>::pack(__uint_as_float(v[8 * k + 2 * e]) * DOWN2, __uint_as_float(v[8 * k + 2 * e + 1]) * DOWN2);
+                    *reinterpret_cast<uint4 *>(sa + nt_at(row, half * 8 + c * 4 + k)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        // P = b A + c A A (A is symmetric: rows serve as columns)
+        products(tmem + 384U, smem_u32(sa), smem_u32(sa), false, NT_M, 2U, NT_M * 128U);
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem + tlane + 384U + half * 64 + c * 32, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = nt_at(row, half * 8 + c * 4 + k);
+                const uint4 a = *reinterpret_cast<const uint4 *>(sa + at);
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = ns_two((&a.x)[e]);
+                    w[e] = half_pack<__half>::pack(fmaf(cb, f.x, cc * __uint_as_float(v[8 * k + 2 * e])), fmaf(cb, f.y, cc * __uint_as_float(v[8 * k + 2 * e + 1])));
+                }
+                *reinterpret_cast<uint4 *>(parts + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        // X <- a X + P X, this CTA's columns
+        products(tmem, smem_u32(parts), smem_u32(xh), true, width, 2U, BK * 128U);
+        const bool last = step + 1U == steps;
+#pragma unroll 1
+        for (uint32_t c = half * 32U; c < width; c += 64U) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem + tlane + c, v);
+            TOUT *o = out + (size_t)z * rows * cols;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = nt_at(row, c / 8U + k);
+                const uint4 h = *reinterpret_cast<const uint4 *>(xh + at), l = *reinterpret_cast<const uint4 *>(xl + at);
+                uint4 nh, nl;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 a = ns_two((&h.x)[e]), b = ns_two((&l.x)[e]);
+                    const float f0 = fmaf(ca, a.x + b.x, __uint_as_float(v[8 * k + 2 * e])), f1 = fmaf(ca, a.y + b.y, __uint_as_float(v[8 * k + 2 * e + 1]));
+                    const uint32_t j = j0 + c + k * 8U + e * 2U;
+                    if (last) {
+                        if (row < m) {
+                            if (j < n) gdb_io<TOUT>::st(o, tall ? (size_t)j * cols + row : (size_t)row * cols + j, f0 * NS_DOWN);
+                            if (j + 1U < n) gdb_io<TOUT>::st(o, tall ? (size_t)(j + 1U) * cols + row : (size_t)row * cols + j + 1U, f1 * NS_DOWN);
+                        }
+                    } else {
+                        const uint32_t p = half_pack<__half>::pack(f0, f1);
+                        const float2 r = ns_two(p);
+                        (&nh.x)[e] = p;
+                        (&nl.x)[e] = half_pack<__half>::pack(f0 - r.x, f1 - r.y);
+                    }
+                }
+                if (!last) {
+                    *reinterpret_cast<uint4 *>(xh + at) = nh;
+                    *reinterpret_cast<uint4 *>(xl + at) = nl;
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    cluster_sync_all();
+    if (warp == 0) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512U) : "memory");
+    }
+}
+
+template <typename T, typename TOUT>
+gd_status ns_launch_tile(gd_backend *be, const void *g, void *out, const gdb200_orthogonalize_args *a)
+{
+    auto kern = ns_tile_kernel<T, TOUT>;
+    static bool ready = false;
+    if (!ready) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NT_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return gdb_fail(be, e, "orthogonalize attributes");
+        ready = true;
+    }
+    const uint64_t n = std::max(a->rows, a->cols);
+    unsigned ctas = 1;
+    while (ctas * NT_W < n) ctas *= 2U;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see gdb_pdl_sync()
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(ctas, (unsigned)a->batch);
+    cfg.blockDim = dim3(NT_THREADS);
+    cfg.dynamicSmemBytes = NT_SMEM;
+    cfg.stream = be->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const bool vec = a->cols % 8U == 0U && (uintptr_t)g % 16U == 0U;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T *)g, (TOUT *)out, (uint32_t)a->rows, (uint32_t)a->cols, a->steps, a->a, a->b, a->c, a->eps, vec, be->err_flag);
+    if (e != cudaSuccess) {
+        be->launches += 1U;
+        return gdb_fail(be, e, "orthogonalize tile");
+    }
+    return gdb_launched(be, "orthogonalize tile");
+}
+
 // a launch of clusters of two
 template <typename K>
 gd_status ns_launch_clusters(gd_backend *be, K kern, dim3 grid, unsigned threads, int smem, const ns_maps &maps, const ns_shape &sh)
@@ -785,6 +1075,12 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
         return GD_OK;
     }
     const uint64_t rows = a->rows, cols = a->cols, m = l.small;
+    if (m <= NT_M && std::max(rows, cols) <= (uint64_t)NT_W * NT_MAX_CTAS) {
+        const bool half_out = out->dtype == GDB_DTYPE_F16;
+        if (x->dtype == GDB_DTYPE_F16) return half_out ? ns_launch_tile<__half, __half>(be, xp, op, a) : ns_launch_tile<__half, __nv_bfloat16>(be, xp, op, a);
+        if (x->dtype == GDB_DTYPE_BF16) return half_out ? ns_launch_tile<__nv_bfloat16, __half>(be, xp, op, a) : ns_launch_tile<__nv_bfloat16, __nv_bfloat16>(be, xp, op, a);
+        return half_out ? ns_launch_tile<float, __half>(be, xp, op, a) : ns_launch_tile<float, __nv_bfloat16>(be, xp, op, a);
+    }
     const bool tall = rows > cols;
     const ns_tensor hi[2] = {{(__half *)(sp + l.hi[0]), rows, cols, l.pitch}, {(__half *)(sp + l.hi[1]), rows, cols, l.pitch}};
     const ns_tensor lo = {(__half *)(sp + l.lo), rows, cols, l.pitch}, gram = {(__half *)(sp + l.gram), m, m, l.small_pitch}, poly = {(__half *)(sp + l.poly), m, m, l.small_pitch};

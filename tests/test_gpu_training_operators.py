@@ -332,7 +332,8 @@ def ns_check(got, want, out_dtype, steps=5, g=None, eps=1e-7, coeff=COEFF):
 
 @pytest.mark.parametrize("kind", ["noise", "strong"])
 @pytest.mark.parametrize("batch,rows,cols", [(1, 1, 1), (2, 1, 9), (1, 9, 1), (3, 5, 7), (1, 64, 64), (2, 63, 200), (2, 200, 63), (1, 128, 128), (3, 129, 128), (1, 257, 129), (1, 130, 1000),
-                                             (1, 1000, 130), (2, 512, 512), (1, 515, 1201), (1, 300, 299), (5, 256, 640), (2, 1304, 1416), (2, 1411, 1301), (2, 1301, 1411)])
+                                             (1, 1000, 130), (2, 512, 512), (1, 515, 1201), (1, 300, 299), (5, 256, 640), (2, 1304, 1416), (2, 1411, 1301), (2, 1301, 1411), (2, 100, 500),
+                                             (1, 4000, 77), (2, 128, 4096), (3, 31, 1025), (2, 2049, 16), (1, 600, 128), (1, 128, 4097), (20, 64, 300)])
 def test_orthogonalize(step, batch, rows, cols, kind):
     for dtype, out_dtype in ((F32, F16), (BF16, BF16), (F16, F16)):
         scale = 1.0 if dtype != F16 else 64.0   # (FP16 holds gradients of a scaled loss)
