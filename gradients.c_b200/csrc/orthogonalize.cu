@@ -57,16 +57,18 @@ __device__ __forceinline__ double ns_squares(const float (&f)[8])
     for (int e = 0; e < 8; ++e) t += (double)f[e] * (double)f[e];
     return t;
 }
+__device__ __forceinline__ float2 ns_two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 // f times the factor as the sum of two FP16 numbers
-__device__ __forceinline__ void ns_halves(const float (&f)[8], double factor, gdb_vec8<__half> &hi, gdb_vec8<__half> &lo)
+__device__ __forceinline__ void ns_halves(const float (&f)[8], double factor, float ff, uint4 &hi, uint4 &lo)
 {
-    const bool normal = factor < 3.0e38 && factor > 1.2e-38;   // the factor is a normal FP32 number
-    const float ff = (float)factor;
+    const bool normal = ff < 3.0e38f && ff > 1.2e-38f;   // ff, the factor in FP32, is a normal number
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float w = normal ? f[e] * ff : (float)((double)f[e] * factor);
-        hi.set(e, w);
-        lo.set(e, w - hi.get(e));
+    for (int e = 0; e < 4; ++e) {
+        const float u = normal ? f[2 * e] * ff : (float)((double)f[2 * e] * factor), v = normal ? f[2 * e + 1] * ff : (float)((double)f[2 * e + 1] * factor);
+        const uint32_t p = half_pack<__half>::pack(u, v);
+        const float2 r = ns_two(p);
+        (&hi.x)[e] = p;
+        (&lo.x)[e] = half_pack<__half>::pack(u - r.x, v - r.y);
     }
 }
 // The matrix is taken as one row of `count` elements.
@@ -115,10 +117,7 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
         const unsigned r = n < 0xffffffffU ? (unsigned)i / octets : (unsigned)(i / octets), c = (unsigned)(i - (size_t)r * octets) * 8U;
         float v[8];
         ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
-        gdb_vec8<__half> a, b;
-        ns_halves(v, f, a, b);
-        h[i] = a.raw;
-        l[i] = b.raw;
+        ns_halves(v, f, (float)f, h[i], l[i]);
     }
 }
 
@@ -180,8 +179,6 @@ __device__ __forceinline__ void ns_store_row(void *base, const uint32_t *w, uint
         }
     }
 }
-__device__ __forceinline__ float2 ns_two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
-
 // the inputs of a piece, on their way while its products are formed
 template <int MODE, int COLS>
 __device__ __forceinline__ void ns_load_piece(ns_row<COLS> &in, ns_row<COLS> &lo, const ns_shape &sh, uint32_t row, uint32_t col0, uint32_t z)
@@ -624,8 +621,8 @@ bool ns_operand(CUtensorMap *m, const ns_tensor &t, uint64_t batch, bool mn, uin
 // halves, and forms its part of A; the parts are added over distributed shared memory (every CTA a share of the rows, then the sum to
 // all), P is formed by every CTA for itself, and the CTA's columns are updated in place. Two exchanges a step in place of three launches
 // that would each occupy a handful of SMs: 17 launches take the host 57 us alone.
-constexpr int NT_M = 128, NT_W = 256, NT_THREADS = 256, NT_MAX_CTAS = 16;
-constexpr int NT_X_BYTES = NT_M * NT_W * 2, NT_A_BYTES = NT_M * NT_M * 2, NT_PARTS = NT_M * NT_M * 4;   // (P takes the place of the parts)
+constexpr int NT_M = 128, NT_W = 256, NT_THREADS = 512, NT_WARPS = NT_THREADS / 32, NT_MAX_CTAS = 16;
+constexpr int NT_X_BYTES = NT_M * NT_W * 2, NT_A_BYTES = NT_M * NT_M * 2, NT_PARTS = NT_M * NT_M * 4;
 constexpr int NT_SMEM = 2 * NT_X_BYTES + NT_A_BYTES + NT_PARTS + 512 + 1024;
 
 // element (row, col) of a tile of 128 rows in blocks of 64 columns, 128-byte swizzle: the 16 bytes that hold columns 8 * octet ...
@@ -634,39 +631,44 @@ __device__ __forceinline__ void nt_fence() { asm volatile("fence.proxy.async;" :
 
 template <typename T, typename TOUT>
 __global__ void __launch_bounds__(NT_THREADS, 1)
-ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols, uint32_t steps, float ca, float cb, float cc, float eps, bool vec, int *err_flag)
+ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols, uint32_t steps, float ca, float cb, float cc, float eps, bool vec, bool vec_out, int *err_flag)
 {
     gdb_pdl_sync();
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
-    unsigned char *xh = smem, *xl = xh + NT_X_BYTES, *sa = xl + NT_X_BYTES, *parts = sa + NT_A_BYTES;   // hi, lo, A, parts of A (then P)
+    unsigned char *xh = smem, *xl = xh + NT_X_BYTES, *sa = xl + NT_X_BYTES, *parts = sa + NT_A_BYTES;   // hi, lo, A (then P), parts of A
     double *sums = reinterpret_cast<double *>(parts + NT_PARTS);                                        // [CTAs], then the warps' sums
-    uint64_t *bar = reinterpret_cast<uint64_t *>(sums + NT_MAX_CTAS + 8);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 1);
+    uint64_t *bar = reinterpret_cast<uint64_t *>(sums + NT_MAX_CTAS + NT_WARPS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 3);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), ctas = gridDim.x, z = blockIdx.y;   // (one cluster per matrix: grid.x is its size)
     const bool tall = rows > cols;
     const uint32_t m = tall ? cols : rows, n = tall ? rows : cols;
     const uint32_t width = ((n + ctas - 1U) / ctas + 63U) & ~63U, j0 = rank * width;   // columns of X here (multiples of 64)
-    const uint32_t done = smem_u32(bar);
+    const uint32_t done = smem_u32(bar), got_parts = done + 8U, got_sum = done + 16U;
     if (threadIdx.x == 0) {
-        mbar_init(done, 1);
+        for (int k = 0; k < 3; ++k) mbar_init(done + 8 * k, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512U) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const T *x = g + (size_t)z * rows * cols;
     // eight columns of a row: contiguous in memory, or one from each of eight rows of a tall matrix (neighbouring threads take
-    // neighbouring elements of those)
+    // neighbouring elements of those). A thread visits the same octets when it loads, splits and stores.
     const uint32_t octets = width / 8U;
     auto place = [&](uint32_t i, uint32_t &row, uint32_t &octet) {
         row = tall ? i % NT_M : i / octets;
         octet = tall ? i / NT_M : i % octets;
     };
-    auto load = [&](uint32_t row, uint32_t octet, float (&f)[8]) {
+    const T *x = g + (size_t)z * rows * cols;
+    double t = 0.0;
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < NT_M * octets; i += NT_THREADS) {
+        uint32_t row, octet;
+        place(i, row, octet);
         const uint32_t j = j0 + octet * 8U;
+        float f[8];
         if (row >= m || j >= n) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = 0.0f;
@@ -676,15 +678,10 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
         } else {
             ns_load8(x + (size_t)row * cols + j, n - j, vec, f);
         }
-    };
-    double t = 0.0;
-#pragma unroll 2
-    for (uint32_t i = threadIdx.x; i < NT_M * octets; i += NT_THREADS) {
-        uint32_t row, octet;
-        place(i, row, octet);
-        float f[8];
-        load(row, octet, f);
         t += ns_squares(f);
+        // as they are, four and four in the places of the two halves
+        *reinterpret_cast<float4 *>(xh + nt_at(row, octet)) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4 *>(xl + nt_at(row, octet)) = make_float4(f[4], f[5], f[6], f[7]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
@@ -696,7 +693,7 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
     cluster_sync_all();                 // (every CTA of the cluster runs before its memory is written)
     if (threadIdx.x < ctas) {
         double s = 0.0;
-        for (int w = 0; w < 8; ++w) s += sums[NT_MAX_CTAS + w];
+        for (int w = 0; w < NT_WARPS; ++w) s += sums[NT_MAX_CTAS + w];
         asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_shared(smem_u32(sums + rank), threadIdx.x)), "l"(__double_as_longlong(s)) : "memory");
     }
     __syncwarp();
@@ -708,17 +705,16 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
     for (uint32_t i = threadIdx.x; i < NT_M * octets; i += NT_THREADS) {
         uint32_t row, octet;
         place(i, row, octet);
-        float f[8];
-        load(row, octet, f);
-        gdb_vec8<__half> h, l;
-        ns_halves(f, factor, h, l);
-        *reinterpret_cast<uint4 *>(xh + nt_at(row, octet)) = h.raw;
-        *reinterpret_cast<uint4 *>(xl + nt_at(row, octet)) = l.raw;
+        const float4 a = *reinterpret_cast<const float4 *>(xh + nt_at(row, octet)), b = *reinterpret_cast<const float4 *>(xl + nt_at(row, octet));
+        const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        ns_halves(f, factor, (float)factor, *reinterpret_cast<uint4 *>(xh + nt_at(row, octet)), *reinterpret_cast<uint4 *>(xl + nt_at(row, octet)));
     }
 
-    const int quad = warp & 3, half = warp >> 2;
+    // a thread's row of A, P and X (tensor-memory lane) and its columns: 32 of every 128
+    const int quad = warp & 3, part = warp >> 2;
     const uint32_t row = quad * 32 + lane, tlane = (uint32_t)(quad * 32) << 16;
     const uint32_t share = NT_M / ctas;   // rows of A that this CTA adds up
+    constexpr float DOWN2 = NS_DOWN * NS_DOWN;
     uint32_t phase = 0;
     bool ok = true;
     // the products of a phase, by one thread, and the wait for them by all
@@ -749,24 +745,31 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
     for (uint32_t step = 0; step < steps; ++step) {
         // this CTA's part of A = X X^T
         products(tmem + 256U, smem_u32(xh), smem_u32(xh), false, NT_M, width / BK, NT_M * 128U);
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + tlane + 256U + part * 32, v);
         if (ctas > 1U) {
-            // no CTA of the cluster still reads its P, which lies where the parts go
-            cluster_sync_all();
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem + tlane + 256U + half * 64 + c * 32, v);
-                const uint32_t to = mapa_shared(smem_u32(parts) + (rank * share + row % share) * 512U, row / share);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t at = to + (((uint32_t)(half * 16 + c * 8 + k) ^ (row & 7U)) << 4);
-                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[4 * k]), "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3]) : "memory");
-                }
+            // Sent with their completion counted at the receiver, 64 KB of parts and 32 KB of sums a step. Nobody is overrun: parts
+            // of the next step are sent by those who have all of this step's sums, sums by those who have all parts.
+            if (threadIdx.x == 0) {
+                mbar_expect_tx(got_parts, NT_PARTS);
+                mbar_expect_tx(got_sum, NT_A_BYTES);
             }
-            cluster_sync_all();
+            const uint32_t to = mapa_shared(smem_u32(parts) + (rank * share + row % share) * 512U, row / share), to_bar = mapa_shared(got_parts, row / share);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t at = to + (((uint32_t)(part * 8 + k) ^ (row & 7U)) << 4);
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(v[4 * k]), "r"(v[4 * k + 1]),
+                             "r"(v[4 * k + 2]), "r"(v[4 * k + 3]), "r"(to_bar)
+                             : "memory");
+            }
+            if (ok && !mbar_wait(got_parts, step & 1U)) {
+                ok = false;
+                atomicExch(err_flag, 722);
+            }
             for (uint32_t i = threadIdx.x; i < share * 32U; i += NT_THREADS) {
                 const uint32_t r = i / 32U, c4 = i % 32U, to_row = rank * share + r;
                 float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
                 for (uint32_t k = 0; k < ctas; ++k) {
                     const float4 p = *reinterpret_cast<const float4 *>(parts + (k * share + r) * 512U + ((c4 ^ (r & 7U)) << 4));
                     s.x += p.x;
@@ -774,73 +777,64 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
                     s.z += p.z;
                     s.w += p.w;
                 }
-                constexpr float DOWN2 = NS_DOWN * NS_DOWN;
                 const uint32_t w0 = half_pack<__half>::pack(s.x * DOWN2, s.y * DOWN2), w1 = half_pack<__half>::pack(s.z * DOWN2, s.w * DOWN2);
                 const uint32_t at = smem_u32(sa) + nt_at(to_row, c4 >> 1) + (c4 & 1U) * 8U;
                 for (uint32_t k = 0; k < ctas; ++k) {
-                    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(at, (rank + k) % ctas)), "r"(w0), "r"(w1) : "memory");
+                    const uint32_t dst = (rank + k) % ctas;
+                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(mapa_shared(at, dst)), "r"(w0), "r"(w1),
+                                 "r"(mapa_shared(got_sum, dst))
+                                 : "memory");
                 }
             }
-            nt_fence();
+            if (ok && !mbar_wait(got_sum, step & 1U)) {
+                ok = false;
+                atomicExch(err_flag, 723);
+            }
             __syncwarp();
-            cluster_sync_all();
         } else {
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem + tlane + 256U + half * 64 + c * 32, v);
-                constexpr float DOWN2 = NS_DOWN * NS_DOWN;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = half_pack<__half>::pack(__uint_as_float(v[8 * k + 2 * e]) * DOWN2, __uint_as_float(v[8 * k + 2 * e + 1]) * DOWN2);
-                    *reinterpret_cast<uint4 *>(sa + nt_at(row, half * 8 + c * 4 + k)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
-        // P = b A + c A A (A is symmetric: rows serve as columns)
-        products(tmem + 384U, smem_u32(sa), smem_u32(sa), false, NT_M, 2U, NT_M * 128U);
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(tmem + tlane + 384U + half * 64 + c * 32, v);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t at = nt_at(row, half * 8 + c * 4 + k);
-                const uint4 a = *reinterpret_cast<const uint4 *>(sa + at);
                 uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = ns_two((&a.x)[e]);
-                    w[e] = half_pack<__half>::pack(fmaf(cb, f.x, cc * __uint_as_float(v[8 * k + 2 * e])), fmaf(cb, f.y, cc * __uint_as_float(v[8 * k + 2 * e + 1])));
-                }
-                *reinterpret_cast<uint4 *>(parts + at) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int e = 0; e < 4; ++e) w[e] = half_pack<__half>::pack(__uint_as_float(v[8 * k + 2 * e]) * DOWN2, __uint_as_float(v[8 * k + 2 * e + 1]) * DOWN2);
+                *reinterpret_cast<uint4 *>(sa + nt_at(row, part * 4 + k)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
+        // P = b A + c A A in the place of A (which is symmetric: rows serve as columns). The other CTAs write the next A there only after
+        // this one has sent its next part, behind the products that read P.
+        products(tmem + 384U, smem_u32(sa), smem_u32(sa), false, NT_M, 2U, NT_M * 128U);
+        tmem_ld_32x32b_x32(tmem + tlane + 384U + part * 32, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t at = nt_at(row, part * 4 + k);
+            const uint4 a = *reinterpret_cast<const uint4 *>(sa + at);
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = ns_two((&a.x)[e]);
+                w[e] = half_pack<__half>::pack(fmaf(cb, f.x, cc * __uint_as_float(v[8 * k + 2 * e])), fmaf(cb, f.y, cc * __uint_as_float(v[8 * k + 2 * e + 1])));
+            }
+            *reinterpret_cast<uint4 *>(sa + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
         // X <- a X + P X, this CTA's columns
-        products(tmem, smem_u32(parts), smem_u32(xh), true, width, 2U, BK * 128U);
+        products(tmem, smem_u32(sa), smem_u32(xh), true, width, 2U, BK * 128U);
         const bool last = step + 1U == steps;
+        const f32x2 ca2 = f2_make(ca, ca);
 #pragma unroll 1
-        for (uint32_t c = half * 32U; c < width; c += 64U) {
-            uint32_t v[32];
+        for (uint32_t c = part * 32U; c < width; c += 128U) {
             tmem_ld_32x32b_x32(tmem + tlane + c, v);
-            TOUT *o = out + (size_t)z * rows * cols;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t at = nt_at(row, c / 8U + k);
                 const uint4 h = *reinterpret_cast<const uint4 *>(xh + at), l = *reinterpret_cast<const uint4 *>(xl + at);
-                uint4 nh, nl;
+                uint4 nh, nl = make_uint4(0U, 0U, 0U, 0U);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 a = ns_two((&h.x)[e]), b = ns_two((&l.x)[e]);
-                    const float f0 = fmaf(ca, a.x + b.x, __uint_as_float(v[8 * k + 2 * e])), f1 = fmaf(ca, a.y + b.y, __uint_as_float(v[8 * k + 2 * e + 1]));
-                    const uint32_t j = j0 + c + k * 8U + e * 2U;
+                    float f0, f1;
+                    f2_split(f2_fma(ca2, f2_add(f2_make(a.x, a.y), f2_make(b.x, b.y)), f2_make(__uint_as_float(v[8 * k + 2 * e]), __uint_as_float(v[8 * k + 2 * e + 1]))), f0, f1);
                     if (last) {
-                        if (row < m) {
-                            if (j < n) gdb_io<TOUT>::st(o, tall ? (size_t)j * cols + row : (size_t)row * cols + j, f0 * NS_DOWN);
-                            if (j + 1U < n) gdb_io<TOUT>::st(o, tall ? (size_t)(j + 1U) * cols + row : (size_t)row * cols + j + 1U, f1 * NS_DOWN);
-                        }
+                        (&nh.x)[e] = half_pack<TOUT>::pack(f0 * NS_DOWN, f1 * NS_DOWN);
                     } else {
                         const uint32_t p = half_pack<__half>::pack(f0, f1);
                         const float2 r = ns_two(p);
@@ -848,11 +842,29 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
                         (&nl.x)[e] = half_pack<__half>::pack(f0 - r.x, f1 - r.y);
                     }
                 }
-                if (!last) {
-                    *reinterpret_cast<uint4 *>(xh + at) = nh;
-                    *reinterpret_cast<uint4 *>(xl + at) = nl;
-                }
+                *reinterpret_cast<uint4 *>(xh + at) = nh;
+                if (!last) *reinterpret_cast<uint4 *>(xl + at) = nl;
             }
+        }
+    }
+    // the result lies in the place of hi
+    __syncthreads();
+    TOUT *o = out + (size_t)z * rows * cols;
+#pragma unroll 2
+    for (uint32_t i = threadIdx.x; i < NT_M * octets; i += NT_THREADS) {
+        uint32_t r, octet;
+        place(i, r, octet);
+        const uint32_t j = j0 + octet * 8U;
+        if (r >= m || j >= n) continue;
+        const uint4 w = *reinterpret_cast<const uint4 *>(xh + nt_at(r, octet));
+        if (!tall && vec_out) {
+            *reinterpret_cast<uint4 *>(o + (size_t)r * cols + j) = w;
+            continue;
+        }
+        unsigned short *p = reinterpret_cast<unsigned short *>(o) + (tall ? (size_t)j * cols + r : (size_t)r * cols + j);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (j + e < n) p[tall ? (size_t)e * cols : (size_t)e] = (unsigned short)((&w.x)[e >> 1] >> (16 * (e & 1)));
         }
     }
     __syncwarp();
@@ -892,7 +904,8 @@ gd_status ns_launch_tile(gd_backend *be, const void *g, void *out, const gdb200_
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     const bool vec = a->cols % 8U == 0U && (uintptr_t)g % 16U == 0U;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T *)g, (TOUT *)out, (uint32_t)a->rows, (uint32_t)a->cols, a->steps, a->a, a->b, a->c, a->eps, vec, be->err_flag);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T *)g, (TOUT *)out, (uint32_t)a->rows, (uint32_t)a->cols, a->steps, a->a, a->b, a->c, a->eps, vec,
+                                             a->cols % 8U == 0U && (uintptr_t)out % 16U == 0U, be->err_flag);
     if (e != cudaSuccess) {
         be->launches += 1U;
         return gdb_fail(be, e, "orthogonalize tile");
