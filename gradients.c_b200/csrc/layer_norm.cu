@@ -7,8 +7,10 @@
 // threads, 16 elements a thread, so that mean and variance are two passes over registers (no cancellation of sums of squares) and
 // x is read once. All sums are FP32.
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace {
+using namespace gdb_t5;
 
 constexpr int LN_EPT = 16;                       // elements of a row that a thread holds
 constexpr size_t LN_MAX_COLS = 512 * LN_EPT;     // rows that a group of one block's threads holds
@@ -19,20 +21,27 @@ template <typename T> struct ln_vec<T, 1> {
     static __device__ __forceinline__ void ld(const T *p, float (&f)[1]) { f[0] = gdb_io<T>::ld(p, 0); }
     static __device__ __forceinline__ void st(T *p, const float (&f)[1]) { gdb_io<T>::st(p, 0, f[0]); }
 };
+// (two 16-bit elements a conversion)
+template <typename T> __device__ __forceinline__ float2 ln_two(uint32_t w);
+template <> __device__ __forceinline__ float2 ln_two<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+template <> __device__ __forceinline__ float2 ln_two<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000U)); }
 template <typename T> struct ln_vec<T, 8> {
     static __device__ __forceinline__ void ld(const T *p, float (&f)[8])
     {
-        gdb_vec8<T> v;
-        v.raw = *reinterpret_cast<const uint4 *>(p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = v.get(e);
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        const float2 a = ln_two<T>(v.x), b = ln_two<T>(v.y), c = ln_two<T>(v.z), d = ln_two<T>(v.w);
+        f[0] = a.x;
+        f[1] = a.y;
+        f[2] = b.x;
+        f[3] = b.y;
+        f[4] = c.x;
+        f[5] = c.y;
+        f[6] = d.x;
+        f[7] = d.y;
     }
     static __device__ __forceinline__ void st(T *p, const float (&f)[8])
     {
-        gdb_vec8<T> v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v.set(e, f[e]);
-        *reinterpret_cast<uint4 *>(p) = v.raw;
+        *reinterpret_cast<uint4 *>(p) = make_uint4(half_pack<T>::pack(f[0], f[1]), half_pack<T>::pack(f[2], f[3]), half_pack<T>::pack(f[4], f[5]), half_pack<T>::pack(f[6], f[7]));
     }
 };
 template <> struct ln_vec<float, 4> {
@@ -156,6 +165,264 @@ layer_norm_fwd_long_kernel(const T *x, const T *__restrict__ w, const T *__restr
     }
 }
 
+// ---- rows streamed through shared memory: as many bytes on their way as HBM wants, whatever the registers hold ----
+// One block per SM walks over tiles of R rows. Bulk copies bring them into a ring, 16 warps work on them, a group of TPR threads per row as
+// in the kernel above, and write the result over the input, bulk copies take it away. Tiles begin on 16 bytes whatever the width is (R is
+// chosen so), so odd rows stream as even ones do: only the reads from shared memory are narrower. A last tile whose bytes are no
+// multiple of 16 is worked on in global memory. The first thread issues all copies between its rows (warps of their own would leave
+// 96 registers a thread for sums that need 110).
+constexpr int LN_WARPS = 16, LN_THREADS = LN_WARPS * 32, LN_MAX_STAGES = 8;
+constexpr size_t LN_RING_BYTES = 208U * 1024U;
+
+struct ln_stream {
+    const void *x, *g, *w, *b;   // g: backward only
+    void *out;                   // y, or dx
+    float2 *stats;               // written forward (may be NULL), read backward
+    float *partial;              // backward: [blocks, 2, cols], or NULL
+    size_t rows;
+    unsigned cols, tile_rows, tile_bytes, stages;
+    float eps;
+};
+
+// BWD: 0 forward, 1 backward, 2 backward into a gradient that is there. Streams: x, and g, and the old dx.
+template <typename T, int TPR, int VE, int BWD>
+__global__ void __launch_bounds__(LN_THREADS, 1)
+layer_norm_stream_kernel(const ln_stream a, int *err_flag)
+{
+    constexpr int NV = LN_EPT / VE, GROUPS = LN_THREADS / TPR, STREAMS = BWD + 1;
+    extern __shared__ __align__(128) unsigned char ring[];   // [stages][streams][tile_bytes], rounded up to 128
+    __shared__ __align__(8) uint64_t bars[2 * LN_MAX_STAGES];
+    __shared__ float2 sh[64];
+    const unsigned stages = a.stages, cols = a.cols;
+    const uint32_t full0 = smem_u32(bars), done0 = full0 + 8U * LN_MAX_STAGES;
+    const size_t slot_bytes = (a.tile_bytes + 127U) & ~127U, stage_bytes = slot_bytes * STREAMS;
+    const size_t tiles = (a.rows + a.tile_rows - 1U) / a.tile_rows;
+    if (threadIdx.x == 0) {
+        for (unsigned s = 0; s < stages; ++s) {
+            mbar_init(full0 + 8U * s, 1);
+            mbar_init(done0 + 8U * s, LN_WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    gdb_pdl_sync();
+    const T *x = reinterpret_cast<const T *>(a.x), *g = reinterpret_cast<const T *>(a.g), *w = reinterpret_cast<const T *>(a.w), *b = reinterpret_cast<const T *>(a.b);
+    T *out = reinterpret_cast<T *>(a.out);
+    // bytes of a tile that go by bulk copies: all or none
+    auto bulk_bytes = [&](size_t tile) {
+        const size_t left = a.rows - tile * a.tile_rows, bytes = (left < a.tile_rows ? left : a.tile_rows) * cols * sizeof(T);
+        return bytes % 16U == 0U ? (unsigned)bytes : 0U;
+    };
+    const bool leader = threadIdx.x == 0;
+    auto fetch = [&](size_t tile, unsigned s) {
+        const unsigned bytes = tile < tiles ? bulk_bytes(tile) : 0U;
+        if (bytes == 0U) return;
+        const size_t at = tile * a.tile_rows * cols;
+        const uint32_t dst = smem_u32(ring + s * stage_bytes), bar = full0 + 8U * s;
+        mbar_expect_tx(bar, STREAMS * bytes);
+        auto copy = [&](int k, const void *src) {
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + (uint32_t)(k * slot_bytes)), "l"(src), "r"(bytes),
+                         "r"(bar)
+                         : "memory");
+        };
+        copy(0, x + at);
+        if (BWD >= 1) copy(1, g + at);
+        if (BWD == 2) copy(2, out + at);
+    };
+    auto send = [&](size_t tile, unsigned s) {
+        if (out != nullptr) {
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + tile * a.tile_rows * cols), "r"(smem_u32(ring + s * stage_bytes)),
+                         "r"(bulk_bytes(tile))
+                         : "memory");
+        }
+        bulk_commit_group();
+    };
+    // stages - 2 tiles are on their way; a tile's stage is filled again two turns after its rows were done, when its results have been read
+    if (leader) {
+        for (unsigned k = 0; k + 2U < stages; ++k) fetch(blockIdx.x + (size_t)k * gridDim.x, k);
+    }
+    const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    float wf[NV][VE], bf[BWD ? 1 : NV][VE], dw[BWD ? NV : 1][VE], db[BWD ? NV : 1][VE];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const unsigned c = (t + j * TPR) * VE;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            wf[j][e] = w != nullptr ? 0.0f : 1.0f;
+            if (BWD) dw[BWD ? j : 0][e] = db[BWD ? j : 0][e] = 0.0f; else bf[BWD ? 0 : j][e] = 0.0f;
+        }
+        if (w != nullptr && c < cols) ln_vec<T, VE>::ld(w + c, wf[j]);
+        if (!BWD && b != nullptr && c < cols) ln_vec<T, VE>::ld(b + c, bf[BWD ? 0 : j]);
+    }
+    const float inv_cols = 1.0f / (float)cols;
+    unsigned flip = 0;
+    // one row; dead groups go along (shuffles and barriers are the whole warp's)
+    auto work = [&](size_t row, bool live, const T *px, const T *pg, const T *pd, T *po) {
+        float h[NV][VE], gf[BWD ? NV : 1][VE];
+        float2 st = make_float2(0.0f, 0.0f), s = make_float2(0.0f, 0.0f);
+        if (BWD && live) st = __ldg(&a.stats[row]);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const unsigned c = (t + j * TPR) * VE;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                h[j][e] = 0.0f;
+                if (BWD) gf[BWD ? j : 0][e] = 0.0f;
+            }
+            if (live && c < cols) {
+                ln_vec<T, VE>::ld(px + c, h[j]);
+                if (BWD) ln_vec<T, VE>::ld(pg + c, gf[BWD ? j : 0]);
+            }
+        }
+        if (BWD) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    float &gj = gf[BWD ? j : 0][e];
+                    h[j][e] = (h[j][e] - st.x) * st.y;
+                    dw[BWD ? j : 0][e] += gj * h[j][e];
+                    db[BWD ? j : 0][e] += gj;
+                    gj *= wf[j][e];
+                    s.x += gj;
+                    s.y += gj * h[j][e];
+                }
+            }
+            s = ln_group_sum<TPR>(s, sh, flip);
+            flip ^= 1U;
+            const float c1 = s.x * inv_cols, c2 = s.y * inv_cols;
+            if (live && po != nullptr) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const unsigned c = (t + j * TPR) * VE;
+                    if (c < cols) {
+                        float o[VE];
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) o[e] = __fmul_rn(st.y, gf[BWD ? j : 0][e] - c1 - h[j][e] * c2);   // (never fused with the addition below)
+                        if (BWD == 2) {
+                            // round, add, round: the entry without accumulation followed by gd_backend_accumulate
+                            float d[VE];
+                            ln_vec<T, VE>::ld(pd + c, d);
+#pragma unroll
+                            for (int e = 0; e < VE; ++e) o[e] = d[e] + gdb_io<T>::rnd(o[e]);
+                        }
+                        ln_vec<T, VE>::st(po + c, o);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) s.x += h[j][e];
+            }
+            const float mean = ln_group_sum<TPR>(s, sh, flip).x * inv_cols;
+            s = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if ((t + j * TPR) * VE < cols) {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        h[j][e] -= mean;
+                        s.x += h[j][e] * h[j][e];
+                    }
+                }
+            }
+            const float inv = rsqrtf(ln_group_sum<TPR>(s, sh, flip ^ 1U).x * inv_cols + a.eps);
+            if (live) {
+                if (a.stats != nullptr && t == 0) a.stats[row] = make_float2(mean, inv);
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const unsigned c = (t + j * TPR) * VE;
+                    if (c < cols) {
+                        float o[VE];
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) o[e] = fmaf(h[j][e] * inv, wf[j][e], bf[BWD ? 0 : j][e]);
+                        ln_vec<T, VE>::st(po + c, o);
+                    }
+                }
+            }
+        }
+    };
+    unsigned s = 0, ph = 0, done_ph = 0, turn = 0;   // done_ph: bit k, parity of stage k's next completion
+    bool ok = true;
+    size_t sent_to = blockIdx.x;                     // (leader) the first tile whose results have not been sent off
+    auto pass_on = [&](unsigned before) {
+        if (ok && !mbar_wait(done0 + 8U * before, (done_ph >> before) & 1U)) {
+            ok = false;
+            atomicExch(err_flag, 602);
+        }
+        done_ph ^= 1U << before;
+        send(sent_to, before);
+        sent_to += gridDim.x;
+    };
+    for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
+        const size_t row0 = tile * a.tile_rows, left = a.rows - row0;
+        const unsigned here = left < a.tile_rows ? (unsigned)left : a.tile_rows;
+        if (bulk_bytes(tile) == 0U) {
+            for (unsigned r = group; r < a.tile_rows; r += GROUPS) {
+                const size_t at = (row0 + (r < here ? r : 0U)) * cols;
+                work(row0 + r, r < here, x + at, g + at, out + at, out == nullptr ? nullptr : out + at);
+            }
+            break;
+        }
+        if (leader) {
+            const unsigned before = s == 0U ? stages - 1U : s - 1U;
+            if (turn >= 1U) pass_on(before);
+            bulk_wait_group_read<1>();
+            fetch(tile + (size_t)(stages - 2U) * gridDim.x, (s + stages - 2U) % stages);
+        }
+        // (a wait that gives up is not waited for again, and the walk goes on: the groups' barriers stay complete)
+        if (ok && !mbar_wait(full0 + 8U * s, ph)) {
+            ok = false;
+            atomicExch(err_flag, 603);
+        }
+        __syncwarp();
+        T *sx = reinterpret_cast<T *>(ring + s * stage_bytes), *sg = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD >= 1 ? slot_bytes : 0U)),
+          *sd = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD == 2 ? 2U * slot_bytes : 0U));
+        for (unsigned r = group; r < a.tile_rows; r += GROUPS) {
+            const unsigned at = (r < here ? r : 0U) * cols;
+            work(row0 + r, r < here, sx + at, sg + at, sd + at, out == nullptr ? nullptr : sx + at);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(done0 + 8U * s) : "memory");
+        if (++s == stages) {
+            s = 0;
+            ph ^= 1U;
+        }
+    }
+    if (leader) {
+        // (turn tiles went through the ring)
+        if (turn >= 1U) pass_on(s == 0U ? stages - 1U : s - 1U);
+        bulk_wait_all();
+    }
+    if (BWD && a.partial != nullptr) {
+        // the groups' sums through the ring (64 KB), added in order
+        __syncthreads();
+        float *sums = reinterpret_cast<float *>(ring) + (size_t)group * 2U * cols;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const unsigned c = (t + j * TPR) * VE;
+            if (c < cols) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    sums[c + e] = dw[BWD ? j : 0][e];
+                    sums[cols + c + e] = db[BWD ? j : 0][e];
+                }
+            }
+        }
+        __syncthreads();
+        sums = reinterpret_cast<float *>(ring);
+        for (unsigned c = threadIdx.x; c < 2U * cols; c += LN_THREADS) {
+            float v = 0.0f;
+#pragma unroll 8
+            for (unsigned k = 0; k < GROUPS; ++k) v += sums[(size_t)k * 2U * cols + c];
+            a.partial[(size_t)blockIdx.x * 2U * cols + c] = v;
+        }
+    }
+}
+
 // Input gradient and this block's share of the weight's and the bias's gradient from one pass over x and g. Groups of TPR threads walk
 // over the rows; the thread's columns of dw and db stay in its registers, the block's sums go to partial[block, 2, cols].
 constexpr int LN_BWD_THREADS = 512;
@@ -166,7 +433,7 @@ layer_norm_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const fl
 {
     gdb_pdl_sync();
     constexpr int NV = LN_EPT / VE, GROUPS = LN_BWD_THREADS / TPR;
-    extern __shared__ float sums[];   // [2, cols]
+    extern __shared__ float sums[];   // [groups, 2, cols]
     __shared__ float2 sh[64];
     const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     float wf[NV][VE], dw[NV][VE], db[NV][VE];
@@ -237,24 +504,26 @@ layer_norm_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const fl
         }
     }
     if (partial == nullptr) return;
-    // groups in order
-    for (unsigned gr = 0; gr < GROUPS; ++gr) {
-        if (gr == group) {
+    // the groups' sums, added in order
+    float *mine = sums + (size_t)group * 2U * cols;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const unsigned c = (t + j * TPR) * VE;
-                if (c < cols) {
+    for (int j = 0; j < NV; ++j) {
+        const unsigned c = (t + j * TPR) * VE;
+        if (c < cols) {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        sums[c + e] = (gr == 0 ? 0.0f : sums[c + e]) + dw[j][e];
-                        sums[cols + c + e] = (gr == 0 ? 0.0f : sums[cols + c + e]) + db[j][e];
-                    }
-                }
+            for (int e = 0; e < VE; ++e) {
+                mine[c + e] = dw[j][e];
+                mine[cols + c + e] = db[j][e];
             }
         }
-        __syncthreads();
     }
-    for (unsigned c = threadIdx.x; c < 2U * cols; c += LN_BWD_THREADS) partial[(size_t)blockIdx.x * 2U * cols + c] = sums[c];
+    __syncthreads();
+    for (unsigned c = threadIdx.x; c < 2U * cols; c += LN_BWD_THREADS) {
+        float v = 0.0f;
+#pragma unroll 8
+        for (unsigned k = 0; k < GROUPS; ++k) v += sums[(size_t)k * 2U * cols + c];
+        partial[(size_t)blockIdx.x * 2U * cols + c] = v;
+    }
 }
 
 // Rows of more than LN_MAX_COLS elements.
@@ -303,26 +572,26 @@ layer_norm_columns_long_kernel(const T *__restrict__ x, const float2 *__restrict
     partial[(size_t)blockIdx.y * 2U * cols + cols + c] = db;
 }
 
-// dw[c] and db[c]: the blocks' partial sums in a fixed order (eight threads a column, every eighth block each), rounded once.
+// dw[c] and db[c]: the blocks' partial sums in a fixed order (32 threads a column, every 32nd block each: one load's latency), rounded once.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 layer_norm_merge_kernel(const float *__restrict__ partial, T *__restrict__ dw, T *__restrict__ db, unsigned blocks, size_t cols)
 {
     gdb_pdl_sync();
-    __shared__ float sh[8][33];
+    __shared__ float sh[32][33];
     const unsigned lane = threadIdx.x & 31, part = threadIdx.x >> 5;
     const size_t c = (size_t)blockIdx.x * 32U + lane;
     float s = 0.0f;
     if (c < 2U * cols) {
-#pragma unroll 4
-        for (unsigned k = part; k < blocks; k += 8U) s += __ldcg(&partial[(size_t)k * 2U * cols + c]);
+#pragma unroll 8
+        for (unsigned k = part; k < blocks; k += 32U) s += __ldcg(&partial[(size_t)k * 2U * cols + c]);
     }
     sh[part][lane] = s;
     __syncthreads();
     if (part == 0 && c < 2U * cols) {
         float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v += sh[k][lane];
+        for (int k = 0; k < 32; ++k) v += sh[k][lane];
         if (c < cols) {
             if (dw != nullptr) gdb_io<T>::st(dw, c, v);
         } else if (db != nullptr) {
@@ -350,9 +619,59 @@ struct ln_call {
      : a.cols <= 256U * LN_EPT  ? GO(256, VE)                                                                                                                 \
                                 : GO(512, VE))
 
+// Tiles of the streaming kernel: rows for all groups of a block, more where rows are short (16 KB a tile keep the copies large) or where
+// the tile would not begin on 16 bytes; false where three stages of them do not fit, the pointers are not aligned, or there are too few
+// tiles for the ring to be of use (below two a block the direct kernels have the shorter way).
+template <typename T, int TPR>
+bool ln_tiles(const gd_backend *be, const ln_call &a, int streams, ln_stream *st, unsigned *blocks)
+{
+    constexpr unsigned GROUPS = LN_THREADS / TPR;
+    if (((uintptr_t)a.x | (uintptr_t)a.g | (uintptr_t)(streams == 1 ? a.out : a.dx)) % 16U != 0U) return false;
+    size_t r = GROUPS;
+    while (r * a.cols * sizeof(T) % 16U != 0U || (r < 8U * GROUPS && 2U * r * a.cols * sizeof(T) <= 16384U)) r *= 2U;
+    const size_t bytes = r * a.cols * sizeof(T), slot = (bytes + 127U) & ~(size_t)127U;
+    const size_t stages = LN_RING_BYTES / (slot * streams), tiles = (a.rows + r - 1U) / r;
+    if (stages < 3U || tiles < 2U * (size_t)be->sm_count) return false;
+    st->tile_rows = (unsigned)r;
+    st->tile_bytes = (unsigned)bytes;
+    st->stages = (unsigned)(stages < LN_MAX_STAGES ? stages : LN_MAX_STAGES);
+    *blocks = (unsigned)(tiles < (size_t)be->sm_count ? tiles : (size_t)be->sm_count);
+    return true;
+}
+template <typename T, int TPR, int VE, int BWD>
+gd_status stream_go(gd_backend *be, const ln_stream &st, unsigned blocks)
+{
+    static bool ready = false;
+    if (!ready) {
+        const cudaError_t e = cudaFuncSetAttribute(layer_norm_stream_kernel<T, TPR, VE, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LN_RING_BYTES);
+        if (e != cudaSuccess) return gdb_fail(be, e, "layer_norm smem attribute");
+        ready = true;
+    }
+    gdb_launch(layer_norm_stream_kernel<T, TPR, VE, BWD>, blocks, LN_THREADS, LN_RING_BYTES, be->stream, st, be->err_flag);
+    return gdb_launched(be, BWD ? "layer_norm_backward" : "layer_norm_forward");
+}
+ln_stream ln_stream_of(const ln_call &a, bool backward, float *partial)
+{
+    ln_stream st = {};
+    st.x = a.x;
+    st.g = a.g;
+    st.w = a.w;
+    st.b = a.b;
+    st.out = backward ? a.dx : a.out;
+    st.stats = a.stats;
+    st.partial = partial;
+    st.rows = a.rows;
+    st.cols = (unsigned)a.cols;
+    st.eps = a.eps;
+    return st;
+}
+
 template <typename T, int TPR, int VE>
 gd_status fwd_go(gd_backend *be, const ln_call &a)
 {
+    ln_stream stream = ln_stream_of(a, false, nullptr);
+    unsigned stream_blocks;
+    if (VE == 1 && ln_tiles<T, TPR>(be, a, 1, &stream, &stream_blocks)) return stream_go<T, TPR, VE, 0>(be, stream, stream_blocks);
     constexpr unsigned THREADS = TPR > 256 ? TPR : 256, PER = THREADS / TPR;
     const size_t blocks = (a.rows + PER - 1U) / PER;
     if (blocks > 0x7fffffffU) return GD_ERR_UNSUPPORTED;
@@ -379,13 +698,17 @@ gd_status fwd_typed(gd_backend *be, const ln_call &a)
 template <typename T, int TPR, int VE>
 gd_status bwd_go(gd_backend *be, const ln_call &a, float *partial, unsigned max_blocks, unsigned *blocks)
 {
+    ln_stream stream = ln_stream_of(a, true, partial);
+    if (max_blocks >= (unsigned)be->sm_count && ln_tiles<T, TPR>(be, a, a.add_to_dx ? 3 : 2, &stream, blocks)) {
+        return a.add_to_dx ? stream_go<T, TPR, VE, 2>(be, stream, *blocks) : stream_go<T, TPR, VE, 1>(be, stream, *blocks);
+    }
     constexpr unsigned PER = LN_BWD_THREADS / TPR;
     const size_t need = (a.rows + PER - 1U) / PER;
     *blocks = (unsigned)(need < max_blocks ? need : max_blocks);
-    const int smem = (int)(2U * a.cols * sizeof(float));
+    const int smem = (int)(PER * 2U * a.cols * sizeof(float));   // (64 KB at most)
     static bool ready = false;
     if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(layer_norm_bwd_kernel<T, TPR, VE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(2U * TPR * LN_EPT * sizeof(float)));
+        const cudaError_t e = cudaFuncSetAttribute(layer_norm_bwd_kernel<T, TPR, VE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(PER * 2U * TPR * LN_EPT * sizeof(float)));
         if (e != cudaSuccess) return gdb_fail(be, e, "layer_norm_backward smem attribute");
         ready = true;
     }
@@ -429,7 +752,7 @@ gd_status bwd_typed(gd_backend *be, const ln_call &a)
 #undef GO
     }
     if (st != GD_OK || !sums) return st;
-    gdb_launch(layer_norm_merge_kernel<T>, (unsigned)((2U * a.cols + 31U) / 32U), 256, 0, be->stream, (const float *)partial, (T *)a.dw, (T *)a.db, blocks, a.cols);
+    gdb_launch(layer_norm_merge_kernel<T>, (unsigned)((2U * a.cols + 31U) / 32U), 1024, 0, be->stream, (const float *)partial, (T *)a.dw, (T *)a.db, blocks, a.cols);
     return gdb_launched(be, "layer_norm_backward merge");
 }
 

@@ -89,7 +89,7 @@ def ln_check(got, ref, dtype):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=ids_of)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 512), (3, 7), (65, 64), (17, 129), (1000, 96), (33, 256), (2, 513), (301, 512), (4099, 24), (130, 1000), (77, 1003), (64, 2048),
-                                       (19, 4104), (5, 8191), (9, 8192), (4, 8193), (3, 20000)])
+                                       (19, 4104), (5, 8191), (9, 8192), (4, 8193), (3, 20000), (5003, 512), (4801, 515), (1301, 2048), (2403, 1003), (40011, 40), (700, 4104), (301, 8192)])
 def test_layer_norm(step, dtype, rows, cols):
     x, w, b, g = ln_data(rows, cols, dtype, rows * 7 + cols)
     ln_check(ln_call(step, x, w, b, g, dtype), ln_reference(x, w, b, g, 1e-5), dtype)
@@ -108,7 +108,7 @@ def test_layer_norm_without_weight_bias_or_statistics(step, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32], ids=ids_of)
-@pytest.mark.parametrize("rows,cols", [(70, 512), (70, 515), (3, 9000)])
+@pytest.mark.parametrize("rows,cols", [(70, 512), (70, 515), (3, 9000), (6000, 512), (4801, 515)])
 def test_layer_norm_backward_adds_into_a_gradient(step, dtype, rows, cols):
     x, w, b, g = ln_data(rows, cols, dtype, 11)
     old = rnd_np(np.random.default_rng(1).standard_normal((rows, cols)).astype(np.float32), dtype)
