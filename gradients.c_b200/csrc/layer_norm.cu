@@ -82,61 +82,94 @@ __device__ __forceinline__ float2 ln_group_sum(float2 v, float2 *sh, unsigned fl
     return v;
 }
 
-// One row per group, LN_FWD_THREADS / TPR rows per block. stats (may be NULL): mean and 1 / deviation of every row.
+// A thread's 16 elements of a row in pairs (sm_100 multiplies and adds two FP32 numbers an instruction): NV accesses of VE elements, TPR
+// accesses apart.
+template <typename T, int VE, int TPR> struct ln_pairs {
+    f32x2 v[LN_EPT / 2];
+    __device__ __forceinline__ void load(const T *p, unsigned t, unsigned cols, bool live, float other = 0.0f)
+    {
+        float f[LN_EPT];
+#pragma unroll
+        for (int j = 0; j < LN_EPT / VE; ++j) {
+            const unsigned c = (t + j * TPR) * VE;
+            float(&fj)[VE] = *reinterpret_cast<float(*)[VE]>(f + j * VE);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) fj[e] = other;
+            if (live && c < cols) ln_vec<T, VE>::ld(p + c, fj);
+        }
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) v[k] = f2_make(f[2 * k], f[2 * k + 1]);
+    }
+    // adds to the elements inside the row
+    __device__ __forceinline__ void center(f32x2 by, unsigned t, unsigned cols)
+    {
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) {
+            const f32x2 d = f2_add(v[k], by);
+            if (VE > 1) {
+                if ((t + (2 * k / VE) * TPR) * VE < cols) v[k] = d;
+            } else {
+                float lo, hi, l0, h0;
+                f2_split(d, lo, hi);
+                f2_split(v[k], l0, h0);
+                v[k] = f2_make(t + 2 * k * TPR < cols ? lo : l0, t + (2 * k + 1) * TPR < cols ? hi : h0);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *p, unsigned t, unsigned cols) const
+    {
+        float f[LN_EPT];
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) f2_split(v[k], f[2 * k], f[2 * k + 1]);
+#pragma unroll
+        for (int j = 0; j < LN_EPT / VE; ++j) {
+            const unsigned c = (t + j * TPR) * VE;
+            if (c < cols) ln_vec<T, VE>::st(p + c, *reinterpret_cast<const float(*)[VE]>(f + j * VE));
+        }
+    }
+};
+__device__ __forceinline__ float2 ln_halves(f32x2 s)
+{
+    float lo, hi;
+    f2_split(s, lo, hi);
+    return make_float2(lo + hi, 0.0f);
+}
+
+// One row per group, threads / TPR rows per block. stats (may be NULL): mean and 1 / deviation of every row.
 template <typename T, int TPR, int VE>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 layer_norm_fwd_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, T *out, float2 *__restrict__ stats, size_t rows, unsigned cols, float eps)
 {
     gdb_pdl_sync();
-    constexpr int NV = LN_EPT / VE, THREADS = TPR > 256 ? TPR : 256;
+    constexpr int THREADS = TPR > 256 ? TPR : 256;
     __shared__ float2 sh[64];
     const unsigned t = threadIdx.x % TPR;
     const size_t row = (size_t)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
     const bool live = row < rows;   // (groups within a warp stay together through the shuffles)
     const T *xr = x + (live ? row : 0) * cols;
-    float f[NV][VE];
-    float2 s = make_float2(0.0f, 0.0f);
+    ln_pairs<T, VE, TPR> f;
+    f.load(xr, t, cols, live);
+    f32x2 s2 = f2_make(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const unsigned c = (t + j * TPR) * VE;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) f[j][e] = 0.0f;
-        if (live && c < cols) ln_vec<T, VE>::ld(xr + c, f[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) s.x += f[j][e];
-    }
+    for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_add(s2, f.v[k]);
+    float2 s = ln_halves(s2);
     const float inv_cols = 1.0f / (float)cols;
     const float mean = ln_group_sum<TPR>(s, sh, 0).x * inv_cols;
-    s = make_float2(0.0f, 0.0f);
+    f.center(f2_make(-mean, -mean), t, cols);
+    s2 = f2_make(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        if ((t + j * TPR) * VE < cols) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                f[j][e] -= mean;
-                s.x += f[j][e] * f[j][e];
-            }
-        }
-    }
+    for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_fma(f.v[k], f.v[k], s2);
+    s = ln_halves(s2);
     const float inv = rsqrtf(ln_group_sum<TPR>(s, sh, 1).x * inv_cols + eps);
     if (!live) return;
     if (stats != nullptr && t == 0) stats[row] = make_float2(mean, inv);
-    T *orow = out + row * cols;
+    ln_pairs<T, VE, TPR> wf, bf;
+    wf.load(w, t, cols, w != nullptr, 1.0f);
+    bf.load(b, t, cols, b != nullptr);
+    const f32x2 inv2 = f2_make(inv, inv);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const unsigned c = (t + j * TPR) * VE;
-        if (c < cols) {
-            float wf[VE], bf[VE], o[VE];
-            if (w != nullptr) ln_vec<T, VE>::ld(w + c, wf);
-            if (b != nullptr) ln_vec<T, VE>::ld(b + c, bf);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) o[e] = fmaf(f[j][e] * inv, w != nullptr ? wf[e] : 1.0f, b != nullptr ? bf[e] : 0.0f);
-            ln_vec<T, VE>::st(orow + c, o);
-        }
-    }
+    for (int k = 0; k < LN_EPT / 2; ++k) f.v[k] = f2_fma(f2_mul(f.v[k], inv2), wf.v[k], bf.v[k]);
+    f.store(out + row * cols, t, cols);
 }
 
 // Rows of more than LN_MAX_COLS elements: a block per row that reads x three times (the second and third time from L2).
@@ -165,12 +198,75 @@ layer_norm_fwd_long_kernel(const T *x, const T *__restrict__ w, const T *__restr
     }
 }
 
+// a thread's sums of g h and of g over the rows, for its columns
+struct ln_sums {
+    f32x2 dw[LN_EPT / 2], db[LN_EPT / 2];
+    __device__ __forceinline__ ln_sums()
+    {
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) dw[k] = db[k] = f2_make(0.0f, 0.0f);
+    }
+    // to[0, c] and to[1, c]
+    template <int VE, int TPR> __device__ __forceinline__ void store(float *to, unsigned t, unsigned cols) const
+    {
+#pragma unroll
+        for (int q = 0; q < LN_EPT; ++q) {
+            const unsigned c = (t + (q / VE) * TPR) * VE + q % VE;
+            float a, b, u, v;
+            f2_split(dw[q / 2], a, b);
+            f2_split(db[q / 2], u, v);
+            if (c < cols) {
+                to[c] = q % 2 == 0 ? a : b;
+                to[cols + c] = q % 2 == 0 ? u : v;
+            }
+        }
+    }
+};
+// One row backward; dead groups go along (shuffles and barriers are the whole warp's). po may be px (or pg); pd: the old gradient.
+template <typename T, int VE, int TPR>
+__device__ __forceinline__ void ln_backward_row(const T *px, const T *pg, const T *pd, T *po, bool live, bool add, float2 st, const ln_pairs<T, VE, TPR> &wf, ln_sums &sums,
+                                                float inv_cols, unsigned t, unsigned cols, float2 *sh, unsigned &flip)
+{
+    ln_pairs<T, VE, TPR> h, g;
+    h.load(px, t, cols, live);
+    g.load(pg, t, cols, live);
+    const f32x2 mean2 = f2_make(-st.x, -st.x), inv2 = f2_make(st.y, st.y);
+    f32x2 s1 = f2_make(0.0f, 0.0f), s2 = s1;
+#pragma unroll
+    for (int k = 0; k < LN_EPT / 2; ++k) {
+        // (outside the row g is zero, and h whatever the mean makes of zero)
+        h.v[k] = f2_mul(f2_add(h.v[k], mean2), inv2);
+        sums.dw[k] = f2_fma(g.v[k], h.v[k], sums.dw[k]);
+        sums.db[k] = f2_add(sums.db[k], g.v[k]);
+        g.v[k] = f2_mul(g.v[k], wf.v[k]);
+        s1 = f2_add(s1, g.v[k]);
+        s2 = f2_fma(g.v[k], h.v[k], s2);
+    }
+    const float2 s = ln_group_sum<TPR>(make_float2(ln_halves(s1).x, ln_halves(s2).x), sh, flip);
+    flip ^= 1U;
+    if (!live || po == nullptr) return;
+    const f32x2 c1 = f2_make(-s.x * inv_cols, -s.x * inv_cols), c2 = f2_make(-s.y * inv_cols, -s.y * inv_cols);
+#pragma unroll
+    for (int k = 0; k < LN_EPT / 2; ++k) g.v[k] = f2_mul(inv2, f2_fma(h.v[k], c2, f2_add(g.v[k], c1)));
+    if (add) {
+        // round, add, round: the entry without accumulation followed by gd_backend_accumulate
+        h.load(pd, t, cols, true);
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) {
+            float a, b;
+            f2_split(g.v[k], a, b);
+            g.v[k] = f2_add(h.v[k], f2_make(gdb_io<T>::rnd(a), gdb_io<T>::rnd(b)));
+        }
+    }
+    g.store(po, t, cols);
+}
+
 // ---- rows streamed through shared memory: as many bytes on their way as HBM wants, whatever the registers hold ----
 // One block per SM walks over tiles of R rows. Bulk copies bring them into a ring, 16 warps work on them, a group of TPR threads per row as
 // in the kernel above, and write the result over the input, bulk copies take it away. Tiles begin on 16 bytes whatever the width is (R is
 // chosen so), so odd rows stream as even ones do: only the reads from shared memory are narrower. A last tile whose bytes are no
-// multiple of 16 is worked on in global memory. The first thread issues all copies between its rows (warps of their own would leave
-// 96 registers a thread for sums that need 110).
+// multiple of 16 is worked on in global memory. The warp that finishes a tile issues the copies (warps for that alone would leave 96
+// registers a thread for sums that need 110; one fixed warp among the 16 is waited for by all).
 constexpr int LN_WARPS = 16, LN_THREADS = LN_WARPS * 32, LN_MAX_STAGES = 8;
 constexpr size_t LN_RING_BYTES = 208U * 1024U;
 
@@ -189,18 +285,19 @@ template <typename T, int TPR, int VE, int BWD>
 __global__ void __launch_bounds__(LN_THREADS, 1)
 layer_norm_stream_kernel(const ln_stream a, int *err_flag)
 {
-    constexpr int NV = LN_EPT / VE, GROUPS = LN_THREADS / TPR, STREAMS = BWD + 1;
+    constexpr int GROUPS = LN_THREADS / TPR, STREAMS = BWD + 1;
     extern __shared__ __align__(128) unsigned char ring[];   // [stages][streams][tile_bytes], rounded up to 128
-    __shared__ __align__(8) uint64_t bars[2 * LN_MAX_STAGES];
+    __shared__ __align__(8) uint64_t bars[LN_MAX_STAGES];
+    __shared__ unsigned arrived[LN_MAX_STAGES];   // warps that are done with the stage's tile
     __shared__ float2 sh[64];
     const unsigned stages = a.stages, cols = a.cols;
-    const uint32_t full0 = smem_u32(bars), done0 = full0 + 8U * LN_MAX_STAGES;
+    const uint32_t full0 = smem_u32(bars);
     const size_t slot_bytes = (a.tile_bytes + 127U) & ~127U, stage_bytes = slot_bytes * STREAMS;
     const size_t tiles = (a.rows + a.tile_rows - 1U) / a.tile_rows;
     if (threadIdx.x == 0) {
         for (unsigned s = 0; s < stages; ++s) {
             mbar_init(full0 + 8U * s, 1);
-            mbar_init(done0 + 8U * s, LN_WARPS);
+            arrived[s] = 0U;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -213,7 +310,6 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         const size_t left = a.rows - tile * a.tile_rows, bytes = (left < a.tile_rows ? left : a.tile_rows) * cols * sizeof(T);
         return bytes % 16U == 0U ? (unsigned)bytes : 0U;
     };
-    const bool leader = threadIdx.x == 0;
     auto fetch = [&](size_t tile, unsigned s) {
         const unsigned bytes = tile < tiles ? bulk_bytes(tile) : 0U;
         if (bytes == 0U) return;
@@ -237,126 +333,42 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         }
         bulk_commit_group();
     };
-    // stages - 2 tiles are on their way; a tile's stage is filled again two turns after its rows were done, when its results have been read
-    if (leader) {
-        for (unsigned k = 0; k + 2U < stages; ++k) fetch(blockIdx.x + (size_t)k * gridDim.x, k);
+    if (threadIdx.x == 0) {
+        for (unsigned k = 0; k < stages; ++k) fetch(blockIdx.x + (size_t)k * gridDim.x, k);
     }
     const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    float wf[NV][VE], bf[BWD ? 1 : NV][VE], dw[BWD ? NV : 1][VE], db[BWD ? NV : 1][VE];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const unsigned c = (t + j * TPR) * VE;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            wf[j][e] = w != nullptr ? 0.0f : 1.0f;
-            if (BWD) dw[BWD ? j : 0][e] = db[BWD ? j : 0][e] = 0.0f; else bf[BWD ? 0 : j][e] = 0.0f;
-        }
-        if (w != nullptr && c < cols) ln_vec<T, VE>::ld(w + c, wf[j]);
-        if (!BWD && b != nullptr && c < cols) ln_vec<T, VE>::ld(b + c, bf[BWD ? 0 : j]);
-    }
+    ln_pairs<T, VE, TPR> wf, bf;
+    wf.load(w, t, cols, w != nullptr, 1.0f);
+    if (!BWD) bf.load(b, t, cols, b != nullptr);
+    ln_sums sums2;
     const float inv_cols = 1.0f / (float)cols;
     unsigned flip = 0;
-    // one row; dead groups go along (shuffles and barriers are the whole warp's)
     auto work = [&](size_t row, bool live, const T *px, const T *pg, const T *pd, T *po) {
-        float h[NV][VE], gf[BWD ? NV : 1][VE];
-        float2 st = make_float2(0.0f, 0.0f), s = make_float2(0.0f, 0.0f);
-        if (BWD && live) st = __ldg(&a.stats[row]);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const unsigned c = (t + j * TPR) * VE;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                h[j][e] = 0.0f;
-                if (BWD) gf[BWD ? j : 0][e] = 0.0f;
-            }
-            if (live && c < cols) {
-                ln_vec<T, VE>::ld(px + c, h[j]);
-                if (BWD) ln_vec<T, VE>::ld(pg + c, gf[BWD ? j : 0]);
-            }
-        }
         if (BWD) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    float &gj = gf[BWD ? j : 0][e];
-                    h[j][e] = (h[j][e] - st.x) * st.y;
-                    dw[BWD ? j : 0][e] += gj * h[j][e];
-                    db[BWD ? j : 0][e] += gj;
-                    gj *= wf[j][e];
-                    s.x += gj;
-                    s.y += gj * h[j][e];
-                }
-            }
-            s = ln_group_sum<TPR>(s, sh, flip);
-            flip ^= 1U;
-            const float c1 = s.x * inv_cols, c2 = s.y * inv_cols;
-            if (live && po != nullptr) {
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const unsigned c = (t + j * TPR) * VE;
-                    if (c < cols) {
-                        float o[VE];
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) o[e] = __fmul_rn(st.y, gf[BWD ? j : 0][e] - c1 - h[j][e] * c2);   // (never fused with the addition below)
-                        if (BWD == 2) {
-                            // round, add, round: the entry without accumulation followed by gd_backend_accumulate
-                            float d[VE];
-                            ln_vec<T, VE>::ld(pd + c, d);
-#pragma unroll
-                            for (int e = 0; e < VE; ++e) o[e] = d[e] + gdb_io<T>::rnd(o[e]);
-                        }
-                        ln_vec<T, VE>::st(po + c, o);
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-#pragma unroll
-                for (int e = 0; e < VE; ++e) s.x += h[j][e];
-            }
-            const float mean = ln_group_sum<TPR>(s, sh, flip).x * inv_cols;
-            s = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                if ((t + j * TPR) * VE < cols) {
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        h[j][e] -= mean;
-                        s.x += h[j][e] * h[j][e];
-                    }
-                }
-            }
-            const float inv = rsqrtf(ln_group_sum<TPR>(s, sh, flip ^ 1U).x * inv_cols + a.eps);
-            if (live) {
-                if (a.stats != nullptr && t == 0) a.stats[row] = make_float2(mean, inv);
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const unsigned c = (t + j * TPR) * VE;
-                    if (c < cols) {
-                        float o[VE];
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) o[e] = fmaf(h[j][e] * inv, wf[j][e], bf[BWD ? 0 : j][e]);
-                        ln_vec<T, VE>::st(po + c, o);
-                    }
-                }
-            }
+            ln_backward_row<T, VE, TPR>(px, pg, pd, po, live, BWD == 2, live ? __ldg(&a.stats[row]) : make_float2(0.0f, 0.0f), wf, sums2, inv_cols, t, cols, sh, flip);
+            return;
         }
+        ln_pairs<T, VE, TPR> f;
+        f.load(px, t, cols, live);
+        f32x2 s2 = f2_make(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_add(s2, f.v[k]);
+        const float mean = ln_group_sum<TPR>(ln_halves(s2), sh, 0).x * inv_cols;
+        f.center(f2_make(-mean, -mean), t, cols);
+        s2 = f2_make(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_fma(f.v[k], f.v[k], s2);
+        const float inv = rsqrtf(ln_group_sum<TPR>(ln_halves(s2), sh, 1).x * inv_cols + a.eps);
+        if (!live) return;
+        if (a.stats != nullptr && t == 0) a.stats[row] = make_float2(mean, inv);
+        const f32x2 inv2 = f2_make(inv, inv);
+#pragma unroll
+        for (int k = 0; k < LN_EPT / 2; ++k) f.v[k] = f2_fma(f2_mul(f.v[k], inv2), wf.v[k], bf.v[k]);
+        f.store(po, t, cols);
     };
-    unsigned s = 0, ph = 0, done_ph = 0, turn = 0;   // done_ph: bit k, parity of stage k's next completion
+    unsigned s = 0, ph = 0;
     bool ok = true;
-    size_t sent_to = blockIdx.x;                     // (leader) the first tile whose results have not been sent off
-    auto pass_on = [&](unsigned before) {
-        if (ok && !mbar_wait(done0 + 8U * before, (done_ph >> before) & 1U)) {
-            ok = false;
-            atomicExch(err_flag, 602);
-        }
-        done_ph ^= 1U << before;
-        send(sent_to, before);
-        sent_to += gridDim.x;
-    };
-    for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
+    for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const size_t row0 = tile * a.tile_rows, left = a.rows - row0;
         const unsigned here = left < a.tile_rows ? (unsigned)left : a.tile_rows;
         if (bulk_bytes(tile) == 0U) {
@@ -365,12 +377,6 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
                 work(row0 + r, r < here, x + at, g + at, out + at, out == nullptr ? nullptr : out + at);
             }
             break;
-        }
-        if (leader) {
-            const unsigned before = s == 0U ? stages - 1U : s - 1U;
-            if (turn >= 1U) pass_on(before);
-            bulk_wait_group_read<1>();
-            fetch(tile + (size_t)(stages - 2U) * gridDim.x, (s + stages - 2U) % stages);
         }
         // (a wait that gives up is not waited for again, and the walk goes on: the groups' barriers stay complete)
         if (ok && !mbar_wait(full0 + 8U * s, ph)) {
@@ -384,36 +390,31 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
             const unsigned at = (r < here ? r : 0U) * cols;
             work(row0 + r, r < here, sx + at, sg + at, sd + at, out == nullptr ? nullptr : sx + at);
         }
+        // the warp that finishes the tile sends it off and fetches the next one for its stage
         fence_proxy_async_smem();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(done0 + 8U * s) : "memory");
+        if ((threadIdx.x & 31) == 0) {
+            __threadfence_block();
+            if (atomicAdd(&arrived[s], 1U) == LN_WARPS - 1U) {
+                arrived[s] = 0U;
+                __threadfence_block();
+                send(tile, s);
+                bulk_wait_group_read<0>();
+                fetch(tile + (size_t)stages * gridDim.x, s);
+            }
+        }
         if (++s == stages) {
             s = 0;
             ph ^= 1U;
         }
     }
-    if (leader) {
-        // (turn tiles went through the ring)
-        if (turn >= 1U) pass_on(s == 0U ? stages - 1U : s - 1U);
-        bulk_wait_all();
-    }
+    if ((threadIdx.x & 31) == 0) bulk_wait_all();
     if (BWD && a.partial != nullptr) {
         // the groups' sums through the ring (64 KB), added in order
         __syncthreads();
-        float *sums = reinterpret_cast<float *>(ring) + (size_t)group * 2U * cols;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const unsigned c = (t + j * TPR) * VE;
-            if (c < cols) {
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    sums[c + e] = dw[BWD ? j : 0][e];
-                    sums[cols + c + e] = db[BWD ? j : 0][e];
-                }
-            }
-        }
+        float *sums = reinterpret_cast<float *>(ring);
+        sums2.template store<VE, TPR>(sums + (size_t)group * 2U * cols, t, cols);
         __syncthreads();
-        sums = reinterpret_cast<float *>(ring);
         for (unsigned c = threadIdx.x; c < 2U * cols; c += LN_THREADS) {
             float v = 0.0f;
 #pragma unroll 8
@@ -432,21 +433,13 @@ layer_norm_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const fl
                       float *__restrict__ partial, size_t rows, unsigned cols)
 {
     gdb_pdl_sync();
-    constexpr int NV = LN_EPT / VE, GROUPS = LN_BWD_THREADS / TPR;
+    constexpr int GROUPS = LN_BWD_THREADS / TPR;
     extern __shared__ float sums[];   // [groups, 2, cols]
     __shared__ float2 sh[64];
     const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    float wf[NV][VE], dw[NV][VE], db[NV][VE];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const unsigned c = (t + j * TPR) * VE;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            wf[j][e] = w != nullptr ? 0.0f : 1.0f;
-            dw[j][e] = db[j][e] = 0.0f;
-        }
-        if (w != nullptr && c < cols) ln_vec<T, VE>::ld(w + c, wf[j]);
-    }
+    ln_pairs<T, VE, TPR> wf;
+    wf.load(w, t, cols, w != nullptr, 1.0f);
+    ln_sums sums2;
     const float inv_cols = 1.0f / (float)cols;
     const size_t stride = (size_t)gridDim.x * GROUPS;
     unsigned flip = 0;
@@ -455,68 +448,12 @@ layer_norm_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const fl
         const size_t row = TPR < 32 ? first + (group & (32U / (TPR < 32 ? TPR : 32) - 1U)) : first;
         const bool live = row < rows;
         const size_t at = (live ? row : 0) * cols;
-        float h[NV][VE], gf[NV][VE];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const unsigned c = (t + j * TPR) * VE;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) h[j][e] = gf[j][e] = 0.0f;
-            if (live && c < cols) {
-                ln_vec<T, VE>::ld(x + at + c, h[j]);
-                ln_vec<T, VE>::ld(g + at + c, gf[j]);
-            }
-        }
-        const float2 st = live ? stats[row] : make_float2(0.0f, 0.0f);
-        float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                h[j][e] = (h[j][e] - st.x) * st.y;
-                dw[j][e] += gf[j][e] * h[j][e];
-                db[j][e] += gf[j][e];
-                gf[j][e] *= wf[j][e];
-                s.x += gf[j][e];
-                s.y += gf[j][e] * h[j][e];
-            }
-        }
-        s = ln_group_sum<TPR>(s, sh, flip);
-        flip ^= 1U;
-        const float c1 = s.x * inv_cols, c2 = s.y * inv_cols;
-        if (live && dx != nullptr) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const unsigned c = (t + j * TPR) * VE;
-                if (c < cols) {
-                    float o[VE];
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) o[e] = __fmul_rn(st.y, gf[j][e] - c1 - h[j][e] * c2);   // (never fused with the addition below)
-                    if (add_to_dx) {
-                        // round, add, round: the entry without accumulation followed by gd_backend_accumulate
-                        float d[VE];
-                        ln_vec<T, VE>::ld(dx + at + c, d);
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) o[e] = d[e] + gdb_io<T>::rnd(o[e]);
-                    }
-                    ln_vec<T, VE>::st(dx + at + c, o);
-                }
-            }
-        }
+        ln_backward_row<T, VE, TPR>(x + at, g + at, dx + at, dx == nullptr ? nullptr : dx + at, live, add_to_dx, live ? stats[row] : make_float2(0.0f, 0.0f), wf, sums2, inv_cols, t,
+                                    cols, sh, flip);
     }
     if (partial == nullptr) return;
     // the groups' sums, added in order
-    float *mine = sums + (size_t)group * 2U * cols;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const unsigned c = (t + j * TPR) * VE;
-        if (c < cols) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                mine[c + e] = dw[j][e];
-                mine[cols + c + e] = db[j][e];
-            }
-        }
-    }
+    sums2.template store<VE, TPR>(sums + (size_t)group * 2U * cols, t, cols);
     __syncthreads();
     for (unsigned c = threadIdx.x; c < 2U * cols; c += LN_BWD_THREADS) {
         float v = 0.0f;
