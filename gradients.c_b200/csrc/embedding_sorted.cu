@@ -17,7 +17,7 @@
 
 namespace {
 
-constexpr int ES_SORT_WARPS = 32;
+constexpr int ES_SORT_WARPS = 32, ES_AHEAD = 8;   // (ids on their way, a lane)
 constexpr unsigned ES_MAX_WIDTH = 1536;      // tokens of a slice: 32 x 1536 counters fill 192 KB
 constexpr int ES_WARPS = 8;                  // of a reducing block
 
@@ -85,11 +85,15 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
     const unsigned per = ((n + ES_SORT_WARPS * 32U - 1U) / (ES_SORT_WARPS * 32U)) * 32U;
     const unsigned i0 = min(n, warp * per), i1 = min(n, i0 + per);
     unsigned below = 0U;
-#pragma unroll 4
-    for (unsigned i = i0 + lane; i < i1; i += 32U) {
-        const unsigned id = (unsigned)__ldg(&ids[i]);   // (a negative id lies above every vocabulary)
-        below += id < v0 ? 1U : 0U;
-        if (id - v0 < w) atomicAdd(&mine[id - v0], 1U);
+    for (unsigned i = i0 + lane; i < i1; i += 32U * ES_AHEAD) {
+        unsigned id[ES_AHEAD];
+#pragma unroll
+        for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u < i1 ? (unsigned)__ldg(&ids[i + 32U * u]) : 0xffffffffU;
+#pragma unroll
+        for (int u = 0; u < ES_AHEAD; ++u) {
+            below += id[u] < v0 ? 1U : 0U;   // (a negative id lies above every vocabulary)
+            if (id[u] - v0 < w) atomicAdd(&mine[id[u] - v0], 1U);
+        }
     }
     below = __reduce_add_sync(0xffffffffU, below);
     if (lane == 0) below_sum[warp] = below;
@@ -141,20 +145,26 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
     }
     if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) count[0] = base;
     // the same ranges again: every id of the slice to its place, equal ids of a warp's 32 in lane order
-    for (unsigned i = i0; i < i1; i += 32U) {
-        const unsigned id = i + lane < i1 ? (unsigned)__ldg(&ids[i + lane]) : 0xffffffffU;
-        const bool in = id - v0 < w;
-        if (__ballot_sync(0xffffffffU, in) == 0U) continue;
-        const unsigned peers = __match_any_sync(0xffffffffU, in ? id - v0 : w + lane);
-        const unsigned before = __popc(peers & ((1U << lane) - 1U));
-        unsigned at = 0U;
-        if (in) at = mine[id - v0] + before;
-        __syncwarp();
-        if (in && before == 0U) mine[id - v0] = at + __popc(peers);
-        __syncwarp();
-        if (in) {
-            order[at] = i + lane;
-            token[at] = (int)id;
+    for (unsigned i = i0; i < i1; i += 32U * ES_AHEAD) {
+        unsigned id[ES_AHEAD];
+#pragma unroll
+        for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u + lane < i1 ? (unsigned)__ldg(&ids[i + 32U * u + lane]) : 0xffffffffU;
+#pragma unroll
+        for (int u = 0; u < ES_AHEAD; ++u) {
+            const unsigned k = id[u] - v0;
+            const bool in = k < w;
+            if (__ballot_sync(0xffffffffU, in) == 0U) continue;
+            const unsigned peers = __match_any_sync(0xffffffffU, in ? k : w + lane);
+            const unsigned before = __popc(peers & ((1U << lane) - 1U));
+            unsigned at = 0U;
+            if (in) at = mine[k] + before;
+            __syncwarp();
+            if (in && before == 0U) mine[k] = at + __popc(peers);
+            __syncwarp();
+            if (in) {
+                order[at] = i + 32U * u + lane;
+                token[at] = (int)id[u];
+            }
         }
     }
 }
@@ -186,6 +196,10 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
     typedef es_vec<T, VE> vec;
     constexpr int COLS = 32 * VE * NV, U = NV == 1 ? 8 : 2;
     __shared__ float head[ES_WARPS][COLS], tail[ES_WARPS][COLS];
+    // of each warp's entries: the first token, and whether its run began before them (1), goes on behind them (2), does both with one token (4);
+    // 8: there are none
+    __shared__ int first_token[ES_WARPS];
+    __shared__ unsigned ends[ES_WARPS];
     const unsigned total = count[0];
     const unsigned e0 = blockIdx.x * piece;
     if (e0 >= total) return;
@@ -210,9 +224,13 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
         }
     };
     // runs that are not complete within the warp's entries
-    const int before = a > 0U && a < b ? token[a - 1] : -1, after = b < total && a < b ? token[b] : -1;
-    bool open_left = a < b && before == token[a];
-    int current = a < b ? token[a] : -1;
+    const int before = a > 0U && a < b ? token[a - 1] : -1, after = b < total && a < b ? token[b] : -1, begin = a < b ? token[a] : -1, end = a < b ? token[b - 1] : -1;
+    bool open_left = a < b && before == begin;
+    int current = begin;
+    if (lane == 0) {
+        first_token[warp] = begin;
+        ends[warp] = a < b ? (before == begin ? 1U : 0U) | (after == end ? 2U : 0U) | (before == begin && after == begin ? 4U : 0U) : 8U;
+    }
     for (unsigned i = a; i < b; i += 32U) {
         const unsigned mine = i + lane < b ? order[i + lane] : 0U;
         const int mine_token = i + lane < b ? token[i + lane] : -1;
@@ -278,68 +296,71 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
     for (int c = threadIdx.x; c < COLS; c += ES_WARPS * 32) {
         if (col0 + c >= dim) break;
         float sum = 0.0f;
-        bool from_before = true;   // the run being added began in an earlier piece
+        bool from_before = true, open = false;   // the run being added began in an earlier piece; goes on behind the last warp
+#pragma unroll
         for (int k = 0; k < ES_WARPS; ++k) {
-            const unsigned ka = min(e1, e0 + k * per), kb = min(e1, ka + per);
-            if (ka >= kb) break;
-            const bool left = ka > 0U && token[ka - 1] == token[ka], right = kb < total && token[kb - 1] == token[kb];
-            const bool through = left && right && token[ka] == token[kb];
-            if (left) {
+            const unsigned f = ends[k];
+            if (f & 8U) continue;
+            open = (f & 2U) != 0U;
+            if (f & 1U) {
                 sum += head[k][c];
-                if (!through) {
+                if (!(f & 4U)) {
                     if (from_before) {
                         partial[(size_t)blockIdx.x * 2U * dim + col0 + c] = sum;
                     } else {
-                        es_store<T, 1>(table + (size_t)token[ka] * dim + col0 + c, &sum, scale, add);
+                        es_store<T, 1>(table + (size_t)first_token[k] * dim + col0 + c, &sum, scale, add);
                     }
                     sum = 0.0f;
-                    from_before = false;
                 }
-            } else {
-                from_before = false;
             }
-            if (right && !through) {
-                sum = tail[k][c];
+            if (!(f & 4U)) {
                 from_before = false;
+                if (f & 2U) sum = tail[k][c];
             }
-            if (kb == e1 && right) partial[((size_t)blockIdx.x * 2U + (from_before ? 0U : 1U)) * dim + col0 + c] = sum;
         }
+        if (open) partial[((size_t)blockIdx.x * 2U + (from_before ? 0U : 1U)) * dim + col0 + c] = sum;
     }
 }
 
-// Block (c, s): the run that begins in piece c and goes on in the next ones, if there is one; a warp adds every eighth of its parts.
+// Block (c, s): the run that begins in piece c and goes on in the next ones, if there is one; a warp adds every eighth of its parts, 128
+// columns at a time.
 template <typename T>
 __global__ void __launch_bounds__(256)
 es_merge_kernel(const float *__restrict__ partial, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table, unsigned piece, size_t dim,
                 float scale, bool add)
 {
     gdb_pdl_sync();
-    __shared__ float sh[8][33];
+    __shared__ float sh[8][128];
     const unsigned total = count[0], c = blockIdx.x, e0 = c * piece, e1 = e0 + piece;
     if (e1 >= total) return;
     const int k = token[e1];
     if (token[e1 - 1] != k || (e0 > 0U && token[e0 - 1] == k)) return;   // complete, or begun earlier
     // last piece whose first entry has this token
     unsigned lo = c + 1U, hi = (total - 1U) / piece;
+    if (lo < hi && token[(size_t)(lo + 1U) * piece] != k) hi = lo;       // (most runs end in the next piece)
     while (lo < hi) {
         const unsigned mid = (lo + hi + 1U) / 2U;
         if (token[(size_t)mid * piece] == k) lo = mid; else hi = mid - 1U;
     }
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-    for (size_t col0 = (size_t)blockIdx.y * 32U; col0 < dim; col0 += (size_t)gridDim.y * 32U) {
-        const size_t col = col0 + lane;
-        float s = 0.0f;
-        if (col < dim) {
-#pragma unroll 4
-            for (unsigned j = c + (unsigned)part; j <= lo; j += 8U) s += __ldcg(&partial[((size_t)j * 2U + (j == c ? 1U : 0U)) * dim + col]);
-        }
-        sh[part][lane] = s;
-        __syncthreads();
-        if (part == 0 && col < dim) {
-            float v = 0.0f;
+    const unsigned parts = min(8U, lo - c + 1U);
+    for (size_t col0 = (size_t)blockIdx.y * 128U; col0 < dim; col0 += (size_t)gridDim.y * 128U) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+        for (unsigned j = c + (unsigned)part; j <= lo; j += 8U) {
+            const float *row = partial + ((size_t)j * 2U + (j == c ? 1U : 0U)) * dim + col0;
 #pragma unroll
-            for (int p = 0; p < 8; ++p) v += sh[p][lane];
-            es_store<T, 1>(table + (size_t)k * dim + col, &v, scale, add);
+            for (int e = 0; e < 4; ++e) {
+                if (col0 + lane + 32 * e < dim) s[e] += __ldcg(&row[lane + 32 * e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sh[part][lane + 32 * e] = s[e];
+        __syncthreads();
+        if (threadIdx.x < 128U && col0 + threadIdx.x < dim) {
+            float v = 0.0f;
+            for (unsigned p = 0; p < parts; ++p) v += sh[p][threadIdx.x];
+            es_store<T, 1>(table + (size_t)k * dim + col0 + threadIdx.x, &v, scale, add);
         }
         __syncthreads();
     }
@@ -366,8 +387,8 @@ gd_status reduce(gd_backend *be, const void *g, const unsigned *order, const int
     gdb_launch(es_reduce_kernel<T, VE, NV>, dim3(pieces, (unsigned)slabs), ES_WARPS * 32, 0, be->stream, (const T *)g, order, token, count, (T *)table, partial, piece, dim, scale, add);
     gd_status st = gdb_launched(be, "embedding_sorted_backward sums");
     if (st != GD_OK || pieces == 1U) return st;
-    const size_t col_blocks = (dim + 31U) / 32U;
-    gdb_launch(es_merge_kernel<T>, dim3(pieces - 1U, (unsigned)(col_blocks < 64U ? col_blocks : 64U)), 256, 0, be->stream, (const float *)partial, token, count, (T *)table, piece, dim,
+    const size_t col_blocks = (dim + 127U) / 128U;
+    gdb_launch(es_merge_kernel<T>, dim3(pieces - 1U, (unsigned)(col_blocks < 4U ? col_blocks : 4U)), 256, 0, be->stream, (const float *)partial, token, count, (T *)table, piece, dim,
                scale, add);
     return gdb_launched(be, "embedding_sorted_backward merge");
 }

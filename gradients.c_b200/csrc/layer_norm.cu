@@ -15,10 +15,9 @@ using namespace gdb_t5;
 constexpr int LN_EPT = 16;                       // elements of a row that a thread holds
 constexpr size_t LN_MAX_COLS = 512 * LN_EPT;     // rows that a group of one block's threads holds
 
-// VE consecutive elements, moved with one access (VE > 1: 16 bytes)
+// VE consecutive elements, stored with one access (VE > 1: 16 bytes)
 template <typename T, int VE> struct ln_vec;
 template <typename T> struct ln_vec<T, 1> {
-    static __device__ __forceinline__ void ld(const T *p, float (&f)[1]) { f[0] = gdb_io<T>::ld(p, 0); }
     static __device__ __forceinline__ void st(T *p, const float (&f)[1]) { gdb_io<T>::st(p, 0, f[0]); }
 };
 // (two 16-bit elements a conversion)
@@ -26,105 +25,141 @@ template <typename T> __device__ __forceinline__ float2 ln_two(uint32_t w);
 template <> __device__ __forceinline__ float2 ln_two<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 template <> __device__ __forceinline__ float2 ln_two<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000U)); }
 template <typename T> struct ln_vec<T, 8> {
-    static __device__ __forceinline__ void ld(const T *p, float (&f)[8])
-    {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const float2 a = ln_two<T>(v.x), b = ln_two<T>(v.y), c = ln_two<T>(v.z), d = ln_two<T>(v.w);
-        f[0] = a.x;
-        f[1] = a.y;
-        f[2] = b.x;
-        f[3] = b.y;
-        f[4] = c.x;
-        f[5] = c.y;
-        f[6] = d.x;
-        f[7] = d.y;
-    }
     static __device__ __forceinline__ void st(T *p, const float (&f)[8])
     {
         *reinterpret_cast<uint4 *>(p) = make_uint4(half_pack<T>::pack(f[0], f[1]), half_pack<T>::pack(f[2], f[3]), half_pack<T>::pack(f[4], f[5]), half_pack<T>::pack(f[6], f[7]));
     }
 };
 template <> struct ln_vec<float, 4> {
-    static __device__ __forceinline__ void ld(const float *p, float (&f)[4])
-    {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        f[0] = v.x;
-        f[1] = v.y;
-        f[2] = v.z;
-        f[3] = v.w;
-    }
     static __device__ __forceinline__ void st(float *p, const float (&f)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]); }
 };
 
-// Sums over a group of TPR threads of a block. Groups of more than a warp meet at a named barrier of their own; `sh` holds two sets of
-// one value pair per warp of the block, used in turn (`flip`), so that one barrier a call is enough.
-template <int TPR>
-__device__ __forceinline__ float2 ln_group_sum(float2 v, float2 *sh, unsigned flip)
+// Sums of K value pairs over a group of TPR threads of a block. Groups of more than a warp meet at a named barrier of their own; `sh` holds
+// two sets of K pairs per warp of the block (at most 16), used in turn (`flip`), so that one barrier a call is enough.
+template <int TPR, int K>
+__device__ __forceinline__ void ln_group_sums(float2 (&v)[K], float2 *sh, unsigned flip)
 {
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffU, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffU, v.y, o);
+#pragma unroll
+        for (int r = 0; r < K; ++r) {
+            v[r].x += __shfl_xor_sync(0xffffffffU, v[r].x, o);
+            v[r].y += __shfl_xor_sync(0xffffffffU, v[r].y, o);
+        }
     }
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;
         const int warp = threadIdx.x >> 5, group = threadIdx.x / TPR;
-        float2 *s = sh + flip * 32U;
-        if ((threadIdx.x & 31) == 0) s[warp] = v;
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(TPR) : "memory");
-        v = make_float2(0.0f, 0.0f);
+        float2 *s = sh + flip * (16U * K);
+        if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            v.x += s[group * W + w].x;
-            v.y += s[group * W + w].y;
+            for (int r = 0; r < K; ++r) s[warp * K + r] = v[r];
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(TPR) : "memory");
+#pragma unroll
+        for (int r = 0; r < K; ++r) {
+            v[r] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                v[r].x += s[(group * W + w) * K + r].x;
+                v[r].y += s[(group * W + w) * K + r].y;
+            }
         }
     }
-    return v;
+}
+template <int TPR>
+__device__ __forceinline__ float2 ln_group_sum(float2 v, float2 *sh, unsigned flip)
+{
+    float2 one[1] = {v};
+    ln_group_sums<TPR, 1>(one, sh, flip);
+    return one[0];
 }
 
-// A thread's 16 elements of a row in pairs (sm_100 multiplies and adds two FP32 numbers an instruction): NV accesses of VE elements, TPR
+// A thread's EPT elements of a row in pairs (sm_100 multiplies and adds two FP32 numbers an instruction): accesses of VE elements, TPR
 // accesses apart.
-template <typename T, int VE, int TPR> struct ln_pairs {
-    f32x2 v[LN_EPT / 2];
-    __device__ __forceinline__ void load(const T *p, unsigned t, unsigned cols, bool live, float other = 0.0f)
-    {
-        float f[LN_EPT];
+template <typename T, int VE, int TPR, int EPT = LN_EPT> struct ln_pairs {
+    f32x2 v[EPT / 2];
+    // Rows fill more than half of a group's places (LN_BY_WIDTH), so the first half needs no test.
+    static __host__ __device__ constexpr bool inside(int j) { return TPR > 8 && 2 * (j + 1) * VE <= EPT; }
+    // a row's elements as they lie in memory, to be taken apart later
+    struct raw {
+        uint4 v[VE > 1 ? EPT / VE : 1];
+        float f[VE > 1 ? 1 : EPT];
+        __device__ __forceinline__ void load(const T *p, unsigned t, unsigned cols)
+        {
 #pragma unroll
-        for (int j = 0; j < LN_EPT / VE; ++j) {
-            const unsigned c = (t + j * TPR) * VE;
-            float(&fj)[VE] = *reinterpret_cast<float(*)[VE]>(f + j * VE);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) fj[e] = other;
-            if (live && c < cols) ln_vec<T, VE>::ld(p + c, fj);
+            for (int j = 0; j < EPT / VE; ++j) {
+                const unsigned c = (t + j * TPR) * VE;
+                if (VE > 1) {
+                    v[VE > 1 ? j : 0] = make_uint4(0U, 0U, 0U, 0U);
+                    if (inside(j) || c < cols) v[VE > 1 ? j : 0] = *reinterpret_cast<const uint4 *>(p + c);
+                } else {
+                    f[VE > 1 ? 0 : j] = 0.0f;
+                    if (inside(j) || c < cols) f[VE > 1 ? 0 : j] = gdb_io<T>::ld(p, c);
+                }
+            }
         }
+    };
+    __device__ __forceinline__ void take(const raw &r)
+    {
+        if constexpr (VE > 1) {
 #pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) v[k] = f2_make(f[2 * k], f[2 * k + 1]);
+            for (int j = 0; j < EPT / VE; ++j) {
+                const uint32_t w[4] = {r.v[j].x, r.v[j].y, r.v[j].z, r.v[j].w};
+#pragma unroll
+                for (int k = 0; k < VE / 2; ++k) {
+                    if constexpr (sizeof(T) == 2) {
+                        const float2 a = ln_two<T>(w[k]);
+                        v[j * (VE / 2) + k] = f2_make(a.x, a.y);
+                    } else {
+                        v[j * (VE / 2) + k] = f2_make(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < EPT / 2; ++k) v[k] = f2_make(r.f[2 * k], r.f[2 * k + 1]);
+        }
+    }
+    __device__ __forceinline__ void fill(float x)
+    {
+#pragma unroll
+        for (int k = 0; k < EPT / 2; ++k) v[k] = f2_make(x, x);
+    }
+    __device__ __forceinline__ void load(const T *p, unsigned t, unsigned cols)
+    {
+        raw r;
+        r.load(p, t, cols);
+        take(r);
     }
     // adds to the elements inside the row
     __device__ __forceinline__ void center(f32x2 by, unsigned t, unsigned cols)
     {
 #pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) {
+        for (int k = 0; k < EPT / 2; ++k) {
             const f32x2 d = f2_add(v[k], by);
+            const int j = 2 * k / VE;
             if (VE > 1) {
-                if ((t + (2 * k / VE) * TPR) * VE < cols) v[k] = d;
+                if (inside(j) || (t + j * TPR) * VE < cols) v[k] = d;
+            } else if (inside(j + 1)) {
+                v[k] = d;
             } else {
                 float lo, hi, l0, h0;
                 f2_split(d, lo, hi);
                 f2_split(v[k], l0, h0);
-                v[k] = f2_make(t + 2 * k * TPR < cols ? lo : l0, t + (2 * k + 1) * TPR < cols ? hi : h0);
+                v[k] = f2_make(t + j * TPR < cols ? lo : l0, t + (j + 1) * TPR < cols ? hi : h0);
             }
         }
     }
     __device__ __forceinline__ void store(T *p, unsigned t, unsigned cols) const
     {
-        float f[LN_EPT];
+        float f[EPT];
 #pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) f2_split(v[k], f[2 * k], f[2 * k + 1]);
+        for (int k = 0; k < EPT / 2; ++k) f2_split(v[k], f[2 * k], f[2 * k + 1]);
 #pragma unroll
-        for (int j = 0; j < LN_EPT / VE; ++j) {
+        for (int j = 0; j < EPT / VE; ++j) {
             const unsigned c = (t + j * TPR) * VE;
-            if (c < cols) ln_vec<T, VE>::st(p + c, *reinterpret_cast<const float(*)[VE]>(f + j * VE));
+            if (inside(j) || c < cols) ln_vec<T, VE>::st(p + c, *reinterpret_cast<const float(*)[VE]>(f + j * VE));
         }
     }
 };
@@ -135,41 +170,53 @@ __device__ __forceinline__ float2 ln_halves(f32x2 s)
     return make_float2(lo + hi, 0.0f);
 }
 
-// One row per group, threads / TPR rows per block. stats (may be NULL): mean and 1 / deviation of every row.
+// A group walks over rows with the next one on its way; weight and bias stay in registers. stats (may be NULL): mean and 1 / deviation of
+// every row.
+template <typename T, int TPR, int VE, int EPT>
+__device__ __forceinline__ void ln_forward_row(ln_pairs<T, VE, TPR, EPT> &f, const ln_pairs<T, VE, TPR, EPT> &wf, const ln_pairs<T, VE, TPR, EPT> &bf, T *po, float2 *stats, bool live,
+                                               unsigned t, unsigned cols, float inv_cols, float eps, float2 *sh)
+{
+    f32x2 s2 = f2_make(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < EPT / 2; ++k) s2 = f2_add(s2, f.v[k]);
+    const float mean = ln_group_sum<TPR>(ln_halves(s2), sh, 0).x * inv_cols;
+    f.center(f2_make(-mean, -mean), t, cols);
+    s2 = f2_make(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < EPT / 2; ++k) s2 = f2_fma(f.v[k], f.v[k], s2);
+    const float inv = rsqrtf(ln_group_sum<TPR>(ln_halves(s2), sh, 1).x * inv_cols + eps);
+    if (!live) return;
+    if (stats != nullptr && t == 0) *stats = make_float2(mean, inv);
+    const f32x2 inv2 = f2_make(inv, inv);
+#pragma unroll
+    for (int k = 0; k < EPT / 2; ++k) f.v[k] = f2_fma(f2_mul(f.v[k], inv2), wf.v[k], bf.v[k]);
+    f.store(po, t, cols);
+}
 template <typename T, int TPR, int VE>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 layer_norm_fwd_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, T *out, float2 *__restrict__ stats, size_t rows, unsigned cols, float eps)
 {
     gdb_pdl_sync();
     constexpr int THREADS = TPR > 256 ? TPR : 256;
+    constexpr unsigned TOGETHER = TPR < 32 ? 32 / TPR : 1;   // groups of a warp: they take the same number of turns
     __shared__ float2 sh[64];
-    const unsigned t = threadIdx.x % TPR;
-    const size_t row = (size_t)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
-    const bool live = row < rows;   // (groups within a warp stay together through the shuffles)
-    const T *xr = x + (live ? row : 0) * cols;
-    ln_pairs<T, VE, TPR> f;
-    f.load(xr, t, cols, live);
-    f32x2 s2 = f2_make(0.0f, 0.0f);
-#pragma unroll
-    for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_add(s2, f.v[k]);
-    float2 s = ln_halves(s2);
+    const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR, mine = group % TOGETHER;
+    const size_t stride = (size_t)gridDim.x * (THREADS / TPR);
+    typedef ln_pairs<T, VE, TPR> pairs;
+    size_t first = (size_t)blockIdx.x * (THREADS / TPR) + group - mine;
+    typename pairs::raw next;
+    next.load(x + (first + mine < rows ? first + mine : 0) * cols, t, cols);
+    pairs wf, bf;
+    if (w != nullptr) wf.load(w, t, cols); else wf.fill(1.0f);
+    if (b != nullptr) bf.load(b, t, cols); else bf.fill(0.0f);
     const float inv_cols = 1.0f / (float)cols;
-    const float mean = ln_group_sum<TPR>(s, sh, 0).x * inv_cols;
-    f.center(f2_make(-mean, -mean), t, cols);
-    s2 = f2_make(0.0f, 0.0f);
-#pragma unroll
-    for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_fma(f.v[k], f.v[k], s2);
-    s = ln_halves(s2);
-    const float inv = rsqrtf(ln_group_sum<TPR>(s, sh, 1).x * inv_cols + eps);
-    if (!live) return;
-    if (stats != nullptr && t == 0) stats[row] = make_float2(mean, inv);
-    ln_pairs<T, VE, TPR> wf, bf;
-    wf.load(w, t, cols, w != nullptr, 1.0f);
-    bf.load(b, t, cols, b != nullptr);
-    const f32x2 inv2 = f2_make(inv, inv);
-#pragma unroll
-    for (int k = 0; k < LN_EPT / 2; ++k) f.v[k] = f2_fma(f2_mul(f.v[k], inv2), wf.v[k], bf.v[k]);
-    f.store(out + row * cols, t, cols);
+    for (; first < rows; first += stride) {
+        const size_t row = first + mine;
+        pairs f;
+        f.take(next);
+        if (first + stride < rows) next.load(x + (row + stride < rows ? row + stride : 0) * cols, t, cols);
+        ln_forward_row(f, wf, bf, out + row * cols, stats == nullptr ? nullptr : stats + row, row < rows, t, cols, inv_cols, eps, sh);
+    }
 }
 
 // Rows of more than LN_MAX_COLS elements: a block per row that reads x three times (the second and third time from L2).
@@ -199,66 +246,93 @@ layer_norm_fwd_long_kernel(const T *x, const T *__restrict__ w, const T *__restr
 }
 
 // a thread's sums of g h and of g over the rows, for its columns
-struct ln_sums {
-    f32x2 dw[LN_EPT / 2], db[LN_EPT / 2];
+template <int EPT> struct ln_sums {
+    f32x2 dw[EPT / 2], db[EPT / 2];
     __device__ __forceinline__ ln_sums()
     {
 #pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) dw[k] = db[k] = f2_make(0.0f, 0.0f);
+        for (int k = 0; k < EPT / 2; ++k) dw[k] = db[k] = f2_make(0.0f, 0.0f);
     }
-    // to[0, c] and to[1, c]
+    // to[0, c] and to[1, c] (float4 accesses where VE allows them: to is 16-byte aligned then, and cols a multiple of 4)
     template <int VE, int TPR> __device__ __forceinline__ void store(float *to, unsigned t, unsigned cols) const
     {
+        constexpr int A = VE > 1 ? 4 : 1;
 #pragma unroll
-        for (int q = 0; q < LN_EPT; ++q) {
+        for (int q = 0; q < EPT; q += A) {
             const unsigned c = (t + (q / VE) * TPR) * VE + q % VE;
-            float a, b, u, v;
-            f2_split(dw[q / 2], a, b);
-            f2_split(db[q / 2], u, v);
-            if (c < cols) {
-                to[c] = q % 2 == 0 ? a : b;
-                to[cols + c] = q % 2 == 0 ? u : v;
+            if (c >= cols) continue;
+            float a[2], b[2], u[2], v[2];
+            f2_split(dw[q / 2], a[0], a[1]);
+            f2_split(db[q / 2], u[0], u[1]);
+            if (A == 4) {
+                f2_split(dw[(q / 2 + 1) % (EPT / 2)], b[0], b[1]);
+                f2_split(db[(q / 2 + 1) % (EPT / 2)], v[0], v[1]);
+                *reinterpret_cast<float4 *>(to + c) = make_float4(a[0], a[1], b[0], b[1]);
+                *reinterpret_cast<float4 *>(to + cols + c) = make_float4(u[0], u[1], v[0], v[1]);
+            } else {
+                to[c] = a[q % 2];
+                to[cols + c] = u[q % 2];
             }
         }
     }
 };
-// One row backward; dead groups go along (shuffles and barriers are the whole warp's). po may be px (or pg); pd: the old gradient.
-template <typename T, int VE, int TPR>
-__device__ __forceinline__ void ln_backward_row(const T *px, const T *pg, const T *pd, T *po, bool live, bool add, float2 st, const ln_pairs<T, VE, TPR> &wf, ln_sums &sums,
-                                                float inv_cols, unsigned t, unsigned cols, float2 *sh, unsigned &flip)
+// K rows backward, their sums exchanged together; dead rows go along (shuffles and barriers are the whole warp's). The elements are read
+// again behind the exchange, so that K rows are on their way without 32 registers each: one row at a time left 16 warps waiting for
+// shuffles (18432 x 512 FP16 17.8 us, of which the memory's 11). px, pg, pd (the old gradient), po (may be px or pg): first row, the others
+// `step` elements on.
+template <typename T, int VE, int TPR, int EPT, int K>
+__device__ __forceinline__ void ln_backward_rows(const T *px, const T *pg, const T *pd, T *po, size_t step, const bool (&live)[K], bool add, const float2 (&st)[K],
+                                                 const ln_pairs<T, VE, TPR, EPT> &wf, ln_sums<EPT> &sums, float inv_cols, unsigned t, unsigned cols, float2 *sh, unsigned &flip)
 {
-    ln_pairs<T, VE, TPR> h, g;
-    h.load(px, t, cols, live);
-    g.load(pg, t, cols, live);
-    const f32x2 mean2 = f2_make(-st.x, -st.x), inv2 = f2_make(st.y, st.y);
-    f32x2 s1 = f2_make(0.0f, 0.0f), s2 = s1;
+    float2 s[K];
 #pragma unroll
-    for (int k = 0; k < LN_EPT / 2; ++k) {
-        // (outside the row g is zero, and h whatever the mean makes of zero)
-        h.v[k] = f2_mul(f2_add(h.v[k], mean2), inv2);
-        sums.dw[k] = f2_fma(g.v[k], h.v[k], sums.dw[k]);
-        sums.db[k] = f2_add(sums.db[k], g.v[k]);
-        g.v[k] = f2_mul(g.v[k], wf.v[k]);
-        s1 = f2_add(s1, g.v[k]);
-        s2 = f2_fma(g.v[k], h.v[k], s2);
-    }
-    const float2 s = ln_group_sum<TPR>(make_float2(ln_halves(s1).x, ln_halves(s2).x), sh, flip);
-    flip ^= 1U;
-    if (!live || po == nullptr) return;
-    const f32x2 c1 = f2_make(-s.x * inv_cols, -s.x * inv_cols), c2 = f2_make(-s.y * inv_cols, -s.y * inv_cols);
+    for (int r = 0; r < K; ++r) {
+        s[r] = make_float2(0.0f, 0.0f);
+        if (!live[r]) continue;
+        ln_pairs<T, VE, TPR, EPT> h, g;
+        h.load(px + r * step, t, cols);
+        g.load(pg + r * step, t, cols);
+        const f32x2 mean2 = f2_make(-st[r].x, -st[r].x), inv2 = f2_make(st[r].y, st[r].y);
+        f32x2 s1 = f2_make(0.0f, 0.0f), s2 = s1;
 #pragma unroll
-    for (int k = 0; k < LN_EPT / 2; ++k) g.v[k] = f2_mul(inv2, f2_fma(h.v[k], c2, f2_add(g.v[k], c1)));
-    if (add) {
-        // round, add, round: the entry without accumulation followed by gd_backend_accumulate
-        h.load(pd, t, cols, true);
-#pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) {
-            float a, b;
-            f2_split(g.v[k], a, b);
-            g.v[k] = f2_add(h.v[k], f2_make(gdb_io<T>::rnd(a), gdb_io<T>::rnd(b)));
+        for (int k = 0; k < EPT / 2; ++k) {
+            // (outside the row g is zero, and h whatever the mean makes of zero)
+            const f32x2 hk = f2_mul(f2_add(h.v[k], mean2), inv2), gw = f2_mul(g.v[k], wf.v[k]);
+            sums.dw[k] = f2_fma(g.v[k], hk, sums.dw[k]);
+            sums.db[k] = f2_add(sums.db[k], g.v[k]);
+            s1 = f2_add(s1, gw);
+            s2 = f2_fma(gw, hk, s2);
         }
+        s[r] = make_float2(ln_halves(s1).x, ln_halves(s2).x);
     }
-    g.store(po, t, cols);
+    ln_group_sums<TPR, K>(s, sh, flip);
+    flip ^= 1U;
+    if (po == nullptr) return;
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+        if (!live[r]) continue;
+        ln_pairs<T, VE, TPR, EPT> h, g;
+        h.load(px + r * step, t, cols);
+        g.load(pg + r * step, t, cols);
+        const f32x2 mean2 = f2_make(-st[r].x, -st[r].x), inv2 = f2_make(st[r].y, st[r].y);
+        const f32x2 c1 = f2_make(-s[r].x * inv_cols, -s[r].x * inv_cols), c2 = f2_make(-s[r].y * inv_cols, -s[r].y * inv_cols);
+#pragma unroll
+        for (int k = 0; k < EPT / 2; ++k) {
+            const f32x2 hk = f2_mul(f2_add(h.v[k], mean2), inv2);
+            g.v[k] = f2_mul(inv2, f2_fma(hk, c2, f2_fma(g.v[k], wf.v[k], c1)));
+        }
+        if (add) {
+            // round, add, round: the entry without accumulation followed by gd_backend_accumulate
+            h.load(pd + r * step, t, cols);
+#pragma unroll
+            for (int k = 0; k < EPT / 2; ++k) {
+                float a, b;
+                f2_split(g.v[k], a, b);
+                g.v[k] = f2_add(h.v[k], f2_make(gdb_io<T>::rnd(a), gdb_io<T>::rnd(b)));
+            }
+        }
+        g.store(po + r * step, t, cols);
+    }
 }
 
 // ---- rows streamed through shared memory: as many bytes on their way as HBM wants, whatever the registers hold ----
@@ -281,7 +355,7 @@ struct ln_stream {
 };
 
 // BWD: 0 forward, 1 backward, 2 backward into a gradient that is there. Streams: x, and g, and the old dx.
-template <typename T, int TPR, int VE, int BWD>
+template <typename T, int TPR, int VE, int EPT, int BWD>
 __global__ void __launch_bounds__(LN_THREADS, 1)
 layer_norm_stream_kernel(const ln_stream a, int *err_flag)
 {
@@ -337,34 +411,31 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         for (unsigned k = 0; k < stages; ++k) fetch(blockIdx.x + (size_t)k * gridDim.x, k);
     }
     const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    ln_pairs<T, VE, TPR> wf, bf;
-    wf.load(w, t, cols, w != nullptr, 1.0f);
-    if (!BWD) bf.load(b, t, cols, b != nullptr);
-    ln_sums sums2;
+    ln_pairs<T, VE, TPR, EPT> wf, bf;
+    if (w != nullptr) wf.load(w, t, cols); else wf.fill(1.0f);
+    if (!BWD && b != nullptr) bf.load(b, t, cols); else bf.fill(0.0f);
+    ln_sums<EPT> sums2;
     const float inv_cols = 1.0f / (float)cols;
     unsigned flip = 0;
-    auto work = [&](size_t row, bool live, const T *px, const T *pg, const T *pd, T *po) {
+    // rows of a tile (or, behind the last full one, of memory), two at a time backward: first row, rows there are
+    auto work = [&](size_t row0, unsigned here, const T *px, const T *pg, const T *pd, T *po) {
         if (BWD) {
-            ln_backward_row<T, VE, TPR>(px, pg, pd, po, live, BWD == 2, live ? __ldg(&a.stats[row]) : make_float2(0.0f, 0.0f), wf, sums2, inv_cols, t, cols, sh, flip);
-            return;
+            for (unsigned r = group; r < a.tile_rows; r += 2U * GROUPS) {
+                const bool live[2] = {r < here, r + GROUPS < here};
+                float2 st[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                if (live[0]) st[0] = __ldg(&a.stats[row0 + r]);
+                if (live[1]) st[1] = __ldg(&a.stats[row0 + r + GROUPS]);
+                const size_t at = (size_t)r * cols;
+                ln_backward_rows<T, VE, TPR, EPT, 2>(px + at, pg + at, pd + at, po == nullptr ? nullptr : po + at, (size_t)GROUPS * cols, live, BWD == 2, st, wf, sums2, inv_cols, t,
+                                                     cols, sh, flip);
+            }
+        } else {
+            for (unsigned r = group; r < a.tile_rows; r += GROUPS) {
+                ln_pairs<T, VE, TPR, EPT> f;
+                if (r < here) f.load(px + (size_t)r * cols, t, cols); else f.fill(0.0f);
+                ln_forward_row(f, wf, bf, po + (size_t)r * cols, a.stats == nullptr ? nullptr : a.stats + row0 + r, r < here, t, cols, inv_cols, a.eps, sh);
+            }
         }
-        ln_pairs<T, VE, TPR> f;
-        f.load(px, t, cols, live);
-        f32x2 s2 = f2_make(0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_add(s2, f.v[k]);
-        const float mean = ln_group_sum<TPR>(ln_halves(s2), sh, 0).x * inv_cols;
-        f.center(f2_make(-mean, -mean), t, cols);
-        s2 = f2_make(0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) s2 = f2_fma(f.v[k], f.v[k], s2);
-        const float inv = rsqrtf(ln_group_sum<TPR>(ln_halves(s2), sh, 1).x * inv_cols + a.eps);
-        if (!live) return;
-        if (a.stats != nullptr && t == 0) a.stats[row] = make_float2(mean, inv);
-        const f32x2 inv2 = f2_make(inv, inv);
-#pragma unroll
-        for (int k = 0; k < LN_EPT / 2; ++k) f.v[k] = f2_fma(f2_mul(f.v[k], inv2), wf.v[k], bf.v[k]);
-        f.store(po, t, cols);
     };
     unsigned s = 0, ph = 0;
     bool ok = true;
@@ -372,10 +443,8 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         const size_t row0 = tile * a.tile_rows, left = a.rows - row0;
         const unsigned here = left < a.tile_rows ? (unsigned)left : a.tile_rows;
         if (bulk_bytes(tile) == 0U) {
-            for (unsigned r = group; r < a.tile_rows; r += GROUPS) {
-                const size_t at = (row0 + (r < here ? r : 0U)) * cols;
-                work(row0 + r, r < here, x + at, g + at, out + at, out == nullptr ? nullptr : out + at);
-            }
+            const size_t at = row0 * cols;
+            work(row0, here, x + at, g + at, out + at, out == nullptr ? nullptr : out + at);
             break;
         }
         // (a wait that gives up is not waited for again, and the walk goes on: the groups' barriers stay complete)
@@ -386,10 +455,7 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         __syncwarp();
         T *sx = reinterpret_cast<T *>(ring + s * stage_bytes), *sg = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD >= 1 ? slot_bytes : 0U)),
           *sd = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD == 2 ? 2U * slot_bytes : 0U));
-        for (unsigned r = group; r < a.tile_rows; r += GROUPS) {
-            const unsigned at = (r < here ? r : 0U) * cols;
-            work(row0 + r, r < here, sx + at, sg + at, sd + at, out == nullptr ? nullptr : sx + at);
-        }
+        work(row0, here, sx, sg, sd, out == nullptr ? nullptr : sx);
         // the warp that finishes the tile sends it off and fetches the next one for its stage
         fence_proxy_async_smem();
         __syncwarp();
@@ -434,12 +500,12 @@ layer_norm_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const fl
 {
     gdb_pdl_sync();
     constexpr int GROUPS = LN_BWD_THREADS / TPR;
-    extern __shared__ float sums[];   // [groups, 2, cols]
+    extern __shared__ __align__(16) float sums[];   // [groups, 2, cols]
     __shared__ float2 sh[64];
     const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     ln_pairs<T, VE, TPR> wf;
-    wf.load(w, t, cols, w != nullptr, 1.0f);
-    ln_sums sums2;
+    if (w != nullptr) wf.load(w, t, cols); else wf.fill(1.0f);
+    ln_sums<LN_EPT> sums2;
     const float inv_cols = 1.0f / (float)cols;
     const size_t stride = (size_t)gridDim.x * GROUPS;
     unsigned flip = 0;
@@ -448,8 +514,9 @@ layer_norm_bwd_kernel(const T *__restrict__ x, const T *__restrict__ w, const fl
         const size_t row = TPR < 32 ? first + (group & (32U / (TPR < 32 ? TPR : 32) - 1U)) : first;
         const bool live = row < rows;
         const size_t at = (live ? row : 0) * cols;
-        ln_backward_row<T, VE, TPR>(x + at, g + at, dx + at, dx == nullptr ? nullptr : dx + at, live, add_to_dx, live ? stats[row] : make_float2(0.0f, 0.0f), wf, sums2, inv_cols, t,
-                                    cols, sh, flip);
+        const bool lives[1] = {live};
+        const float2 st[1] = {live ? stats[row] : make_float2(0.0f, 0.0f)};
+        ln_backward_rows<T, VE, TPR, LN_EPT, 1>(x + at, g + at, dx + at, dx == nullptr ? nullptr : dx + at, 0, lives, add_to_dx, st, wf, sums2, inv_cols, t, cols, sh, flip);
     }
     if (partial == nullptr) return;
     // the groups' sums, added in order
@@ -546,45 +613,51 @@ struct ln_call {
     bool add_to_dx;
 };
 
-// threads of a row: enough for 16 elements each
-#define LN_BY_WIDTH(GO, VE)                                                                                                                                   \
-    (a.cols <= 8U * LN_EPT      ? GO(8, VE)                                                                                                                   \
-     : a.cols <= 16U * LN_EPT   ? GO(16, VE)                                                                                                                  \
-     : a.cols <= 32U * LN_EPT   ? GO(32, VE)                                                                                                                  \
-     : a.cols <= 64U * LN_EPT   ? GO(64, VE)                                                                                                                  \
-     : a.cols <= 128U * LN_EPT  ? GO(128, VE)                                                                                                                 \
-     : a.cols <= 256U * LN_EPT  ? GO(256, VE)                                                                                                                 \
+// threads of a row: enough for EPT elements each
+#define LN_BY_WIDTH(GO, VE, EPT)                                                                                                                                   \
+    (a.cols <= 8U * EPT      ? GO(8, VE)                                                                                                                   \
+     : a.cols <= 16U * EPT   ? GO(16, VE)                                                                                                                  \
+     : a.cols <= 32U * EPT   ? GO(32, VE)                                                                                                                  \
+     : a.cols <= 64U * EPT   ? GO(64, VE)                                                                                                                  \
+     : a.cols <= 128U * EPT  ? GO(128, VE)                                                                                                                 \
+     : a.cols <= 256U * EPT  ? GO(256, VE)                                                                                                                 \
                                 : GO(512, VE))
 
 // Tiles of the streaming kernel: rows for all groups of a block, more where rows are short (16 KB a tile keep the copies large) or where
 // the tile would not begin on 16 bytes; false where three stages of them do not fit, the pointers are not aligned, or there are too few
 // tiles for the ring to be of use (below two a block the direct kernels have the shorter way).
-template <typename T, int TPR>
+template <typename T, int TPR, int EPT>
 bool ln_tiles(const gd_backend *be, const ln_call &a, int streams, ln_stream *st, unsigned *blocks)
 {
+    if (a.cols > (size_t)TPR * EPT) return false;
     constexpr unsigned GROUPS = LN_THREADS / TPR;
     if (((uintptr_t)a.x | (uintptr_t)a.g | (uintptr_t)(streams == 1 ? a.out : a.dx)) % 16U != 0U) return false;
     size_t r = GROUPS;
+    // backward takes two rows of a group at a time; with the old gradient as a third stream the tiles stay the same, and with them the
+    // order of the weight's and the bias's sums
+    const int counted = streams > 1 ? 2 : 1;
+    if (counted == 2 && 12U * GROUPS * a.cols * sizeof(T) <= LN_RING_BYTES) r *= 2U;
     while (r * a.cols * sizeof(T) % 16U != 0U || (r < 8U * GROUPS && 2U * r * a.cols * sizeof(T) <= 16384U)) r *= 2U;
     const size_t bytes = r * a.cols * sizeof(T), slot = (bytes + 127U) & ~(size_t)127U;
     const size_t stages = LN_RING_BYTES / (slot * streams), tiles = (a.rows + r - 1U) / r;
-    if (stages < 3U || tiles < 2U * (size_t)be->sm_count) return false;
+    if (LN_RING_BYTES / (slot * counted) < 3U || tiles < 2U * (size_t)be->sm_count) return false;
     st->tile_rows = (unsigned)r;
     st->tile_bytes = (unsigned)bytes;
     st->stages = (unsigned)(stages < LN_MAX_STAGES ? stages : LN_MAX_STAGES);
     *blocks = (unsigned)(tiles < (size_t)be->sm_count ? tiles : (size_t)be->sm_count);
     return true;
 }
-template <typename T, int TPR, int VE, int BWD>
+template <typename T, int TPR, int VE, int EPT, int BWD>
 gd_status stream_go(gd_backend *be, const ln_stream &st, unsigned blocks)
 {
+    auto kern = layer_norm_stream_kernel<T, TPR, VE, EPT, BWD>;
     static bool ready = false;
     if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(layer_norm_stream_kernel<T, TPR, VE, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LN_RING_BYTES);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LN_RING_BYTES);
         if (e != cudaSuccess) return gdb_fail(be, e, "layer_norm smem attribute");
         ready = true;
     }
-    gdb_launch(layer_norm_stream_kernel<T, TPR, VE, BWD>, blocks, LN_THREADS, LN_RING_BYTES, be->stream, st, be->err_flag);
+    gdb_launch(kern, blocks, LN_THREADS, LN_RING_BYTES, be->stream, st, be->err_flag);
     return gdb_launched(be, BWD ? "layer_norm_backward" : "layer_norm_forward");
 }
 ln_stream ln_stream_of(const ln_call &a, bool backward, float *partial)
@@ -603,16 +676,24 @@ ln_stream ln_stream_of(const ln_call &a, bool backward, float *partial)
     return st;
 }
 
+// The streaming kernel where it takes the call; GD_ERR_UNSUPPORTED where it does not. Backward, FP32 rows have 8 elements a thread (two
+// rows of a group then fit the ring).
+template <typename T, int VE, int BWD>
+gd_status stream_typed(gd_backend *be, const ln_call &a, float *partial, unsigned *blocks)
+{
+    constexpr int EPT = sizeof(T) == 2 || BWD == 0 ? 16 : 8;
+    ln_stream st = ln_stream_of(a, BWD != 0, partial);
+    if (a.cols > 512U * EPT) return GD_ERR_UNSUPPORTED;
+#define GO(TPR, V) (ln_tiles<T, TPR, EPT>(be, a, BWD + 1, &st, blocks) ? stream_go<T, TPR, V, EPT, BWD>(be, st, *blocks) : GD_ERR_UNSUPPORTED)
+    return LN_BY_WIDTH(GO, VE, EPT);
+#undef GO
+}
+
 template <typename T, int TPR, int VE>
 gd_status fwd_go(gd_backend *be, const ln_call &a)
 {
-    ln_stream stream = ln_stream_of(a, false, nullptr);
-    unsigned stream_blocks;
-    if (VE == 1 && ln_tiles<T, TPR>(be, a, 1, &stream, &stream_blocks)) return stream_go<T, TPR, VE, 0>(be, stream, stream_blocks);
     constexpr unsigned THREADS = TPR > 256 ? TPR : 256, PER = THREADS / TPR;
-    const size_t blocks = (a.rows + PER - 1U) / PER;
-    if (blocks > 0x7fffffffU) return GD_ERR_UNSUPPORTED;
-    gdb_launch(layer_norm_fwd_kernel<T, TPR, VE>, (unsigned)blocks, THREADS, 0, be->stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.out, a.stats, a.rows,
+    gdb_launch(layer_norm_fwd_kernel<T, TPR, VE>, gdb_grid_for(a.rows, PER, be, 1024U / THREADS), THREADS, 0, be->stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.out, a.stats, a.rows,
                (unsigned)a.cols, a.eps);
     return gdb_launched(be, "layer_norm_forward");
 }
@@ -627,18 +708,19 @@ gd_status fwd_typed(gd_backend *be, const ln_call &a)
         return gdb_launched(be, "layer_norm_forward");
     }
     const bool vec = a.cols % VE == 0U && (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.b | (uintptr_t)a.out) % 16U) == 0U;
+    if (!vec) {
+        unsigned blocks;
+        const gd_status st = stream_typed<T, 1, 0>(be, a, nullptr, &blocks);
+        if (st != GD_ERR_UNSUPPORTED) return st;
+    }
 #define GO(TPR, V) fwd_go<T, TPR, V>(be, a)
-    return vec ? LN_BY_WIDTH(GO, VE) : LN_BY_WIDTH(GO, 1);
+    return vec ? LN_BY_WIDTH(GO, VE, LN_EPT) : LN_BY_WIDTH(GO, 1, LN_EPT);
 #undef GO
 }
 
 template <typename T, int TPR, int VE>
 gd_status bwd_go(gd_backend *be, const ln_call &a, float *partial, unsigned max_blocks, unsigned *blocks)
 {
-    ln_stream stream = ln_stream_of(a, true, partial);
-    if (max_blocks >= (unsigned)be->sm_count && ln_tiles<T, TPR>(be, a, a.add_to_dx ? 3 : 2, &stream, blocks)) {
-        return a.add_to_dx ? stream_go<T, TPR, VE, 2>(be, stream, *blocks) : stream_go<T, TPR, VE, 1>(be, stream, *blocks);
-    }
     constexpr unsigned PER = LN_BWD_THREADS / TPR;
     const size_t need = (a.rows + PER - 1U) / PER;
     *blocks = (unsigned)(need < max_blocks ? need : max_blocks);
@@ -684,9 +766,14 @@ gd_status bwd_typed(gd_backend *be, const ln_call &a)
     } else {
         const unsigned most = (unsigned)(!sums || fit > (size_t)be->sm_count ? (size_t)be->sm_count : fit);
         const bool vec = a.cols % VE == 0U && (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.g | (uintptr_t)a.dx) % 16U) == 0U;
+        st = most < (unsigned)be->sm_count ? GD_ERR_UNSUPPORTED
+             : a.add_to_dx                 ? (vec ? stream_typed<T, VE, 2>(be, a, partial, &blocks) : stream_typed<T, 1, 2>(be, a, partial, &blocks))
+                                           : (vec ? stream_typed<T, VE, 1>(be, a, partial, &blocks) : stream_typed<T, 1, 1>(be, a, partial, &blocks));
+        if (st == GD_ERR_UNSUPPORTED) {
 #define GO(TPR, V) bwd_go<T, TPR, V>(be, a, partial, most, &blocks)
-        st = vec ? LN_BY_WIDTH(GO, VE) : LN_BY_WIDTH(GO, 1);
+            st = vec ? LN_BY_WIDTH(GO, VE, LN_EPT) : LN_BY_WIDTH(GO, 1, LN_EPT);
 #undef GO
+        }
     }
     if (st != GD_OK || !sums) return st;
     gdb_launch(layer_norm_merge_kernel<T>, (unsigned)((2U * a.cols + 31U) / 32U), 1024, 0, be->stream, (const float *)partial, (T *)a.dw, (T *)a.db, blocks, a.cols);
