@@ -75,7 +75,7 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
 {
     gdb_pdl_sync();
     extern __shared__ unsigned counters[];   // [warps, width], then the slice's running sums
-    __shared__ unsigned warp_sum[ES_SORT_WARPS], below_sum[ES_SORT_WARPS];
+    __shared__ unsigned warp_sum[ES_SORT_WARPS], below_sum[ES_SORT_WARPS], absent[ES_MAX_WIDTH / 32U];   // absent: a bit per token without an id
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned v0 = blockIdx.x * width, w = min(width, vocab - v0);
     unsigned *mine = counters + (size_t)warp * width;
@@ -132,16 +132,19 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
                 at += c;
             }
         }
-        // rows that no id names
-        if (clear != nullptr) {
-            const V zero = {};
-            for (unsigned s = __ballot_sync(0xffffffffU, k < w && total == 0U); s != 0U; s &= s - 1U) {
-                V *row = clear + (size_t)(v0 + k0 + warp * 32U + (unsigned)__ffs(s) - 1U) * row_vecs;
-                for (size_t c = lane; c < row_vecs; c += 32U) row[c] = zero;
-            }
-        }
+        const unsigned none = __ballot_sync(0xffffffffU, k < w && total == 0U);
+        if (lane == 0 && k0 + warp * 32U < w) absent[k0 / 32U + warp] = none;
         base += all;
         __syncthreads();
+    }
+    // rows that no id names
+    if (clear != nullptr) {
+        const V zero = {};
+        for (unsigned k = warp; k < w; k += ES_SORT_WARPS) {
+            if (((absent[k / 32U] >> (k & 31U)) & 1U) == 0U) continue;
+            V *row = clear + (size_t)(v0 + k) * row_vecs;
+            for (size_t c = lane; c < row_vecs; c += 32U) row[c] = zero;
+        }
     }
     if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) count[0] = base;
     // the same ranges again: every id of the slice to its place, equal ids of a warp's 32 in lane order
@@ -154,7 +157,12 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
             const unsigned k = id[u] - v0;
             const bool in = k < w;
             if (__ballot_sync(0xffffffffU, in) == 0U) continue;
-            const unsigned peers = __match_any_sync(0xffffffffU, in ? k : w + lane);
+            // lanes with the same token, a bit of it at a time (a match instruction took three times as long)
+            unsigned peers = __ballot_sync(0xffffffffU, in);
+            for (unsigned bit = 1U; bit < w; bit <<= 1) {
+                const unsigned set = __ballot_sync(0xffffffffU, (k & bit) != 0U);
+                peers &= (k & bit) != 0U ? set : ~set;
+            }
             const unsigned before = __popc(peers & ((1U << lane) - 1U));
             unsigned at = 0U;
             if (in) at = mine[k] + before;
@@ -418,7 +426,9 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     unsigned width = (vocab + (unsigned)be->sm_count - 1U) / (unsigned)be->sm_count;
     if (width > ES_MAX_WIDTH) width = ES_MAX_WIDTH;
     const unsigned slices = (vocab + width - 1U) / width;
-    const int smem = (int)(width * ES_SORT_WARPS * sizeof(unsigned));
+    // (more than half of an SM's shared memory: blocks that start while the preceding kernel drains would pair up on the SMs it left first)
+    int smem = (int)(width * ES_SORT_WARPS * sizeof(unsigned));
+    if (smem < 116 * 1024) smem = 116 * 1024;
     static bool ready = false;
     if (!ready) {
         const int most = (int)(ES_MAX_WIDTH * ES_SORT_WARPS * sizeof(unsigned));
