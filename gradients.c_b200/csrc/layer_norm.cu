@@ -843,7 +843,7 @@ gd_status gdb200_layer_norm_backward(gd_backend *be, const gd_backend_tensor_vie
     void *xp, *wp, *sp, *gp, *dxp, *dwp, *dbp;
     if (!ln_ptr(x, x->dtype, n, &xp) || !ln_ptr(weight, x->dtype, args->cols, &wp) || !ln_ptr(stats, GDB_DTYPE_F32, 2U * args->rows, &sp) ||
         !ln_ptr(grad_out, x->dtype, n, &gp) || !ln_ptr(grad_x, x->dtype, n, &dxp) || !ln_ptr(grad_weight, x->dtype, args->cols, &dwp) ||
-        !ln_ptr(grad_bias, x->dtype, args->cols, &dbp) || ((uintptr_t)sp % 8U) != 0U) {
+        !ln_ptr(grad_bias, x->dtype, args->cols, &dbp) || ((uintptr_t)sp % 8U) != 0U || (accumulate != 0 && dxp == gp)) {
         return GD_ERR_INVALID_ARGUMENT;
     }
     if (args->rows == 0U) {

@@ -129,6 +129,15 @@ class OrthogonalizeArgs(C.Structure):
     _fields_ = [("batch", U64), ("rows", U64), ("cols", U64), ("steps", U32), ("a", F), ("b", F), ("c", F), ("eps", F)]
 
 
+class MuonDesc(C.Structure):
+    _fields_ = [("param_buffer", P), ("param_offset", SZ), ("master_buffer", P), ("master_offset", SZ), ("grad_buffer", P), ("grad_offset", SZ),
+                ("grad_scale_buffer", P), ("grad_scale_offset", SZ), ("found_inf_buffer", P), ("found_inf_offset", SZ),
+                ("momentum_buffer", P), ("momentum_offset", SZ), ("direction_buffer", P), ("direction_offset", SZ), ("update_buffer", P), ("update_offset", SZ),
+                ("steps_buffer", P), ("param_step_offset", SZ), ("optimizer_step_offset", SZ), ("count", U64),
+                ("param_dtype", U32), ("grad_dtype", U32), ("update_dtype", U32), ("nesterov", I32_T), ("update_optimizer_step", I32_T),
+                ("momentum", F), ("step", F), ("decay", F)]
+
+
 GPT_MAX_LAYERS = 64
 GPT_MAX_PARAMS = 1 + 10 * GPT_MAX_LAYERS + 3
 
@@ -324,6 +333,8 @@ PROTOTYPES = {
     "gdb200_embedding_sorted_backward": (_ST, [P, TV, TV, TV, I32_T, F, C.POINTER(EmbeddingArgs)]),
     "gdb200_orthogonalize_scratch_bytes": (SZ, [C.POINTER(OrthogonalizeArgs)]),
     "gdb200_orthogonalize": (_ST, [P, TV, TV, TV, C.POINTER(OrthogonalizeArgs)]),
+    "gdb200_muon_momentum_batch": (_ST, [P, C.POINTER(MuonDesc), U32]),
+    "gdb200_muon_apply_batch": (_ST, [P, C.POINTER(MuonDesc), U32]),
     "gdb200_matmul_tn_colsum": (_ST, [P, MV, MV, MV, VV]),
     "gdb200_argmax_rows": (_ST, [P, TV, F, TV]),
     "gdb200_gpt_prefill": (_ST, [P, C.POINTER(GptSpec), C.POINTER(GptBatch), SZ, SZ, C.POINTER(GptDecodeState), C.POINTER(SZ)]),

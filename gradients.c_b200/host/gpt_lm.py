@@ -18,7 +18,7 @@ import numpy as np
 
 from . import abi, ops
 from .abi import F16, BF16, F32, I32, U16, BackendError
-from .optim import AdamW, AdamwConfig, AmpConfig, AmpScaler, gd_backward_amp
+from .optim import AdamW, AdamwConfig, AmpConfig, AmpScaler, Muon, MuonConfig, gd_backward_amp
 from .runtime import Context, Tensor
 
 MASK64 = (1 << 64) - 1
@@ -247,10 +247,14 @@ class GptLm:
     def n_params(self) -> int:
         return sum(t.count for t in self.params.values())
 
-    def make_optimizer(self, config: AdamwConfig) -> AdamW:
+    def make_optimizer(self, config: AdamwConfig, muon: Optional[MuonConfig] = None) -> AdamW:
+        """AdamW for every parameter, or with `muon` Muon for the blocks' matrices and AdamW for the embedding, the head, norms and biases."""
         names = list(self.params.keys())
         wds = [config.weight_decay if self.weight_decay_mask[n] else 0.0 for n in names]
-        return AdamW(self.ctx, [self.params[n] for n in names], config, wds)
+        params = [self.params[n] for n in names]
+        if muon is not None:
+            return Muon(self.ctx, params, muon, config, wds, [i for i, n in enumerate(names) if n.startswith("blocks.") and len(params[i].shape) == 2])
+        return AdamW(self.ctx, params, config, wds)
 
     # ---- forward ----
     def _site_seed(self, site: int, layer: int, step: int) -> int:
@@ -426,6 +430,7 @@ class TrainConfig:
     weight_decay: float = 1.0e-4
     grad_clip_norm: float = 1.0
     amp: AmpConfig = field(default_factory=AmpConfig)
+    muon: Optional[MuonConfig] = None   # the blocks' matrices by Muon (Trainer; NativeTrainer's sequence has AdamW only)
 
     @staticmethod
     def baseline() -> "TrainConfig":
@@ -437,7 +442,7 @@ class Trainer:
 
     def __init__(self, model: GptLm, cfg: TrainConfig, dp=None):
         self.model, self.cfg, self.ctx = model, cfg, model.ctx
-        self.optimizer = model.make_optimizer(AdamwConfig(cfg.lr, cfg.beta1, cfg.beta2, cfg.eps, cfg.weight_decay, True))
+        self.optimizer = model.make_optimizer(AdamwConfig(cfg.lr, cfg.beta1, cfg.beta2, cfg.eps, cfg.weight_decay, True), cfg.muon)
         self.scaler = AmpScaler(self.ctx, cfg.amp)
         self.global_step = 0
         self.dp = dp
@@ -472,6 +477,8 @@ class NativeTrainer(Trainer):
     rounding points and results are the same; only the host that enqueues the calls differs."""
 
     def __init__(self, model: GptLm, cfg: TrainConfig, dp=None):
+        if cfg.muon is not None:
+            raise ValueError("the native step sequence updates by AdamW; Muon runs in Trainer")
         super().__init__(model, cfg, dp)
         import ctypes as C
         self._C = C

@@ -64,6 +64,28 @@ def gd_embedding(ctx: Context, table: Tensor, ids: Tensor) -> Tensor:
     return out
 
 
+def gd_embedding_scaled(ctx: Context, table: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
+    """out = scale * table[ids] (gdb200_embedding_scaled_forward). The backward pass sorts the ids and adds the rows of each token in their
+    order: no FP32 table, the same bits on every call; a gradient that the table has already (a tied head's) is added to in the same call."""
+    vocab, dim = table.shape
+    out = ctx.scratch_empty(table.dtype, ids.shape + (dim,), "embedding_scaled")
+    args = abi.EmbeddingArgs(ids.count, vocab, dim)
+    ctx.check(ctx.lib.gdb200_embedding_scaled_forward(ctx.backend, _tvp(table), _tvp(ids), _tvp(out), scale, byref(args)), "embedding_scaled_forward")
+    out.requires_grad = table.requires_grad
+    if table.requires_grad:
+        def backward():
+            if out.grad is None:
+                return
+            into = table.grad is not None
+            dtable = table.grad if into else ctx.scratch_empty(table.dtype, table.shape, "d_table")
+            ctx.check(ctx.lib.gdb200_embedding_sorted_backward(ctx.backend, _tvp(out.grad), _tvp(ids), _tvp(dtable), 1 if into else 0, scale, byref(args)),
+                      "embedding_sorted_backward")
+            if not into:
+                ctx.accumulate_grad(table, dtable)
+        ctx.record(backward)
+    return out
+
+
 # --------------------------------------------------------------------------- dropout
 def _dropout_backward_mask(ctx: Context, mask: Tensor, grad_out: Tensor, scale: float) -> Tensor:
     dx = ctx.scratch_empty(grad_out.dtype, grad_out.shape, "d_dropout")
@@ -184,6 +206,41 @@ def gd_rms_norm(ctx: Context, x: Tensor, weight: Tensor, eps: float) -> Tensor:
                 partial = ctx.scratch_empty(F32, (args.row_blocks, cols), "rms_partial")
                 ctx.check(ctx.lib.gd_backend_rms_norm_weight_backward_stats(ctx.backend, _tvp(x), _tvp(inv), _tvp(out.grad), _tvp(dw), _tvp(partial), byref(args)), "rms_norm_weight_backward_stats")
                 ctx.accumulate_grad(weight, dw)
+        ctx.record(backward)
+    return out
+
+
+# --------------------------------------------------------------------------- layer_norm
+def gd_layer_norm(ctx: Context, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1.0e-5) -> Tensor:
+    """y = (x - mean) / sqrt(var + eps) * w + b over the last dimension, saving mean and 1 / sqrt(var + eps) of the rows
+    (gdb200_layer_norm_forward); weight and bias may be None. One backward call gives all three gradients and adds into one that x has."""
+    rows, cols = _flat2(x)
+    args = abi.LayerNormArgs(rows, cols, eps, 0)
+    out = ctx.scratch_empty(x.dtype, x.shape, "layer_norm")
+    learn_w, learn_b = weight is not None and weight.requires_grad, bias is not None and bias.requires_grad
+    needs_grad = ctx.grad_enabled and (x.requires_grad or learn_w or learn_b)
+    stats = ctx.scratch_empty(F32, (rows, 2), "layer_norm_stats") if needs_grad else None
+    ctx.check(ctx.lib.gdb200_layer_norm_forward(ctx.backend, _tvp(x), _tvp(weight), _tvp(bias), _tvp(out), _tvp(stats), byref(args)), "layer_norm_forward")
+    out.requires_grad = needs_grad
+    if needs_grad:
+        def backward():
+            if out.grad is None:
+                return
+            # (a residual connection may have given x the very tensor that is out's gradient)
+            into = x.requires_grad and x.grad is not None and x.grad is not out.grad
+            dx = None
+            if x.requires_grad:
+                dx = x.grad if into else ctx.scratch_empty(x.dtype, x.shape, "d_layer_norm_x")
+            dw = ctx.scratch_empty(weight.dtype, weight.shape, "d_layer_norm_w") if learn_w else None
+            db = ctx.scratch_empty(bias.dtype, bias.shape, "d_layer_norm_b") if learn_b else None
+            ctx.check(ctx.lib.gdb200_layer_norm_backward(ctx.backend, _tvp(x), _tvp(weight), _tvp(stats), _tvp(out.grad), _tvp(dx), 1 if into else 0, _tvp(dw), _tvp(db),
+                                                         byref(args)), "layer_norm_backward")
+            if dx is not None and not into:
+                ctx.accumulate_grad(x, dx)
+            if dw is not None:
+                ctx.accumulate_grad(weight, dw)
+            if db is not None:
+                ctx.accumulate_grad(bias, db)
         ctx.record(backward)
     return out
 

@@ -1,4 +1,4 @@
-"""AdamW with FP32 master weights, device-side AMP loss scaling and global-norm clipping.
+"""AdamW (and Muon for matrices) with FP32 master weights, device-side AMP loss scaling and global-norm clipping.
 
 Mirrors the reference optimizer's host logic for the path gpt_lm uses
 (src/optim/adamw.c: gd_amp_scaler_* :1099-1352, gd_backward_amp seed :1354-1395,
@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import abi
-from .abi import F16, BF16, F32, I32
+from .abi import F16, BF16, F32, I32, U8
 from .runtime import Context, Tensor
 
 byref = C.byref
@@ -43,6 +43,19 @@ class AdamwConfig:  # gd_adamw_config_default, src/optim/adamw.c:1087-1097
     eps: float = 1.0e-8
     weight_decay: float = 0.01
     bias_correction: bool = True
+
+
+@dataclass
+class MuonConfig:
+    """Muon: matrices step along the orthogonalised momentum of their gradients, W <- W - lr * update_rms * sqrt(max(rows, cols)) * O - lr *
+    weight_decay * W. The factor gives a step of any matrix the root mean square lr * update_rms, about that of an AdamW step, so that both
+    share a learning rate; the three coefficients are those of the Newton-Schulz polynomial a x + b x^3 + c x^5."""
+    momentum: float = 0.95
+    nesterov: bool = True
+    steps: int = 5
+    coefficients: tuple = (3.4445, -4.7750, 2.0315)
+    eps: float = 1.0e-7
+    update_rms: float = 0.2
 
 
 def gd_lr_scheduler_value(max_lr: float, min_lr: float, warmup_steps: int, total_steps: int, step: int) -> float:
@@ -115,7 +128,7 @@ class ParamSlot:
     lr_mult: float
     master: Optional[Tensor]
     m: Tensor
-    v: Tensor
+    v: Optional[Tensor]   # None: stepped by Muon, which has no second moment
 
 
 class AdamW:
@@ -125,7 +138,8 @@ class AdamW:
 
     F_BETA1, F_BETA2, F_STEP, F_DECAY, F_EPS = range(5)
 
-    def __init__(self, ctx: Context, params: Sequence[Tensor], config: AdamwConfig, weight_decays: Optional[Sequence[float]] = None):
+    def __init__(self, ctx: Context, params: Sequence[Tensor], config: AdamwConfig, weight_decays: Optional[Sequence[float]] = None, *,
+                 without_v: Sequence[int] = ()):
         self.ctx, self.config = ctx, config
         self.slots: list[ParamSlot] = []
         for i, p in enumerate(params):
@@ -135,7 +149,7 @@ class AdamW:
                 master = ctx.empty(ctx.state, F32, p.shape, "master")
                 master.write(p.read_f32())
             m = ctx.zeros(ctx.state, F32, p.shape, "adam_m")
-            v = ctx.zeros(ctx.state, F32, p.shape, "adam_v")
+            v = None if i in without_v else ctx.zeros(ctx.state, F32, p.shape, "adam_v")
             self.slots.append(ParamSlot(p, wd, 1.0, master, m, v))
         n = len(self.slots)
         f32 = np.zeros((5, n), dtype=np.float32)
@@ -193,6 +207,11 @@ class AdamW:
             return
         ctx.check(lib.gd_backend_grad_clip_scale(ctx.backend, self._norm_descs, count, self.grad_clip_scale.buffer,
                                                  self.grad_clip_scale.offset, max_grad_norm, GRAD_CLIP_SCALE_EPS), "grad_clip_scale")
+        self._update(active, lr, found_buf, found_off)
+        scaler.finish_step()
+
+    def _update(self, active: Sequence[int], lr: float, found_buf, found_off: int) -> None:
+        """The AdamW update of the slots `active`."""
         cfg = self.config
         bias_correction = 1 if cfg.bias_correction else 0
         shared = (self.state_f32, self.state_i32, self.grad_clip_scale)   # a program may put others in their place
@@ -208,8 +227,7 @@ class AdamW:
             d.found_inf_buffer, d.found_inf_offset = found_buf, found_off
             d.bias_correction = bias_correction
             d.lr, d.beta1, d.beta2, d.eps, d.weight_decay = lr * s.lr_mult, cfg.beta1, cfg.beta2, cfg.eps, s.weight_decay
-        ctx.check(lib.gd_backend_adamw_batch(ctx.backend, self._adamw_descs, count), "adamw_batch")
-        scaler.finish_step()
+        self.ctx.check(self.ctx.lib.gd_backend_adamw_batch(self.ctx.backend, self._adamw_descs, len(active)), "adamw_batch")
 
     def _lay_out(self, d: abi.AdamwDesc, i: int, s: ParamSlot, first: bool) -> None:
         """The fields of slot i's descriptor that stay as they are from step to step."""
@@ -235,3 +253,81 @@ class AdamW:
     def zero_grad(self) -> None:
         for s in self.slots:
             s.param.grad = None
+
+
+class Muon(AdamW):
+    """Muon for the parameters `matrices` (indices into params; None: all of rank 2), AdamW for the others, in one step with one gradient norm,
+    one loss scale and one overflow flag. A matrix keeps its momentum where AdamW keeps the first moment (slot.m) and has no second one.
+    Equal shapes are orthogonalised in one call; directions and updates lie in the scratch arena while the step's calls are enqueued."""
+
+    def __init__(self, ctx: Context, params: Sequence[Tensor], config: MuonConfig, adamw: AdamwConfig, weight_decays: Optional[Sequence[float]] = None,
+                 matrices: Optional[Sequence[int]] = None):
+        params = list(params)
+        chosen = [i for i, p in enumerate(params) if len(p.shape) == 2] if matrices is None else sorted({int(i) for i in matrices})
+        for i in chosen:
+            if not 0 <= i < len(params) or len(params[i].shape) != 2 or params[i].count == 0:
+                raise ValueError(f"Muon steps along matrices: parameter {i} is none")
+        if config.steps < 1 or len(config.coefficients) != 3:
+            raise ValueError("Muon takes one Newton-Schulz step or more and three coefficients")
+        self.muon = config
+        self.scratch_need: dict[tuple, int] = {}   # (matrices, rows, cols) of a group: bytes of the orthogonalisation's scratch
+        for shape in {params[i].shape for i in chosen}:
+            self._scratch_bytes(ctx, (1,) + shape)
+        super().__init__(ctx, params, adamw, weight_decays, without_v=chosen)
+        self.matrices = chosen
+        self._muon_descs = (abi.MuonDesc * max(1, len(chosen)))()
+
+    def _args(self, shape: tuple) -> abi.OrthogonalizeArgs:
+        c = self.muon
+        return abi.OrthogonalizeArgs(*shape, c.steps, *c.coefficients, c.eps)
+
+    def _scratch_bytes(self, ctx: Context, shape: tuple) -> int:
+        need = self.scratch_need.get(shape)
+        if need is None:
+            need = self.scratch_need[shape] = int(ctx.lib.gdb200_orthogonalize_scratch_bytes(byref(self._args(shape))))
+            if need == 0:
+                raise ValueError(f"Muon does not take {shape[0]} matrices of {shape[1]} x {shape[2]}")
+        return need
+
+    def _update(self, active: Sequence[int], lr: float, found_buf, found_off: int) -> None:
+        chosen = set(self.matrices)
+        rest = [i for i in active if i not in chosen]
+        super()._update(rest, lr, found_buf, found_off)
+        groups: dict[tuple, list[int]] = {}
+        for i in active:
+            if i in chosen:
+                groups.setdefault(self.slots[i].param.shape, []).append(i)
+        if not groups:
+            return
+        ctx, lib, cfg, descs = self.ctx, self.ctx.lib, self.muon, self._muon_descs
+        mark, count, work = ctx.scratch.top, 0, []
+        for shape, members in groups.items():
+            full = (len(members),) + shape
+            direction = ctx.scratch_empty(F32, full, "muon_direction")
+            update = ctx.scratch_empty(F16, full, "muon_update")
+            work.append((full, direction, update))
+            for i, d_i, u_i in ((i, direction.rows(k, 1), update.rows(k, 1)) for k, i in enumerate(members)):
+                s, d = self.slots[i], descs[count]
+                p, g = s.param, s.param.grad
+                d.param_buffer, d.param_offset, d.param_dtype, d.count = p.buffer, p.offset, p.dtype, p.count
+                d.master_buffer, d.master_offset = (s.master.buffer, s.master.offset) if s.master is not None else (None, 0)
+                d.grad_buffer, d.grad_offset, d.grad_dtype = g.arena.buffer, g.offset, g.dtype
+                d.grad_scale_buffer, d.grad_scale_offset = self.grad_clip_scale.buffer, self.grad_clip_scale.offset
+                d.found_inf_buffer, d.found_inf_offset = found_buf, found_off
+                d.momentum_buffer, d.momentum_offset = s.m.buffer, s.m.offset
+                d.direction_buffer, d.direction_offset = d_i.buffer, d_i.offset
+                d.update_buffer, d.update_offset, d.update_dtype = u_i.buffer, u_i.offset, F16
+                d.steps_buffer, d.param_step_offset = self.state_i32.buffer, self.state_i32.offset + i * 4
+                d.optimizer_step_offset, d.update_optimizer_step = self.state_i32.offset + self.n * 4, 1 if not rest and count == 0 else 0
+                d.nesterov, d.momentum = 1 if cfg.nesterov else 0, cfg.momentum
+                rate = lr * s.lr_mult
+                d.step, d.decay = rate * cfg.update_rms * math.sqrt(max(shape)), rate * s.weight_decay
+                count += 1
+        ctx.check(lib.gdb200_muon_momentum_batch(ctx.backend, descs, count), "muon_momentum_batch")
+        for full, direction, update in work:
+            top = ctx.scratch.top     # one scratch for all groups: their calls follow one another on the stream
+            lent = ctx.scratch_empty(U8, (self._scratch_bytes(ctx, full),), "muon_scratch")
+            ctx.check(lib.gdb200_orthogonalize(ctx.backend, direction.ref(), update.ref(), lent.ref(), byref(self._args(full))), "orthogonalize")
+            ctx.scratch.top = top
+        ctx.check(lib.gdb200_muon_apply_batch(ctx.backend, descs, count), "muon_apply_batch")
+        ctx.scratch.top = mark

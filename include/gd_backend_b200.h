@@ -581,6 +581,41 @@ size_t gdb200_orthogonalize_scratch_bytes(const gdb200_orthogonalize_args *args)
 gd_status gdb200_orthogonalize(gd_backend *backend, const gd_backend_tensor_view *x, const gd_backend_tensor_view *out, const gd_backend_tensor_view *scratch,
                                const gdb200_orthogonalize_args *args);
 
+/* The elementwise halves of a Muon step for any number of tensors in one call (the optimizer stands beside AdamW, src/optim/adamw.c; its
+ * clipping and loss scale are AdamW's). gdb200_muon_momentum_batch: g = grad * grad_scale (0 where the scale is 0), momentum <- mu *
+ * momentum + g, direction = nesterov ? g + mu * momentum : momentum; with an overflow found the momentum stays and the direction is zeros.
+ * gdb200_muon_apply_batch: p <- p - step * update - decay * p in FP32 on the master (param itself where master_buffer is NULL), param =
+ * round(p), the step counters + 1; with an overflow found nothing changes. Between the two a caller orthogonalises the directions into the
+ * updates. Each entry reads and checks its own fields only, all descriptors before the first launch. momentum, direction and master are
+ * F32, the other dtypes any of F16, BF16, F32; grad_scale, found_inf, master and steps may be NULL; count > 0. */
+typedef struct gdb200_muon_desc {
+    gd_backend_buffer *param_buffer;
+    size_t param_offset;
+    gd_backend_buffer *master_buffer;
+    size_t master_offset;
+    gd_backend_buffer *grad_buffer;
+    size_t grad_offset;
+    gd_backend_buffer *grad_scale_buffer;
+    size_t grad_scale_offset;
+    gd_backend_buffer *found_inf_buffer;
+    size_t found_inf_offset;
+    gd_backend_buffer *momentum_buffer;
+    size_t momentum_offset;
+    gd_backend_buffer *direction_buffer;
+    size_t direction_offset;
+    gd_backend_buffer *update_buffer;
+    size_t update_offset;
+    gd_backend_buffer *steps_buffer;      /* U32 counters */
+    size_t param_step_offset;
+    size_t optimizer_step_offset;
+    uint64_t count;
+    uint32_t param_dtype, grad_dtype, update_dtype;
+    int32_t nesterov, update_optimizer_step;
+    float momentum, step, decay;
+} gdb200_muon_desc;
+gd_status gdb200_muon_momentum_batch(gd_backend *backend, const gdb200_muon_desc *descs, uint32_t desc_count);
+gd_status gdb200_muon_apply_batch(gd_backend *backend, const gdb200_muon_desc *descs, uint32_t desc_count);
+
 /* Native sequencing of one gpt_lm training step (no counterpart in the reference's backend ABI; it
  * replays the call sequence of the reference's host: src/train/trainer.c:75-223,
  * examples/gpt_lm/gpt_lm_shared.c:602-823, src/optim/adamw.c:2163-2270). The caller lays out
