@@ -18,8 +18,8 @@
 namespace {
 
 constexpr int ES_SORT_WARPS = 32, ES_AHEAD = 8;   // (ids on their way, a lane)
-constexpr unsigned ES_MAX_WIDTH = 1536;      // tokens of a slice: 32 x 1536 counters fill 192 KB
-constexpr int ES_WARPS = 8;                  // of a reducing block
+constexpr unsigned ES_MAX_WIDTH = 1536, ES_ZEROS = 4096, ES_SORT_SMEM = 220 * 1024;   // tokens of a slice (32 x 1536 counters fill 192 KB), bytes
+constexpr int ES_WARPS = 8, ES_BLOCKS = 4;   // of a reducing block; blocks on an SM
 
 template <typename T, int VE> struct es_vec {
     T v[VE];
@@ -67,40 +67,55 @@ es_lookup_kernel(const T *__restrict__ table, const int *__restrict__ ids, T *__
 
 // ------------------------------------------------------------------ sort
 // Block b owns tokens [b * width, (b + 1) * width). order[k] = position of the k-th id in token order, token[k] = that id; count[0] = ids
-// inside the table. `clear` != NULL: the gradient table, whose rows without an id are set to zero.
+// inside the table. `clear` != NULL: the gradient table, whose rows without an id are set to zero. A warp notes up to `notes` ids of the
+// slice, so that only a warp with more (of a frequent token) has to look at its ids again: what bounds the kernel is the instructions
+// that every block spends on every id. Whole vectors are cleared by bulk copies of zeros beside the sorting.
 template <typename V>
 __global__ void __launch_bounds__(ES_SORT_WARPS * 32)
-es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned width, unsigned *__restrict__ order, int *__restrict__ token,
+es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned width, unsigned notes, unsigned *__restrict__ order, int *__restrict__ token,
                unsigned *__restrict__ count, V *__restrict__ clear, size_t row_vecs)
 {
     gdb_pdl_sync();
-    extern __shared__ unsigned counters[];   // [warps, width], then the slice's running sums
+    constexpr bool BULK = sizeof(V) == 16U;
+    extern __shared__ uint2 sort_smem[];     // notes: [warps, notes] (position, token - v0); counters [warps, width], then places
     __shared__ unsigned warp_sum[ES_SORT_WARPS], below_sum[ES_SORT_WARPS], absent[ES_MAX_WIDTH / 32U];   // absent: a bit per token without an id
+    __shared__ __align__(128) uint4 zeros[BULK ? ES_ZEROS / 16U : 1U];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned v0 = blockIdx.x * width, w = min(width, vocab - v0);
-    unsigned *mine = counters + (size_t)warp * width;
+    uint2 *note = sort_smem + (size_t)warp * notes;
+    unsigned *counters = reinterpret_cast<unsigned *>(sort_smem + (size_t)ES_SORT_WARPS * notes), *mine = counters + (size_t)warp * width;
     for (unsigned k = threadIdx.x; k < ES_SORT_WARPS * width; k += blockDim.x) counters[k] = 0U;
+    if constexpr (BULK) {
+        if (threadIdx.x < ES_ZEROS / 16U) zeros[threadIdx.x] = make_uint4(0U, 0U, 0U, 0U);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     __syncthreads();
-    // a warp reads a range of the ids, 32 at a time, twice: counts first
+    // a warp reads a range of the ids, 32 at a time
     const unsigned per = ((n + ES_SORT_WARPS * 32U - 1U) / (ES_SORT_WARPS * 32U)) * 32U;
     const unsigned i0 = min(n, warp * per), i1 = min(n, i0 + per);
-    unsigned below = 0U;
-    for (unsigned i = i0 + lane; i < i1; i += 32U * ES_AHEAD) {
+    unsigned below = 0U, found = 0U;
+    const unsigned lower = (1U << lane) - 1U;
+    for (unsigned i = i0; i < i1; i += 32U * ES_AHEAD) {
         unsigned id[ES_AHEAD];
 #pragma unroll
-        for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u < i1 ? (unsigned)__ldg(&ids[i + 32U * u]) : 0xffffffffU;
+        for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u + lane < i1 ? (unsigned)__ldg(&ids[i + 32U * u + lane]) : 0xffffffffU;
 #pragma unroll
         for (int u = 0; u < ES_AHEAD; ++u) {
             below += id[u] < v0 ? 1U : 0U;   // (a negative id lies above every vocabulary)
-            if (id[u] - v0 < w) atomicAdd(&mine[id[u] - v0], 1U);
+            const unsigned k = id[u] - v0, here = __ballot_sync(0xffffffffU, k < w);
+            if (here == 0U) continue;
+            if (k < w) {
+                atomicAdd(&mine[k], 1U);
+                const unsigned at = found + __popc(here & lower);
+                if (at < notes) note[at] = make_uint2(i + 32U * u + lane, k);
+            }
+            found += __popc(here);
         }
     }
     below = __reduce_add_sync(0xffffffffU, below);
     if (lane == 0) below_sum[warp] = below;
     __syncthreads();
-    unsigned base = 0U;
-#pragma unroll
-    for (int k = 0; k < ES_SORT_WARPS; ++k) base += below_sum[k];
+    unsigned base = __reduce_add_sync(0xffffffffU, below_sum[lane]);
     // place of the first id of (token, warp), tokens first: a thread per token, 1024 tokens at a time
     for (unsigned k0 = 0; k0 < w; k0 += blockDim.x) {
         const unsigned k = k0 + threadIdx.x;
@@ -117,12 +132,8 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
         }
         if (lane == 31) warp_sum[warp] = incl;
         __syncthreads();
-        unsigned before = base, all = 0U;
-#pragma unroll
-        for (int s = 0; s < ES_SORT_WARPS; ++s) {
-            before += s < warp ? warp_sum[s] : 0U;
-            all += warp_sum[s];
-        }
+        const unsigned sums = warp_sum[lane], all = __reduce_add_sync(0xffffffffU, sums);
+        const unsigned before = base + __reduce_add_sync(0xffffffffU, lane < warp ? sums : 0U);
         if (k < w) {
             unsigned at = before + incl - total;
 #pragma unroll 8
@@ -131,48 +142,71 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
                 counters[(size_t)s * width + k] = at;
                 at += c;
             }
+            if constexpr (BULK) {
+                if (clear != nullptr && total == 0U) {
+                    V *row = clear + (size_t)(v0 + k) * row_vecs;
+                    const unsigned from = (unsigned)__cvta_generic_to_shared(zeros);
+                    for (size_t c = 0; c < row_vecs; c += ES_ZEROS / 16U) {
+                        const unsigned bytes = (unsigned)min(row_vecs - c, (size_t)(ES_ZEROS / 16U)) * 16U;
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(row + c), "r"(from), "r"(bytes) : "memory");
+                    }
+                }
+            }
         }
         const unsigned none = __ballot_sync(0xffffffffU, k < w && total == 0U);
-        if (lane == 0 && k0 + warp * 32U < w) absent[k0 / 32U + warp] = none;
+        if (!BULK && lane == 0 && k0 + warp * 32U < w) absent[k0 / 32U + warp] = none;
         base += all;
         __syncthreads();
     }
-    // rows that no id names
-    if (clear != nullptr) {
+    if constexpr (BULK) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) count[0] = base;
+    // every id of the slice to its place, equal ids of a warp's 32 in lane order
+    const auto put = [&](bool in, unsigned pos, unsigned k) {
+        // lanes with the same token, a bit of it at a time (a match instruction took three times as long)
+        unsigned peers = __ballot_sync(0xffffffffU, in);
+        for (unsigned bit = 1U; bit < w; bit <<= 1) {
+            const unsigned set = __ballot_sync(0xffffffffU, (k & bit) != 0U);
+            peers &= (k & bit) != 0U ? set : ~set;
+        }
+        const unsigned before = __popc(peers & lower);
+        unsigned at = 0U;
+        if (in) at = mine[k] + before;
+        __syncwarp();
+        if (in && before == 0U) mine[k] = at + __popc(peers);
+        __syncwarp();
+        if (in) {
+            order[at] = pos;
+            token[at] = (int)(v0 + k);
+        }
+    };
+    if (found <= notes) {
+        for (unsigned j = 0; j < found; j += 32U) {
+            const bool in = j + lane < found;
+            const uint2 e = in ? note[j + lane] : make_uint2(0U, 0U);
+            put(in, e.x, e.y);
+        }
+    } else {
+        for (unsigned i = i0; i < i1; i += 32U * ES_AHEAD) {
+            unsigned id[ES_AHEAD];
+#pragma unroll
+            for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u + lane < i1 ? (unsigned)__ldg(&ids[i + 32U * u + lane]) : 0xffffffffU;
+#pragma unroll 1
+            for (int u = 0; u < ES_AHEAD; ++u) {
+                unsigned k = id[0] - v0;   // (the array moves on: its places are registers)
+#pragma unroll
+                for (int m = 1; m < ES_AHEAD; ++m) id[m - 1] = id[m];
+                if (__ballot_sync(0xffffffffU, k < w) != 0U) put(k < w, i + 32U * u + lane, k);
+            }
+        }
+    }
+    if constexpr (BULK) {
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else if (clear != nullptr) {
         const V zero = {};
         for (unsigned k = warp; k < w; k += ES_SORT_WARPS) {
             if (((absent[k / 32U] >> (k & 31U)) & 1U) == 0U) continue;
             V *row = clear + (size_t)(v0 + k) * row_vecs;
             for (size_t c = lane; c < row_vecs; c += 32U) row[c] = zero;
-        }
-    }
-    if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) count[0] = base;
-    // the same ranges again: every id of the slice to its place, equal ids of a warp's 32 in lane order
-    for (unsigned i = i0; i < i1; i += 32U * ES_AHEAD) {
-        unsigned id[ES_AHEAD];
-#pragma unroll
-        for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u + lane < i1 ? (unsigned)__ldg(&ids[i + 32U * u + lane]) : 0xffffffffU;
-#pragma unroll
-        for (int u = 0; u < ES_AHEAD; ++u) {
-            const unsigned k = id[u] - v0;
-            const bool in = k < w;
-            if (__ballot_sync(0xffffffffU, in) == 0U) continue;
-            // lanes with the same token, a bit of it at a time (a match instruction took three times as long)
-            unsigned peers = __ballot_sync(0xffffffffU, in);
-            for (unsigned bit = 1U; bit < w; bit <<= 1) {
-                const unsigned set = __ballot_sync(0xffffffffU, (k & bit) != 0U);
-                peers &= (k & bit) != 0U ? set : ~set;
-            }
-            const unsigned before = __popc(peers & ((1U << lane) - 1U));
-            unsigned at = 0U;
-            if (in) at = mine[k] + before;
-            __syncwarp();
-            if (in && before == 0U) mine[k] = at + __popc(peers);
-            __syncwarp();
-            if (in) {
-                order[at] = i + 32U * u + lane;
-                token[at] = (int)id[u];
-            }
         }
     }
 }
@@ -196,24 +230,35 @@ __device__ __forceinline__ void es_store(T *p, const float *s, float scale, bool
 // Block (c, s): sorted entries [c * piece, (c + 1) * piece), a warp an eighth of them, columns [s * 32 * VE * NV, ...).
 // partial[c, 0] = sum of the run that began in an earlier piece, partial[c, 1] = of the one that begins here and goes on behind.
 template <typename T, int VE, int NV>
-__global__ void __launch_bounds__(ES_WARPS * 32)
+__global__ void __launch_bounds__(ES_WARPS * 32, ES_BLOCKS)
 es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table,
-                 float *__restrict__ partial, unsigned piece, size_t dim, float scale, bool add)
+                 float *__restrict__ partial, unsigned n, unsigned piece, size_t dim, float scale, bool add)
 {
     gdb_pdl_sync();
     typedef es_vec<T, VE> vec;
-    constexpr int COLS = 32 * VE * NV, U = NV == 1 ? 8 : 2;
-    __shared__ float head[ES_WARPS][COLS], tail[ES_WARPS][COLS];
+    // Whole vectors travel through shared memory, ES_AHEAD_ROWS rows on their way: a thread copies and reads its own 16 bytes. (As registers
+    // the rows of a ring share the few scoreboards of a warp, and waiting for one waits for those asked for last as well: 34 to 54 us
+    // where this takes 24, 16384 rows of 2048 BF16.) Single elements are fetched four rows at a time.
+    constexpr bool ASYNC = sizeof(vec) == 16U;
+    constexpr int COLS = 32 * VE * NV, SLOTS = 8, U = ASYNC ? SLOTS - 1 : 2;
+    static_assert(!ASYNC || NV == 1, "one vector per lane and row");
+    __shared__ float head[ES_WARPS][COLS];
+    __shared__ __align__(16) unsigned char ring[ES_WARPS][ASYNC ? SLOTS * 512 : COLS * 4];   // (its beginning holds the warp's last sums behind the loop)
+    const auto tail = [&](int w) { return reinterpret_cast<float *>(ring[w]); };
     // of each warp's entries: the first token, and whether its run began before them (1), goes on behind them (2), does both with one token (4);
     // 8: there are none
     __shared__ int first_token[ES_WARPS];
     __shared__ unsigned ends[ES_WARPS];
-    const unsigned total = count[0];
-    const unsigned e0 = blockIdx.x * piece;
-    if (e0 >= total) return;
-    const unsigned e1 = min(total, e0 + piece);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned per = piece / ES_WARPS, a = min(e1, e0 + warp * per), b = min(e1, a + per);
+    const unsigned e0 = blockIdx.x * piece, per = piece / ES_WARPS, a = e0 + warp * per;
+    // (all n places of the lists may be read; those behind the ids inside the table hold nothing that is used)
+    unsigned mine = a + lane < n ? __ldg(&order[a + lane]) : 0U;
+    int mine_token = a + lane < n ? __ldg(&token[a + lane]) : -1;
+    const int token_before = a > 0U && a <= n ? __ldg(&token[a - 1U]) : -1, token_after = a + per < n ? __ldg(&token[a + per]) : -1;
+    const unsigned total = count[0];
+    if (e0 >= total) return;
+    const unsigned e1 = min(total, e0 + piece), b = min(e1, a + per);
+    const bool some = a < b;
     const size_t col0 = (size_t)blockIdx.y * COLS;
     float acc[NV][VE];
 #pragma unroll
@@ -232,72 +277,88 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
         }
     };
     // runs that are not complete within the warp's entries
-    const int before = a > 0U && a < b ? token[a - 1] : -1, after = b < total && a < b ? token[b] : -1, begin = a < b ? token[a] : -1, end = a < b ? token[b - 1] : -1;
-    bool open_left = a < b && before == begin;
+    const int begin = __shfl_sync(0xffffffffU, mine_token, 0), after = b < total ? token_after : -1;
+    bool open_left = some && token_before == begin;
     int current = begin;
-    if (lane == 0) {
-        first_token[warp] = begin;
-        ends[warp] = a < b ? (before == begin ? 1U : 0U) | (after == end ? 2U : 0U) | (before == begin && after == begin ? 4U : 0U) : 8U;
-    }
-    for (unsigned i = a; i < b; i += 32U) {
-        const unsigned mine = i + lane < b ? order[i + lane] : 0U;
-        const int mine_token = i + lane < b ? token[i + lane] : -1;
-        const int here = (int)min(32U, b - i);
-        for (int k = 0; k < here; k += U) {
-            vec v[U][NV];
-            int tok[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const unsigned pos = __shfl_sync(0xffffffffU, mine, (k + u) & 31);
-                tok[u] = __shfl_sync(0xffffffffU, mine_token, (k + u) & 31);
-                if (k + u < here) {
-#pragma unroll
-                    for (int j = 0; j < NV; ++j) {
-                        const size_t c = col0 + (lane + 32 * j) * VE;
-                        if (c < dim) v[u][j] = *reinterpret_cast<const vec *>(g + (size_t)pos * dim + c);
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (k + u >= here) break;
-                if (tok[u] != current) {
-                    if (open_left) {
-                        keep(head[warp]);
-                        open_left = false;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < NV; ++j) {
-                            const size_t c = col0 + (lane + 32 * j) * VE;
-                            if (c < dim) es_store<T, VE>(table + (size_t)current * dim + c, acc[j], scale, add);
-#pragma unroll
-                            for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
-                        }
-                    }
-                    current = tok[u];
-                }
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    if (col0 + (lane + 32 * j) * VE < dim) {
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) acc[j][e] += gdb_io<T>::ld(v[u][j].v, e);
-                    }
-                }
-            }
-        }
-    }
-    if (a < b) {
+    auto finish = [&] {
         if (open_left) {
             keep(head[warp]);
-        } else if (after == current) {
-            keep(tail[warp]);
-        } else {
+            open_left = false;
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const size_t c = col0 + (lane + 32 * j) * VE;
+            if (c < dim) es_store<T, VE>(table + (size_t)current * dim + c, acc[j], scale, add);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
+        }
+    };
+    for (unsigned i = a; i < b; i += 32U) {
+        if (i != a) {
+            mine = i + lane < b ? order[i + lane] : 0U;
+            mine_token = i + lane < b ? token[i + lane] : -1;
+        }
+        const int here = (int)min(32U, b - i);
+        const auto add_row = [&](int q, const vec *row) {
+            const int tok = __shfl_sync(0xffffffffU, mine_token, q);
+            if (tok != current) {
+                finish();
+                current = tok;
+            }
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const size_t c = col0 + (lane + 32 * j) * VE;
-                if (c < dim) es_store<T, VE>(table + (size_t)current * dim + c, acc[j], scale, add);
+                if (col0 + (lane + 32 * j) * VE < dim) {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) acc[j][e] += gdb_io<T>::ld(row[j].v, e);
+                }
+            }
+        };
+        if constexpr (ASYNC) {
+            const bool inside = col0 + lane * VE < dim;
+            const unsigned slots = (unsigned)__cvta_generic_to_shared(ring[warp]) + 16U * lane;
+            const T *column = g + col0 + lane * VE;
+            const auto fetch = [&](int q) {
+                const unsigned pos = __shfl_sync(0xffffffffU, mine, q & 31);
+                if (q < here && inside) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + 512U * (q % SLOTS)), "l"(column + (size_t)pos * dim) : "memory");
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll
+            for (int q = 0; q < U; ++q) fetch(q);
+#pragma unroll 1
+            for (int q = 0; q < here; ++q) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(U - 1) : "memory");
+                const vec row = *reinterpret_cast<const vec *>(ring[warp] + 512 * (q % SLOTS) + 16 * lane);
+                add_row(q, &row);
+                fetch(q + U);   // (to the place that was read one row ago)
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        } else {
+            for (int q = 0; q < here; q += U) {
+                vec v[U][NV];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const T *row = g + (size_t)__shfl_sync(0xffffffffU, mine, (q + u) & 31) * dim + col0;
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        if (q + u < here && col0 + (lane + 32 * j) * VE < dim) v[u][j] = *reinterpret_cast<const vec *>(row + (lane + 32 * j) * VE);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (q + u < here) add_row(q + u, v[u]);
+                }
             }
         }
+    }
+    __syncwarp();
+    const bool goes_on = some && after == current;
+    if (lane == 0) {
+        first_token[warp] = begin;
+        ends[warp] = some ? (token_before == begin ? 1U : 0U) | (goes_on ? 2U : 0U) | (token_before == begin && after == begin ? 4U : 0U) : 8U;
+    }
+    if (some) {
+        if (goes_on && !open_left) keep(tail(warp)); else finish();
     }
     __syncthreads();
     // runs that cross the warps of the block, a thread per column, warps in order
@@ -323,7 +384,7 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
             }
             if (!(f & 4U)) {
                 from_before = false;
-                if (f & 2U) sum = tail[k][c];
+                if (f & 2U) sum = tail(k)[c];
             }
         }
         if (open) partial[((size_t)blockIdx.x * 2U + (from_before ? 0U : 1U)) * dim + col0 + c] = sum;
@@ -334,18 +395,17 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
 // columns at a time.
 template <typename T>
 __global__ void __launch_bounds__(256)
-es_merge_kernel(const float *__restrict__ partial, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table, unsigned piece, size_t dim,
-                float scale, bool add)
+es_merge_kernel(const float *__restrict__ partial, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table, unsigned n, unsigned piece,
+                size_t dim, float scale, bool add)
 {
     gdb_pdl_sync();
     __shared__ float sh[8][128];
-    const unsigned total = count[0], c = blockIdx.x, e0 = c * piece, e1 = e0 + piece;
-    if (e1 >= total) return;
-    const int k = token[e1];
-    if (token[e1 - 1] != k || (e0 > 0U && token[e0 - 1] == k)) return;   // complete, or begun earlier
-    // last piece whose first entry has this token
-    unsigned lo = c + 1U, hi = (total - 1U) / piece;
-    if (lo < hi && token[(size_t)(lo + 1U) * piece] != k) hi = lo;       // (most runs end in the next piece)
+    const unsigned c = blockIdx.x, e0 = c * piece, e1 = e0 + piece, e2 = e1 + piece;   // (e1 < n)
+    const int k = __ldg(&token[e1]), last = __ldg(&token[e1 - 1]), before = e0 > 0U ? __ldg(&token[e0 - 1]) : -1, next = e2 < n && e2 > e1 ? __ldg(&token[e2]) : -1;
+    const unsigned total = count[0];
+    if (e1 >= total || last != k || before == k) return;   // nothing behind this piece, complete, or begun earlier
+    // last piece whose first entry has this token (most runs end in the next one)
+    unsigned lo = c + 1U, hi = e2 < total && next == k ? (total - 1U) / piece : lo;
     while (lo < hi) {
         const unsigned mid = (lo + hi + 1U) / 2U;
         if (token[(size_t)mid * piece] == k) lo = mid; else hi = mid - 1U;
@@ -387,16 +447,17 @@ gd_status lookup(gd_backend *be, const void *table, const int *ids, void *out, c
 }
 
 template <typename T, int VE, int NV>
-gd_status reduce(gd_backend *be, const void *g, const unsigned *order, const int *token, const unsigned *count, void *table, float *partial, unsigned piece, unsigned pieces,
-                 size_t dim, float scale, bool add)
+gd_status reduce(gd_backend *be, const void *g, const unsigned *order, const int *token, const unsigned *count, void *table, float *partial, unsigned n, unsigned piece,
+                 unsigned pieces, size_t dim, float scale, bool add)
 {
     const size_t slabs = (dim + 32U * VE * NV - 1U) / (32U * VE * NV);
     if (slabs > 65535U) return GD_ERR_UNSUPPORTED;
-    gdb_launch(es_reduce_kernel<T, VE, NV>, dim3(pieces, (unsigned)slabs), ES_WARPS * 32, 0, be->stream, (const T *)g, order, token, count, (T *)table, partial, piece, dim, scale, add);
+    gdb_launch(es_reduce_kernel<T, VE, NV>, dim3(pieces, (unsigned)slabs), ES_WARPS * 32, 0, be->stream, (const T *)g, order, token, count, (T *)table, partial, n, piece, dim, scale,
+               add);
     gd_status st = gdb_launched(be, "embedding_sorted_backward sums");
     if (st != GD_OK || pieces == 1U) return st;
     const size_t col_blocks = (dim + 127U) / 128U;
-    gdb_launch(es_merge_kernel<T>, dim3(pieces - 1U, (unsigned)(col_blocks < 4U ? col_blocks : 4U)), 256, 0, be->stream, (const float *)partial, token, count, (T *)table, piece, dim,
+    gdb_launch(es_merge_kernel<T>, dim3(pieces - 1U, (unsigned)(col_blocks < 4U ? col_blocks : 4U)), 256, 0, be->stream, (const float *)partial, token, count, (T *)table, n, piece, dim,
                scale, add);
     return gdb_launched(be, "embedding_sorted_backward merge");
 }
@@ -417,9 +478,11 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     unsigned *count = reinterpret_cast<unsigned *>(be->ws + 2U * list);
     float *partial = reinterpret_cast<float *>(be->ws + 2U * list + 256U);
     const size_t fit = (be->ws_bytes - 2U * list - 256U) / (2U * dim * sizeof(float));
-    // entries of a warp: 32, fewer while the blocks would not fill the GPU twice, more where the partial sums would not fit the workspace
-    size_t per = 32U;
-    while (per > 8U && ((size_t)n + per * ES_WARPS - 1U) / (per * ES_WARPS) * slabs < 2U * (size_t)be->sm_count) per /= 2U;
+    // entries of a warp: what gives every place on the GPU one block, 8 at least (rows on their way); more where the partial sums would not
+    // fit the workspace
+    size_t per = ((size_t)n * slabs + (size_t)be->sm_count * ES_BLOCKS * ES_WARPS - 1U) / ((size_t)be->sm_count * ES_BLOCKS * ES_WARPS);
+    if (per < 8U) per = 8U;
+    if (per > 4096U) per = 4096U;
     while (((size_t)n + per * ES_WARPS - 1U) / (per * ES_WARPS) > fit) per *= 2U;
     const size_t piece = per * ES_WARPS, pieces = ((size_t)n + piece - 1U) / piece;
     // a slice of the vocabulary per block, two blocks' worth of SMs at most where the counters allow it
@@ -427,25 +490,27 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     if (width > ES_MAX_WIDTH) width = ES_MAX_WIDTH;
     const unsigned slices = (vocab + width - 1U) / width;
     // (more than half of an SM's shared memory: blocks that start while the preceding kernel drains would pair up on the SMs it left first)
-    int smem = (int)(width * ES_SORT_WARPS * sizeof(unsigned));
+    const unsigned range = ((n + ES_SORT_WARPS * 32U - 1U) / (ES_SORT_WARPS * 32U)) * 32U, room = (unsigned)((ES_SORT_SMEM - width * ES_SORT_WARPS * 4U) / (ES_SORT_WARPS * 8U));
+    const unsigned notes = range < room ? range : room;
+    int smem = (int)((width * 4U + notes * 8U) * ES_SORT_WARPS);
     if (smem < 116 * 1024) smem = 116 * 1024;
     static bool ready = false;
     if (!ready) {
-        const int most = (int)(ES_MAX_WIDTH * ES_SORT_WARPS * sizeof(unsigned));
+        const int most = (int)ES_SORT_SMEM;
         cudaError_t e = cudaFuncSetAttribute(es_sort_kernel<uint4>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(es_sort_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return gdb_fail(be, e, "embedding_sorted_backward smem attribute");
         ready = true;
     }
     if (vec) {
-        gdb_launch(es_sort_kernel<uint4>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, order, token, count, add ? (uint4 *)nullptr : (uint4 *)table, row_bytes / 16U);
+        gdb_launch(es_sort_kernel<uint4>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, notes, order, token, count, add ? (uint4 *)nullptr : (uint4 *)table, row_bytes / 16U);
     } else {
-        gdb_launch(es_sort_kernel<T>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, order, token, count, add ? (T *)nullptr : (T *)table, dim);
+        gdb_launch(es_sort_kernel<T>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, notes, order, token, count, add ? (T *)nullptr : (T *)table, dim);
     }
     gd_status st = gdb_launched(be, "embedding_sorted_backward sort");
     if (st != GD_OK) return st;
-    return vec ? reduce<T, VE, 1>(be, g, order, token, count, table, partial, (unsigned)piece, (unsigned)pieces, dim, scale, add)
-               : reduce<T, 1, 8>(be, g, order, token, count, table, partial, (unsigned)piece, (unsigned)pieces, dim, scale, add);
+    return vec ? reduce<T, VE, 1>(be, g, order, token, count, table, partial, n, (unsigned)piece, (unsigned)pieces, dim, scale, add)
+               : reduce<T, 1, 8>(be, g, order, token, count, table, partial, n, (unsigned)piece, (unsigned)pieces, dim, scale, add);
 }
 
 bool es_args_ok(const gd_backend_tensor_view *rows, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *table, const gd_backend_embedding_args *a)

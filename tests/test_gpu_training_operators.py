@@ -251,6 +251,19 @@ def test_embedding_sorted_backward_large_vocabulary(step):
     within(emb_backward(step, g, ids, vocab, F16, 1.0), want, F16, slack, "d_table")
 
 
+@pytest.mark.parametrize("n,vocab,kind", [(80000, 300, "half"), (80000, 5, "one"), (70001, 40000, "half")])
+def test_embedding_sorted_backward_frequent_tokens(step, n, vocab, kind):
+    """More ids of one slice in a warp's range than it can note, beside other tokens of the slice; rows of zeros next to them."""
+    dim = 8
+    rng = np.random.default_rng(n)
+    ids = emb_ids(kind, n, vocab, rng).astype(np.int32)
+    g = rnd_np(rng.standard_normal((n, dim)).astype(np.float32), F32)
+    want, slack = emb_reference(g, ids, vocab, 1.0)
+    got = emb_backward(step, g, ids, vocab, F32, 1.0)
+    within(got, want, F32, slack, "d_table")
+    np.testing.assert_array_equal(got, emb_backward(step, g, ids, vocab, F32, 1.0))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=ids_of)
 @pytest.mark.parametrize("n,vocab,dim", [(1, 1, 1), (3, 9, 5), (64, 2048, 512), (130, 77, 96), (33, 50, 2048), (1000, 10, 8), (7, 20, 4099)])
 def test_embedding_scaled_forward(step, dtype, n, vocab, dim):
