@@ -15,6 +15,8 @@
 // Every sum is FP32 in an order that depends on the ids alone.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int ES_SORT_WARPS = 32, ES_AHEAD = 8;   // (ids on their way, a lane)
@@ -29,16 +31,40 @@ template <> struct __align__(16) es_vec<__nv_bfloat16, 8> { __nv_bfloat16 v[8]; 
 template <> struct __align__(16) es_vec<float, 4> { float v[4]; };
 
 // ------------------------------------------------------------------ forward
-// LANES threads per row, ROWS rows each in flight.
-template <typename T, int VE, int LANES>
+// round(scale * v) of the elements of 16 bytes, two 16-bit ones at a time, or of one element
+template <typename T>
+__device__ __forceinline__ uint4 es_scaled(uint4 v, float scale)
+{
+    unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4U) {
+            w[k] = __float_as_uint(__uint_as_float(w[k]) * scale);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+            *reinterpret_cast<__half2 *>(&w[k]) = __floats2half2_rn(f.x * scale, f.y * scale);
+        } else {
+            *reinterpret_cast<__nv_bfloat162 *>(&w[k]) = __floats2bfloat162_rn(__uint_as_float(w[k] << 16) * scale, __uint_as_float(w[k] & 0xffff0000U) * scale);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ T es_scaled(T v, float scale)
+{
+    T r;
+    gdb_io<T>::st(&r, 0, gdb_io<T>::ld(&v, 0) * scale);
+    return r;
+}
+
+// LANES threads per row, ROWS rows each in flight; V: uint4 where rows are whole 16-byte vectors, else T.
+template <typename T, typename V, int LANES>
 __global__ void __launch_bounds__(256)
-es_lookup_kernel(const T *__restrict__ table, const int *__restrict__ ids, T *__restrict__ out, size_t n, size_t vocab, size_t dim, float scale)
+es_lookup_kernel(const V *__restrict__ table, const int *__restrict__ ids, V *__restrict__ out, size_t n, size_t vocab, size_t vecs, float scale)
 {
     gdb_pdl_sync();
     constexpr int ROWS = 4, PER = 256 / LANES;
-    typedef es_vec<T, VE> vec;
     const unsigned t = threadIdx.x % LANES, r = threadIdx.x / LANES;
-    const size_t vecs = dim / VE;
     for (size_t first = (size_t)blockIdx.x * PER * ROWS; first < n; first += (size_t)gridDim.x * PER * ROWS) {
         int id[ROWS];
 #pragma unroll
@@ -47,19 +73,16 @@ es_lookup_kernel(const T *__restrict__ table, const int *__restrict__ ids, T *__
             id[u] = row < n ? __ldg(&ids[row]) : -1;
         }
         for (size_t v = t; v < vecs; v += LANES) {
-            vec a[ROWS];
+            V a[ROWS];
 #pragma unroll
             for (int u = 0; u < ROWS; ++u) {
-                if (id[u] >= 0 && (size_t)id[u] < vocab) a[u] = *reinterpret_cast<const vec *>(table + (size_t)id[u] * dim + v * VE);
+                if (id[u] >= 0 && (size_t)id[u] < vocab) a[u] = __ldg(table + (size_t)id[u] * vecs + v); else a[u] = V{};
             }
 #pragma unroll
             for (int u = 0; u < ROWS; ++u) {
                 const size_t row = first + u * PER + r;
-                if (row >= n) continue;
                 const bool in = id[u] >= 0 && (size_t)id[u] < vocab;
-#pragma unroll
-                for (int e = 0; e < VE; ++e) gdb_io<T>::st(a[u].v, e, in ? gdb_io<T>::ld(a[u].v, e) * scale : __int_as_float(0x7fc00000));
-                *reinterpret_cast<vec *>(out + row * dim + v * VE) = a[u];
+                if (row < n) out[row * vecs + v] = es_scaled<T>(a[u], in ? scale : __int_as_float(0x7fc00000));   // (a row of NaN)
             }
         }
     }
@@ -434,13 +457,13 @@ es_merge_kernel(const float *__restrict__ partial, const int *__restrict__ token
     }
 }
 
-template <typename T, int VE>
+template <typename T, typename V>
 gd_status lookup(gd_backend *be, const void *table, const int *ids, void *out, const gd_backend_embedding_args *a, float scale)
 {
-    const size_t vecs = a->dim / VE;
+    const size_t vecs = a->dim / (sizeof(V) / sizeof(T));
 #define GO(LANES)                                                                                                                                             \
-    gdb_launch(es_lookup_kernel<T, VE, LANES>, gdb_grid_for((a->ids_count + 4U * (256 / LANES) - 1U) / (4U * (256 / LANES)), 1U, be, 32U), 256, 0, be->stream, \
-               (const T *)table, ids, (T *)out, a->ids_count, a->vocab, a->dim, scale)
+    gdb_launch(es_lookup_kernel<T, V, LANES>, gdb_grid_for((a->ids_count + 4U * (256 / LANES) - 1U) / (4U * (256 / LANES)), 1U, be, 32U), 256, 0, be->stream, \
+               (const V *)table, ids, (V *)out, a->ids_count, a->vocab, vecs, scale)
     if (vecs <= 16U) GO(16); else if (vecs <= 32U) GO(32); else if (vecs <= 64U) GO(64); else if (vecs <= 128U) GO(128); else GO(256);
 #undef GO
     return gdb_launched(be, "embedding_scaled_forward");
@@ -544,9 +567,9 @@ gd_status gdb200_embedding_scaled_forward(gd_backend *be, const gd_backend_tenso
         return GD_OK;
     }
     const bool vec = args->dim % (16U / gdb_dtype_size(dt)) == 0U && (((uintptr_t)tp | (uintptr_t)op) % 16U) == 0U;
-    if (dt == GDB_DTYPE_F16) return vec ? lookup<__half, 8>(be, tp, ip, op, args, scale) : lookup<__half, 1>(be, tp, ip, op, args, scale);
-    if (dt == GDB_DTYPE_BF16) return vec ? lookup<__nv_bfloat16, 8>(be, tp, ip, op, args, scale) : lookup<__nv_bfloat16, 1>(be, tp, ip, op, args, scale);
-    return vec ? lookup<float, 4>(be, tp, ip, op, args, scale) : lookup<float, 1>(be, tp, ip, op, args, scale);
+    if (dt == GDB_DTYPE_F16) return vec ? lookup<__half, uint4>(be, tp, ip, op, args, scale) : lookup<__half, __half>(be, tp, ip, op, args, scale);
+    if (dt == GDB_DTYPE_BF16) return vec ? lookup<__nv_bfloat16, uint4>(be, tp, ip, op, args, scale) : lookup<__nv_bfloat16, __nv_bfloat16>(be, tp, ip, op, args, scale);
+    return vec ? lookup<float, uint4>(be, tp, ip, op, args, scale) : lookup<float, float>(be, tp, ip, op, args, scale);
 }
 
 gd_status gdb200_embedding_sorted_backward(gd_backend *be, const gd_backend_tensor_view *grad_out, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *grad_table,
