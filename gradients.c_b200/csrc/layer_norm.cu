@@ -192,31 +192,65 @@ __device__ __forceinline__ void ln_forward_row(ln_pairs<T, VE, TPR, EPT> &f, con
     for (int k = 0; k < EPT / 2; ++k) f.v[k] = f2_fma(f2_mul(f.v[k], inv2), wf.v[k], bf.v[k]);
     f.store(po, t, cols);
 }
+constexpr int LN_AHEAD = 3;                      // rows of a group on their way
+__host__ __device__ constexpr int ln_fwd_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+// (blocks on an SM, as the registers allow)
+__host__ __device__ constexpr int ln_fwd_blocks(int tpr, int ve) { return tpr > 256 ? 1 : (ve > 1 ? 3 : 2); }
+template <typename T, int VE> __host__ __device__ constexpr size_t ln_fwd_smem(int tpr) { return VE > 1 ? (size_t)LN_AHEAD * (LN_EPT / VE) * ln_fwd_threads(tpr) * 16U : 0U; }
 template <typename T, int TPR, int VE>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+__global__ void __launch_bounds__(ln_fwd_threads(TPR), ln_fwd_blocks(TPR, VE))
 layer_norm_fwd_kernel(const T *x, const T *__restrict__ w, const T *__restrict__ b, T *out, float2 *__restrict__ stats, size_t rows, unsigned cols, float eps)
 {
     gdb_pdl_sync();
-    constexpr int THREADS = TPR > 256 ? TPR : 256;
+    constexpr int THREADS = ln_fwd_threads(TPR), PIECES = LN_EPT / VE;
     constexpr unsigned TOGETHER = TPR < 32 ? 32 / TPR : 1;   // groups of a warp: they take the same number of turns
     __shared__ float2 sh[64];
+    extern __shared__ uint4 ahead[];     // [LN_AHEAD, PIECES, THREADS]: a thread copies and reads its own places only
     const unsigned t = threadIdx.x % TPR, group = threadIdx.x / TPR, mine = group % TOGETHER;
     const size_t stride = (size_t)gridDim.x * (THREADS / TPR);
     typedef ln_pairs<T, VE, TPR> pairs;
     size_t first = (size_t)blockIdx.x * (THREADS / TPR) + group - mine;
     typename pairs::raw next;
-    next.load(x + (first + mine < rows ? first + mine : 0) * cols, t, cols);
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(ahead + threadIdx.x);
+    const auto fetch = [&](size_t row, unsigned slot) {
+        const T *p = x + row * cols;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const unsigned c = (t + j * TPR) * VE, bytes = pairs::inside(j) || c < cols ? 16U : 0U;   // (the rest of the 16 bytes is zeros)
+            if (row < rows) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + (slot * PIECES + j) * (THREADS * 16U)), "l"(bytes != 0U ? p + c : p), "r"(bytes) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (VE > 1) {
+#pragma unroll
+        for (unsigned k = 0; k < LN_AHEAD; ++k) fetch(first + mine + k * stride, k);
+    } else {
+        next.load(x + (first + mine < rows ? first + mine : 0) * cols, t, cols);
+    }
     pairs wf, bf;
     if (w != nullptr) wf.load(w, t, cols); else wf.fill(1.0f);
     if (b != nullptr) bf.load(b, t, cols); else bf.fill(0.0f);
     const float inv_cols = 1.0f / (float)cols;
+    unsigned slot = 0;
     for (; first < rows; first += stride) {
         const size_t row = first + mine;
         pairs f;
+        if constexpr (VE > 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LN_AHEAD - 1) : "memory");
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) next.v[j] = ahead[(slot * PIECES + j) * THREADS + threadIdx.x];
+        }
         f.take(next);
-        if (first + stride < rows) next.load(x + (row + stride < rows ? row + stride : 0) * cols, t, cols);
+        if constexpr (VE == 1) {
+            if (first + stride < rows) next.load(x + (row + stride < rows ? row + stride : 0) * cols, t, cols);
+        }
         ln_forward_row(f, wf, bf, out + row * cols, stats == nullptr ? nullptr : stats + row, row < rows, t, cols, inv_cols, eps, sh);
+        if constexpr (VE > 1) {
+            fetch(row + LN_AHEAD * stride, slot);   // (the row that lay there is in registers and behind two exchanges)
+            slot = slot + 1U < LN_AHEAD ? slot + 1U : 0U;
+        }
     }
+    if constexpr (VE > 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // Rows of more than LN_MAX_COLS elements: a block per row that reads x three times (the second and third time from L2).
@@ -417,14 +451,20 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
     ln_sums<EPT> sums2;
     const float inv_cols = 1.0f / (float)cols;
     unsigned flip = 0;
+    float2 ahead[2];   // statistics of the group's next two rows
+    auto look_ahead = [&](size_t row) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) ahead[k] = row + k * GROUPS < a.rows ? __ldg(&a.stats[row + k * GROUPS]) : make_float2(0.0f, 0.0f);
+    };
+    if (BWD) look_ahead((size_t)blockIdx.x * a.tile_rows + group);
     // rows of a tile (or, behind the last full one, of memory), two at a time backward: first row, rows there are
     auto work = [&](size_t row0, unsigned here, const T *px, const T *pg, const T *pd, T *po) {
         if (BWD) {
             for (unsigned r = group; r < a.tile_rows; r += 2U * GROUPS) {
                 const bool live[2] = {r < here, r + GROUPS < here};
-                float2 st[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                if (live[0]) st[0] = __ldg(&a.stats[row0 + r]);
-                if (live[1]) st[1] = __ldg(&a.stats[row0 + r + GROUPS]);
+                const float2 st[2] = {ahead[0], ahead[1]};
+                const bool more = r + 2U * GROUPS < a.tile_rows;
+                look_ahead(more ? row0 + r + 2U * GROUPS : row0 + (size_t)gridDim.x * a.tile_rows + group);
                 const size_t at = (size_t)r * cols;
                 ln_backward_rows<T, VE, TPR, EPT, 2>(px + at, pg + at, pd + at, po == nullptr ? nullptr : po + at, (size_t)GROUPS * cols, live, BWD == 2, st, wf, sums2, inv_cols, t,
                                                      cols, sh, flip);
@@ -692,9 +732,16 @@ gd_status stream_typed(gd_backend *be, const ln_call &a, float *partial, unsigne
 template <typename T, int TPR, int VE>
 gd_status fwd_go(gd_backend *be, const ln_call &a)
 {
-    constexpr unsigned THREADS = TPR > 256 ? TPR : 256, PER = THREADS / TPR;
-    gdb_launch(layer_norm_fwd_kernel<T, TPR, VE>, gdb_grid_for(a.rows, PER, be, 1024U / THREADS), THREADS, 0, be->stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.out, a.stats, a.rows,
-               (unsigned)a.cols, a.eps);
+    constexpr unsigned THREADS = ln_fwd_threads(TPR), PER = THREADS / TPR;
+    constexpr size_t smem = ln_fwd_smem<T, VE>(TPR);
+    static bool ready = false;
+    if (!ready) {
+        const cudaError_t e = cudaFuncSetAttribute(layer_norm_fwd_kernel<T, TPR, VE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return gdb_fail(be, e, "layer_norm_forward smem attribute");
+        ready = true;
+    }
+    gdb_launch(layer_norm_fwd_kernel<T, TPR, VE>, gdb_grid_for(a.rows, PER, be, ln_fwd_blocks(TPR, VE)), THREADS, smem, be->stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.out,
+               a.stats, a.rows, (unsigned)a.cols, a.eps);
     return gdb_launched(be, "layer_norm_forward");
 }
 
