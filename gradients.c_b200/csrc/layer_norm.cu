@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(LN_THREADS, 1)
 layer_norm_stream_kernel(const ln_stream a, int *err_flag)
 {
     constexpr int GROUPS = LN_THREADS / TPR, STREAMS = BWD + 1;
+    constexpr bool DIRECT = VE > 1;   // whole vectors are stored by the threads themselves
     extern __shared__ __align__(128) unsigned char ring[];   // [stages][streams][tile_bytes], rounded up to 128
     __shared__ __align__(8) uint64_t bars[LN_MAX_STAGES];
     __shared__ unsigned arrived[LN_MAX_STAGES];   // warps that are done with the stage's tile
@@ -495,7 +496,7 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         __syncwarp();
         T *sx = reinterpret_cast<T *>(ring + s * stage_bytes), *sg = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD >= 1 ? slot_bytes : 0U)),
           *sd = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD == 2 ? 2U * slot_bytes : 0U));
-        work(row0, here, sx, sg, sd, out == nullptr ? nullptr : sx);
+        work(row0, here, sx, sg, sd, out == nullptr ? nullptr : (DIRECT ? out + row0 * cols : sx));
         // the warp that finishes the tile sends it off and fetches the next one for its stage
         fence_proxy_async_smem();
         __syncwarp();
@@ -504,8 +505,10 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
             if (atomicAdd(&arrived[s], 1U) == LN_WARPS - 1U) {
                 arrived[s] = 0U;
                 __threadfence_block();
-                send(tile, s);
-                bulk_wait_group_read<0>();
+                if (!DIRECT) {
+                    send(tile, s);
+                    bulk_wait_group_read<0>();
+                }
                 fetch(tile + (size_t)stages * gridDim.x, s);
             }
         }
@@ -514,7 +517,7 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
             ph ^= 1U;
         }
     }
-    if ((threadIdx.x & 31) == 0) bulk_wait_all();
+    if (!DIRECT && (threadIdx.x & 31) == 0) bulk_wait_all();
     if (BWD && a.partial != nullptr) {
         // the groups' sums through the ring (64 KB), added in order
         __syncthreads();
