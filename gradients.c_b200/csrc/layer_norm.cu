@@ -371,10 +371,12 @@ __device__ __forceinline__ void ln_backward_rows(const T *px, const T *pg, const
 
 // ---- rows streamed through shared memory: as many bytes on their way as HBM wants, whatever the registers hold ----
 // One block per SM walks over tiles of R rows. Bulk copies bring them into a ring, 16 warps work on them, a group of TPR threads per row as
-// in the kernel above, and write the result over the input, bulk copies take it away. Tiles begin on 16 bytes whatever the width is (R is
-// chosen so), so odd rows stream as even ones do: only the reads from shared memory are narrower. A last tile whose bytes are no
-// multiple of 16 is worked on in global memory. The warp that finishes a tile issues the copies (warps for that alone would leave 96
-// registers a thread for sums that need 110; one fixed warp among the 16 is waited for by all).
+// in the kernel above, and store the result themselves (written into the ring and copied away from there, a stage came free later:
+// backward 18432 x 512 FP16 15.2 instead of 13.6 us, 16384 x 2048 BF16 44.0 instead of 41.0, 4099 x 1003 FP32 12.6 instead of 11.8).
+// Tiles begin on 16 bytes whatever the width is (R is chosen so), so odd rows stream as even ones do: only the reads from shared memory
+// are narrower. A last tile whose bytes are no multiple of 16 is worked on in global memory. The warp that finishes a tile issues the next
+// copies into its stage (warps for that alone would leave 96 registers a thread for sums that need 110; one fixed warp among the 16 is
+// waited for by all).
 constexpr int LN_WARPS = 16, LN_THREADS = LN_WARPS * 32, LN_MAX_STAGES = 8;
 constexpr size_t LN_RING_BYTES = 208U * 1024U;
 
@@ -394,7 +396,6 @@ __global__ void __launch_bounds__(LN_THREADS, 1)
 layer_norm_stream_kernel(const ln_stream a, int *err_flag)
 {
     constexpr int GROUPS = LN_THREADS / TPR, STREAMS = BWD + 1;
-    constexpr bool DIRECT = VE > 1;   // whole vectors are stored by the threads themselves
     extern __shared__ __align__(128) unsigned char ring[];   // [stages][streams][tile_bytes], rounded up to 128
     __shared__ __align__(8) uint64_t bars[LN_MAX_STAGES];
     __shared__ unsigned arrived[LN_MAX_STAGES];   // warps that are done with the stage's tile
@@ -433,14 +434,6 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         copy(0, x + at);
         if (BWD >= 1) copy(1, g + at);
         if (BWD == 2) copy(2, out + at);
-    };
-    auto send = [&](size_t tile, unsigned s) {
-        if (out != nullptr) {
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + tile * a.tile_rows * cols), "r"(smem_u32(ring + s * stage_bytes)),
-                         "r"(bulk_bytes(tile))
-                         : "memory");
-        }
-        bulk_commit_group();
     };
     if (threadIdx.x == 0) {
         for (unsigned k = 0; k < stages; ++k) fetch(blockIdx.x + (size_t)k * gridDim.x, k);
@@ -496,8 +489,8 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
         __syncwarp();
         T *sx = reinterpret_cast<T *>(ring + s * stage_bytes), *sg = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD >= 1 ? slot_bytes : 0U)),
           *sd = reinterpret_cast<T *>(ring + s * stage_bytes + (BWD == 2 ? 2U * slot_bytes : 0U));
-        work(row0, here, sx, sg, sd, out == nullptr ? nullptr : (DIRECT ? out + row0 * cols : sx));
-        // the warp that finishes the tile sends it off and fetches the next one for its stage
+        work(row0, here, sx, sg, sd, out == nullptr ? nullptr : out + row0 * cols);
+        // the warp that finishes the tile fetches the next one for its stage
         fence_proxy_async_smem();
         __syncwarp();
         if ((threadIdx.x & 31) == 0) {
@@ -505,10 +498,6 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
             if (atomicAdd(&arrived[s], 1U) == LN_WARPS - 1U) {
                 arrived[s] = 0U;
                 __threadfence_block();
-                if (!DIRECT) {
-                    send(tile, s);
-                    bulk_wait_group_read<0>();
-                }
                 fetch(tile + (size_t)stages * gridDim.x, s);
             }
         }
@@ -517,7 +506,6 @@ layer_norm_stream_kernel(const ln_stream a, int *err_flag)
             ph ^= 1U;
         }
     }
-    if (!DIRECT && (threadIdx.x & 31) == 0) bulk_wait_all();
     if (BWD && a.partial != nullptr) {
         // the groups' sums through the ring (64 KB), added in order
         __syncthreads();
@@ -674,7 +662,7 @@ bool ln_tiles(const gd_backend *be, const ln_call &a, int streams, ln_stream *st
 {
     if (a.cols > (size_t)TPR * EPT) return false;
     constexpr unsigned GROUPS = LN_THREADS / TPR;
-    if (((uintptr_t)a.x | (uintptr_t)a.g | (uintptr_t)(streams == 1 ? a.out : a.dx)) % 16U != 0U) return false;
+    if (((uintptr_t)a.x | (uintptr_t)a.g | (uintptr_t)a.dx) % 16U != 0U) return false;
     size_t r = GROUPS;
     // backward takes two rows of a group at a time; with the old gradient as a third stream the tiles stay the same, and with them the
     // order of the weight's and the bias's sums
