@@ -7,7 +7,7 @@
 // matrices with a few strong directions), sums FP32. The iterate is carried as the sum of two FP16 numbers, X = hi + lo: the product
 // takes hi, the linear term a X takes both. With hi alone the rounding of the strong directions, spread over all directions and
 // amplified a-fold per step as the weak ones are, is 0.8 % of the result for strong directions 20 times the others (3 % for 200
-// times), with the pair 0.02-0.2 %. X is kept times 2^10, which takes its elements (about 1 / sqrt(rows * cols)) out of the range
+// times), with the pair 0.02-0.2 %; where small matrices leave the time, A, P and the operand X are pairs too. X is kept times 2^10, which takes its elements (about 1 / sqrt(rows * cols)) out of the range
 // where FP16 loses bits.
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -127,16 +127,25 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
 // either order of the product's operands does.
 enum { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
 
+// Smaller sides up to which an FP16 result gets its full precision: operands as sums of two FP16 numbers, hi hi + hi lo + lo hi of three
+// products in one accumulator. Rounded to one FP16 number each, A and P cost the result up to 2e-3 in the 2-norm where its singular values
+// are close together (rounding errors of the diagonals add up), 3e-4 where a few stand out; with three products what is left is the
+// result's own rounding, 2e-4. Time of a call, one product and three: 129 x 140 55 and 86 us, 129 x 1000 72 and 118, 300 x 300 69 and 123,
+// 400 x 420 80 and 141: small matrices wait for launches more than for products. Larger ones would pay three times the products and keep
+// one; so do BF16 results, whose rounding is 1.7e-3 (but where one launch does all, below, three take 6 us more of 25 to 60).
+constexpr uint64_t NS_FINE = 448;
+
 struct ns_maps {
-    CUtensorMap a, b;        // operands
+    CUtensorMap a, b, a_lo, b_lo;   // operands
 };
 // What the epilogue reads and writes, [batch, M, pitch] with rows of a multiple of 32 bytes (LAST's output: dense, any alignment).
 struct ns_shape {
     uint32_t M, N, K, tiles_m, tiles_n, batch, pitch;
+    uint32_t parts;          // of a product: 1: hi hi; 3: hi hi + hi lo + lo hi, and A and P have low halves too
     float alpha, beta;
-    const __half *in;        // POLY: A; UPDATE, LAST: hi
-    __half *lo;              // UPDATE: in and out; LAST: in
-    void *out;               // A, P, the next hi, or the caller's tensor
+    const __half *in, *in_lo;   // POLY: A; UPDATE, LAST: X
+    void *out;               // A, P, the next X, or the caller's tensor
+    __half *out_lo;
     bool wide_out;           // LAST: the caller's rows take 32-byte stores
 };
 
@@ -179,6 +188,13 @@ __device__ __forceinline__ void ns_store_row(void *base, const uint32_t *w, uint
         }
     }
 }
+// two numbers as sums of two FP16 ones each
+__device__ __forceinline__ void ns_split2(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    hi = half_pack<__half>::pack(a, b);
+    const float2 r = ns_two(hi);
+    lo = half_pack<__half>::pack(a - r.x, b - r.y);
+}
 // the inputs of a piece, on their way while its products are formed
 template <int MODE, int COLS>
 __device__ __forceinline__ void ns_load_piece(ns_row<COLS> &in, ns_row<COLS> &lo, const ns_shape &sh, uint32_t row, uint32_t col0, uint32_t z)
@@ -187,7 +203,20 @@ __device__ __forceinline__ void ns_load_piece(ns_row<COLS> &in, ns_row<COLS> &lo
     const uint32_t left = row < sh.M && col0 < sh.N ? sh.N - col0 : 0U;
     const size_t at = ((size_t)z * sh.M + (left != 0U ? row : 0U)) * sh.pitch + (left != 0U ? col0 : 0U);
     ns_load_row(in, sh.in + at, left);
-    if (MODE != NS_POLY) ns_load_row(lo, sh.lo + at, left);
+    if (MODE != NS_POLY || sh.parts > 1U) ns_load_row(lo, sh.in_lo + at, left);
+}
+// the transposed piece: row e of it are the lanes' elements e
+__device__ __forceinline__ void ns_store_mirrored(__half *out, const uint32_t *v, const ns_shape &sh, uint32_t row0, uint32_t col0, uint32_t z, unsigned char *stage, int lane)
+{
+#pragma unroll
+    for (int e = 0; e < NS_PIECE; ++e) *reinterpret_cast<unsigned short *>(stage + e * NS_STAGE_ROW + lane * 2) = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+    __syncwarp();
+    uint32_t w[NS_PIECE / 2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(w + 4 * j) = *reinterpret_cast<const uint4 *>(stage + lane * NS_STAGE_ROW + j * 16);
+    const uint32_t row = col0 + lane, left = row < sh.M && row0 < sh.N ? sh.N - row0 : 0U;
+    ns_store_row<NS_PIECE>(out + ((size_t)z * sh.M + row) * sh.pitch + row0, w, left);
+    __syncwarp();
 }
 // v: the piece's accumulators. `stage` (this warp's): where a piece is transposed, or rows that take no 32-byte stores are put together.
 template <int MODE, typename TOUT, int COLS>
@@ -203,7 +232,7 @@ __device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row
         float f0 = sh.alpha * __uint_as_float(v[2 * e]), f1 = sh.alpha * __uint_as_float(v[2 * e + 1]);
         if (MODE != NS_GRAM) {
             float2 a = ns_two(in.w[e]);
-            if (MODE != NS_POLY) {
+            if (MODE != NS_POLY || sh.parts > 1U) {
                 const float2 l = ns_two(lo.w[e]);
                 a.x += l.x;
                 a.y += l.y;
@@ -214,11 +243,7 @@ __device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row
         if (MODE == NS_LAST) {
             v[e] = half_pack<TOUT>::pack(f0 * NS_DOWN, f1 * NS_DOWN);
         } else {
-            v[e] = half_pack<__half>::pack(f0, f1);
-            if (MODE == NS_UPDATE) {
-                const float2 r = ns_two(v[e]);
-                lo.w[e] = half_pack<__half>::pack(f0 - r.x, f1 - r.y);
-            }
+            if (MODE == NS_UPDATE || sh.parts > 1U) ns_split2(f0, f1, v[e], lo.w[e]); else v[e] = half_pack<__half>::pack(f0, f1);
         }
     }
     if (MODE == NS_LAST) {
@@ -247,26 +272,17 @@ __device__ __forceinline__ void ns_finish_piece(const ns_shape &sh, const ns_row
     }
     __half *out = reinterpret_cast<__half *>(sh.out);
     ns_store_row<COLS>(out + at, v, left);
-    if (MODE == NS_UPDATE) {
-        ns_store_row<COLS>(sh.lo + at, lo.w, left);
-    } else if (COLS == NS_PIECE && mirror) {
-        // the transposed piece: row e of it are the lanes' elements e
-#pragma unroll
-        for (int e = 0; e < NS_PIECE; ++e) *reinterpret_cast<unsigned short *>(stage + e * NS_STAGE_ROW + lane * 2) = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint4 t = *reinterpret_cast<const uint4 *>(stage + lane * NS_STAGE_ROW + j * 16);
-            v[4 * j] = t.x;
-            v[4 * j + 1] = t.y;
-            v[4 * j + 2] = t.z;
-            v[4 * j + 3] = t.w;
+    if (MODE == NS_UPDATE || sh.parts > 1U) ns_store_row<COLS>(sh.out_lo + at, lo.w, left);
+    if constexpr (MODE != NS_UPDATE && COLS == NS_PIECE) {
+        if (mirror) {
+            ns_store_mirrored(out, v, sh, row0, col0, z, stage, lane);
+            if (sh.parts > 1U) ns_store_mirrored(sh.out_lo, lo.w, sh, row0, col0, z, stage, lane);
         }
-        const uint32_t row_t = col0 + lane, left_t = row_t < sh.M && row0 < sh.N ? sh.N - row0 : 0U;
-        ns_store_row<COLS>(out + ((size_t)z * sh.M + row_t) * sh.pitch + row0, v, left_t);
-        __syncwarp();
     }
 }
+
+// which of a product's parts a k step belongs to
+__device__ __forceinline__ uint32_t ns_part(uint32_t it, uint32_t part_iters) { return (it >= part_iters ? 1U : 0U) + (it >= 2U * part_iters ? 1U : 0U); }
 
 // ---- one CTA, one tile of 128 x BN: small matrices, where the number of SMs at work counts ----
 // SPLIT: two CTAs of a cluster take half of the contraction each and send each other the sums of half of the tile's columns (GRAM of long
@@ -307,22 +323,26 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
         tm = blockIdx.x / sh.tiles_n;
         tn = blockIdx.x - tm * sh.tiles_n;
     }
-    const uint32_t rank = SPLIT ? cluster_ctarank() : 0U, all_iters = (sh.K + BK - 1) / BK;
+    const uint32_t rank = SPLIT ? cluster_ctarank() : 0U, part_iters = (sh.K + BK - 1) / BK, all_iters = part_iters * sh.parts;
     const uint32_t first = rank * ((all_iters + 1U) / 2U), n_iters = SPLIT ? (rank == 0U ? (all_iters + 1U) / 2U : all_iters - first) : all_iters;
     const uint32_t m0 = tm * BM, n0 = tn * BN;
     const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[STAGES]), accum_bar = smem_u32(&bars[2 * STAGES]);
     auto load_a = [&](uint32_t it) {
-        const uint32_t s = it % STAGES, dst = smem_u32(smem + s * plan::STAGE_BYTES), bar = full0 + 8 * s;
+        const uint32_t s = it % STAGES, dst = smem_u32(smem + s * plan::STAGE_BYTES), bar = full0 + 8 * s, p = ns_part(first + it, part_iters);
+        const CUtensorMap *map = p == 2U ? &maps.a_lo : &maps.a;
+        const int k0 = (int)((first + it - p * part_iters) * BK);
         if (A_MN) {
-            tma_load_3d(dst, &maps.a, (int)m0, (int)((first + it) * BK), (int)z, bar);
-            tma_load_3d(dst + BK * 128, &maps.a, (int)m0 + 64, (int)((first + it) * BK), (int)z, bar);
+            tma_load_3d(dst, map, (int)m0, k0, (int)z, bar);
+            tma_load_3d(dst + BK * 128, map, (int)m0 + 64, k0, (int)z, bar);
         } else {
-            tma_load_3d(dst, &maps.a, (int)((first + it) * BK), (int)m0, (int)z, bar);
+            tma_load_3d(dst, map, k0, (int)m0, (int)z, bar);
         }
     };
     auto load_b = [&](uint32_t it) {
-        const uint32_t s = it % STAGES, dst = smem_u32(smem + s * plan::STAGE_BYTES) + BM * BK * 2, bar = full0 + 8 * s;
-        if (B_MN) tma_load_3d(dst, &maps.b, (int)n0, (int)((first + it) * BK), (int)z, bar); else tma_load_3d(dst, &maps.b, (int)((first + it) * BK), (int)n0, (int)z, bar);
+        const uint32_t s = it % STAGES, dst = smem_u32(smem + s * plan::STAGE_BYTES) + BM * BK * 2, bar = full0 + 8 * s, p = ns_part(first + it, part_iters);
+        const CUtensorMap *map = p == 1U ? &maps.b_lo : &maps.b;
+        const int k0 = (int)((first + it - p * part_iters) * BK);
+        if (B_MN) tma_load_3d(dst, map, (int)n0, k0, (int)z, bar); else tma_load_3d(dst, map, k0, (int)n0, (int)z, bar);
     };
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2 * STAGES + 1; ++s) mbar_init(full0 + 8 * s, 1);
@@ -453,7 +473,7 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * NS2_STAGES + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
-    const uint32_t n_iters = (sh.K + BK - 1) / BK;
+    const uint32_t part_iters = (sh.K + BK - 1) / BK, n_iters = part_iters * sh.parts;
     const uint32_t per = SYM ? sh.tiles_n * (sh.tiles_n + 1U) / 2U : sh.tiles_m * sh.tiles_n, units = per * sh.batch;
     auto tile_of = [&](uint32_t u, uint32_t &z, uint32_t &tm, uint32_t &tn) {
         z = u / per;
@@ -501,18 +521,20 @@ ns_pair_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *err
                     }
                     if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * NS2_STAGE_BYTES);
                     const uint32_t a_dst = smem_u32(smem + s * NS2_STAGE_BYTES), b_dst = a_dst + BM * BK * 2, bar = full_leader + 8 * s;
-                    const int k0 = (int)(kb * BK);
+                    const uint32_t p = ns_part(kb, part_iters);
+                    const CUtensorMap *a = p == 2U ? &maps.a_lo : &maps.a, *b = p == 1U ? &maps.b_lo : &maps.b;
+                    const int k0 = (int)((kb - p * part_iters) * BK);
                     if (A_MN) {
-                        tma_load_3d_pair(a_dst, &maps.a, am, k0, (int)z, bar);
-                        tma_load_3d_pair(a_dst + BK * 128, &maps.a, am + 64, k0, (int)z, bar);
+                        tma_load_3d_pair(a_dst, a, am, k0, (int)z, bar);
+                        tma_load_3d_pair(a_dst + BK * 128, a, am + 64, k0, (int)z, bar);
                     } else {
-                        tma_load_3d_pair(a_dst, &maps.a, k0, am, (int)z, bar);
+                        tma_load_3d_pair(a_dst, a, k0, am, (int)z, bar);
                     }
                     if (B_MN) {
-                        tma_load_3d_pair(b_dst, &maps.b, bn, k0, (int)z, bar);
-                        tma_load_3d_pair(b_dst + BK * 128, &maps.b, bn + 64, k0, (int)z, bar);
+                        tma_load_3d_pair(b_dst, b, bn, k0, (int)z, bar);
+                        tma_load_3d_pair(b_dst + BK * 128, b, bn + 64, k0, (int)z, bar);
                     } else {
-                        tma_load_3d_pair(b_dst, &maps.b, k0, bn, (int)z, bar);
+                        tma_load_3d_pair(b_dst, b, k0, bn, (int)z, bar);
                     }
                 }
             }
@@ -608,22 +630,28 @@ bool ns_map(CUtensorMap *m, uint32_t dtype, const void *base, uint64_t batch, ui
 }
 
 struct ns_tensor {       // a matrix of the scratch, as an operand and in the epilogue
-    __half *p;
+    __half *p, *lo;
     uint64_t rows, cols, pitch;
 };
-bool ns_operand(CUtensorMap *m, const ns_tensor &t, uint64_t batch, bool mn, uint32_t tile)
+bool ns_operand(CUtensorMap *m, const ns_tensor &t, const __half *p, uint64_t batch, bool mn, uint32_t tile)
 {
-    return mn ? ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, BK, 64, true) : ns_map(m, GDB_DTYPE_F16, t.p, batch, t.rows, t.cols, t.pitch, tile, BK, true);
+    return mn ? ns_map(m, GDB_DTYPE_F16, p, batch, t.rows, t.cols, t.pitch, BK, 64, true) : ns_map(m, GDB_DTYPE_F16, p, batch, t.rows, t.cols, t.pitch, tile, BK, true);
 }
+// the maps of a product that comes again every step (or every second one), kept for the call
+struct ns_memo {
+    ns_maps maps;
+    bool ready;
+};
 
 // ---- matrices whose smaller side is at most 128: all steps in one launch, a cluster of up to 16 CTAs per matrix ----
-// A and P are one tile. Each CTA keeps up to 256 columns of X (rows for a tall matrix: X is taken transposed then) in shared memory, both
+// A and P are one tile. Each CTA keeps up to 192 columns of X (rows for a tall matrix: X is taken transposed then) in shared memory, both
 // halves, and forms its part of A; the parts are added over distributed shared memory (every CTA a share of the rows, then the sum to
 // all), P is formed by every CTA for itself, and the CTA's columns are updated in place. Two exchanges a step in place of three launches
 // that would each occupy a handful of SMs: 17 launches take the host 57 us alone.
-constexpr int NT_M = 128, NT_W = 256, NT_THREADS = 512, NT_WARPS = NT_THREADS / 32, NT_MAX_CTAS = 16;
-constexpr int NT_X_BYTES = NT_M * NT_W * 2, NT_A_BYTES = NT_M * NT_M * 2, NT_PARTS = NT_M * NT_M * 4;
-constexpr int NT_SMEM = 2 * NT_X_BYTES + NT_A_BYTES + NT_PARTS + 512 + 1024;
+constexpr int NT_M = 128, NT_W = 192, NT_W_ALONE = 256, NT_THREADS = 512, NT_WARPS = NT_THREADS / 32, NT_MAX_CTAS = 16;
+constexpr int NT_X_BYTES = NT_M * NT_W * 2, NT_X_BYTES_ALONE = NT_M * NT_W_ALONE * 2, NT_A_BYTES = NT_M * NT_M * 2, NT_PARTS = NT_M * NT_M * 4;
+constexpr int NT_SMEM = 2 * NT_X_BYTES + 2 * NT_A_BYTES + NT_PARTS + 512 + 1024;   // (one alone has no parts)
+static_assert(2 * NT_X_BYTES_ALONE <= 2 * NT_X_BYTES + NT_PARTS, "room for the columns of one CTA");
 
 // element (row, col) of a tile of 128 rows in blocks of 64 columns, 128-byte swizzle: the 16 bytes that hold columns 8 * octet ...
 __device__ __forceinline__ uint32_t nt_at(uint32_t row, uint32_t octet) { return (octet >> 3) * (NT_M * 128U) + row * 128U + (((octet & 7U) ^ (row & 7U)) << 4); }
@@ -636,12 +664,13 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
     gdb_pdl_sync();
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023U) & ~(uintptr_t)1023U);
-    unsigned char *xh = smem, *xl = xh + NT_X_BYTES, *sa = xl + NT_X_BYTES, *parts = sa + NT_A_BYTES;   // hi, lo, A (then P), parts of A
+    const uint32_t rank = cluster_ctarank(), ctas = gridDim.x, z = blockIdx.y;   // (one cluster per matrix: grid.x is its size)
+    unsigned char *sa = smem, *sl = sa + NT_A_BYTES, *xh = sl + NT_A_BYTES, *xl = xh + (ctas == 1U ? NT_X_BYTES_ALONE : NT_X_BYTES),   // A (then P) and X, hi and lo each
+                  *parts = smem + 2 * NT_A_BYTES + 2 * NT_X_BYTES;                                                                         // parts of A
     double *sums = reinterpret_cast<double *>(parts + NT_PARTS);                                        // [CTAs], then the warps' sums
     uint64_t *bar = reinterpret_cast<uint64_t *>(sums + NT_MAX_CTAS + NT_WARPS);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + 3);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank(), ctas = gridDim.x, z = blockIdx.y;   // (one cluster per matrix: grid.x is its size)
     const bool tall = rows > cols;
     const uint32_t m = tall ? cols : rows, n = tall ? rows : cols;
     const uint32_t width = ((n + ctas - 1U) / ctas + 63U) & ~63U, j0 = rank * width;   // columns of X here (multiples of 64)
@@ -717,19 +746,23 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
     constexpr float DOWN2 = NS_DOWN * NS_DOWN;
     uint32_t phase = 0;
     bool ok = true;
-    // the products of a phase, by one thread, and the wait for them by all
-    auto products = [&](uint32_t d, uint32_t a, uint32_t b, bool b_mn, uint32_t n_cols, uint32_t blocks, uint32_t block_bytes) {
+    // the products of a phase, hi hi + hi lo + lo hi, by one thread, and the wait for them by all
+    auto products = [&](uint32_t d, const unsigned char *a_hi, const unsigned char *a_lo, const unsigned char *b_hi, const unsigned char *b_lo, bool b_mn, uint32_t n_cols,
+                        uint32_t blocks, uint32_t block_bytes) {
         nt_fence();
         tcgen05_fence_before();
         __syncthreads();
         if (threadIdx.x == 0) {
             tcgen05_fence_after();
             const uint32_t idesc = (1U << 4) | ((b_mn ? 1U : 0U) << 16) | ((n_cols >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-            for (uint32_t k = 0; k < blocks; ++k) {
-                for (uint32_t kk = 0; kk < BK / UMMA_K; ++kk) {
-                    const uint64_t ad = make_smem_desc(a + k * (NT_M * 128U) + kk * 32, 16, 1024);
-                    const uint64_t bd = b_mn ? make_smem_desc(b + k * block_bytes + kk * 2048, NT_M * 128U, 1024) : make_smem_desc(b + k * block_bytes + kk * 32, 16, 1024);
-                    tcgen05_mma_f16(d, ad, bd, idesc, (k != 0 || kk != 0) ? 1U : 0U);
+            for (uint32_t q = 0; q < 3U; ++q) {
+                const uint32_t a = smem_u32(q == 2U ? a_lo : a_hi), b = smem_u32(q == 1U ? b_lo : b_hi);
+                for (uint32_t k = 0; k < blocks; ++k) {
+                    for (uint32_t kk = 0; kk < BK / UMMA_K; ++kk) {
+                        const uint64_t ad = make_smem_desc(a + k * (NT_M * 128U) + kk * 32, 16, 1024);
+                        const uint64_t bd = b_mn ? make_smem_desc(b + k * block_bytes + kk * 2048, NT_M * 128U, 1024) : make_smem_desc(b + k * block_bytes + kk * 32, 16, 1024);
+                        tcgen05_mma_f16(d, ad, bd, idesc, (q != 0 || k != 0 || kk != 0) ? 1U : 0U);
+                    }
                 }
             }
             tcgen05_commit(done);
@@ -744,15 +777,15 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
     };
     for (uint32_t step = 0; step < steps; ++step) {
         // this CTA's part of A = X X^T
-        products(tmem + 256U, smem_u32(xh), smem_u32(xh), false, NT_M, width / BK, NT_M * 128U);
+        products(tmem + 256U, xh, xl, xh, xl, false, NT_M, width / BK, NT_M * 128U);
         uint32_t v[32];
         tmem_ld_32x32b_x32(tmem + tlane + 256U + part * 32, v);
         if (ctas > 1U) {
-            // Sent with their completion counted at the receiver, 64 KB of parts and 32 KB of sums a step. Nobody is overrun: parts
+            // Sent with their completion counted at the receiver, 64 KB of parts and as many of sums a step. Nobody is overrun: parts
             // of the next step are sent by those who have all of this step's sums, sums by those who have all parts.
             if (threadIdx.x == 0) {
                 mbar_expect_tx(got_parts, NT_PARTS);
-                mbar_expect_tx(got_sum, NT_A_BYTES);
+                mbar_expect_tx(got_sum, 2 * NT_A_BYTES);
             }
             const uint32_t to = mapa_shared(smem_u32(parts) + (rank * share + row % share) * 512U, row / share), to_bar = mapa_shared(got_parts, row / share);
 #pragma unroll
@@ -777,12 +810,16 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
                     s.z += p.z;
                     s.w += p.w;
                 }
-                const uint32_t w0 = half_pack<__half>::pack(s.x * DOWN2, s.y * DOWN2), w1 = half_pack<__half>::pack(s.z * DOWN2, s.w * DOWN2);
+                uint32_t w[4];   // hi, hi, lo, lo
+                ns_split2(s.x * DOWN2, s.y * DOWN2, w[0], w[2]);
+                ns_split2(s.z * DOWN2, s.w * DOWN2, w[1], w[3]);
                 const uint32_t at = smem_u32(sa) + nt_at(to_row, c4 >> 1) + (c4 & 1U) * 8U;
                 for (uint32_t k = 0; k < ctas; ++k) {
                     const uint32_t dst = (rank + k) % ctas;
-                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(mapa_shared(at, dst)), "r"(w0), "r"(w1),
-                                 "r"(mapa_shared(got_sum, dst))
+                    const uint32_t to_sum = mapa_shared(at, dst), to_bar = mapa_shared(got_sum, dst);
+                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to_sum), "r"(w[0]), "r"(w[1]), "r"(to_bar) : "memory");
+                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to_sum + (uint32_t)NT_A_BYTES), "r"(w[2]), "r"(w[3]),
+                                 "r"(to_bar)
                                  : "memory");
                 }
             }
@@ -794,30 +831,32 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                uint32_t w[4];
+                uint32_t w[4], l[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = half_pack<__half>::pack(__uint_as_float(v[8 * k + 2 * e]) * DOWN2, __uint_as_float(v[8 * k + 2 * e + 1]) * DOWN2);
+                for (int e = 0; e < 4; ++e) ns_split2(__uint_as_float(v[8 * k + 2 * e]) * DOWN2, __uint_as_float(v[8 * k + 2 * e + 1]) * DOWN2, w[e], l[e]);
                 *reinterpret_cast<uint4 *>(sa + nt_at(row, part * 4 + k)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4 *>(sl + nt_at(row, part * 4 + k)) = make_uint4(l[0], l[1], l[2], l[3]);
             }
         }
         // P = b A + c A A in the place of A (which is symmetric: rows serve as columns). The other CTAs write the next A there only after
         // this one has sent its next part, behind the products that read P.
-        products(tmem + 384U, smem_u32(sa), smem_u32(sa), false, NT_M, 2U, NT_M * 128U);
+        products(tmem + 384U, sa, sl, sa, sl, false, NT_M, 2U, NT_M * 128U);
         tmem_ld_32x32b_x32(tmem + tlane + 384U + part * 32, v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint32_t at = nt_at(row, part * 4 + k);
-            const uint4 a = *reinterpret_cast<const uint4 *>(sa + at);
-            uint32_t w[4];
+            const uint4 a = *reinterpret_cast<const uint4 *>(sa + at), b = *reinterpret_cast<const uint4 *>(sl + at);
+            uint32_t w[4], l[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 f = ns_two((&a.x)[e]);
-                w[e] = half_pack<__half>::pack(fmaf(cb, f.x, cc * __uint_as_float(v[8 * k + 2 * e])), fmaf(cb, f.y, cc * __uint_as_float(v[8 * k + 2 * e + 1])));
+                const float2 f = ns_two((&a.x)[e]), r = ns_two((&b.x)[e]);
+                ns_split2(fmaf(cb, f.x + r.x, cc * __uint_as_float(v[8 * k + 2 * e])), fmaf(cb, f.y + r.y, cc * __uint_as_float(v[8 * k + 2 * e + 1])), w[e], l[e]);
             }
             *reinterpret_cast<uint4 *>(sa + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(sl + at) = make_uint4(l[0], l[1], l[2], l[3]);
         }
         // X <- a X + P X, this CTA's columns
-        products(tmem, smem_u32(sa), smem_u32(xh), true, width, 2U, BK * 128U);
+        products(tmem, sa, sl, xh, xl, true, width, 2U, BK * 128U);
         const bool last = step + 1U == steps;
         const f32x2 ca2 = f2_make(ca, ca);
 #pragma unroll 1
@@ -836,10 +875,7 @@ ns_tile_kernel(const T *__restrict__ g, TOUT *out, uint32_t rows, uint32_t cols,
                     if (last) {
                         (&nh.x)[e] = half_pack<TOUT>::pack(f0 * NS_DOWN, f1 * NS_DOWN);
                     } else {
-                        const uint32_t p = half_pack<__half>::pack(f0, f1);
-                        const float2 r = ns_two(p);
-                        (&nh.x)[e] = p;
-                        (&nl.x)[e] = half_pack<__half>::pack(f0 - r.x, f1 - r.y);
+                        ns_split2(f0, f1, (&nh.x)[e], (&nl.x)[e]);
                     }
                 }
                 *reinterpret_cast<uint4 *>(xh + at) = nh;
@@ -888,7 +924,9 @@ gd_status ns_launch_tile(gd_backend *be, const void *g, void *out, const gdb200_
     }
     const uint64_t n = std::max(a->rows, a->cols);
     unsigned ctas = 1;
-    while (ctas * NT_W < n) ctas *= 2U;
+    if (n > NT_W_ALONE) {
+        while (ctas * NT_W < n) ctas *= 2U;
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -973,7 +1011,7 @@ gd_status ns_launch_pair(gd_backend *be, const ns_maps &maps, const ns_shape &sh
 
 // One product of a step: operands xa and xb; sh has what the epilogue needs.
 template <bool A_MN, bool B_MN, int MODE, typename TOUT = __half>
-gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, ns_shape sh)
+gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, ns_shape sh, ns_memo *memo)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
     const uint64_t sms = (uint64_t)be->sm_count, clusters = sms / 2U;
@@ -992,7 +1030,7 @@ gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, n
     // k step of 64 and round of tiles (the operands' way into shared memory), and what a further round adds where one CTA per SM starts
     // anew. One call on a 512 x 512, 1024 x 1024, 2048 x 2048 matrix: pair 182, 221, 322 us, 128 x 64 tiles 91, 134, 411 us, 128 x 32
     // tiles 83, 123, 413 us.
-    const uint32_t wide = singles(64), narrow = B_MN ? 0U : singles(32), iters = (sh.K + BK - 1U) / BK;
+    const uint32_t wide = singles(64), narrow = B_MN ? 0U : singles(32), iters = (sh.K + BK - 1U) / BK * sh.parts;
     auto cost = [&](uint64_t fixed, uint64_t again, uint64_t step, uint64_t tiles, uint64_t places, uint64_t its) {
         const uint64_t rounds = (tiles + places - 1U) / places;
         return fixed + again * (rounds - 1U) + step * its * rounds;
@@ -1005,8 +1043,13 @@ gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, n
     const uint32_t bn = pair ? 256U : (slim ? 32U : 64U);
     sh.tiles_m = pair ? p_m : s_m;
     sh.tiles_n = (sh.N + bn - 1U) / bn;
-    ns_maps maps;
-    if (!ns_operand(&maps.a, xa, sh.batch, A_MN, 128) || !ns_operand(&maps.b, xb, sh.batch, B_MN, pair ? 128 : bn)) return GD_ERR_UNSUPPORTED;
+    ns_maps &maps = memo->maps;   // (UPDATE's and LAST's tiles are the same)
+    if (!memo->ready) {
+        const uint32_t box = pair ? 128U : bn;
+        if (!ns_operand(&maps.a, xa, xa.p, sh.batch, A_MN, 128) || !ns_operand(&maps.b, xb, xb.p, sh.batch, B_MN, box)) return GD_ERR_UNSUPPORTED;
+        if (sh.parts > 1U && (!ns_operand(&maps.a_lo, xa, xa.lo, sh.batch, A_MN, 128) || !ns_operand(&maps.b_lo, xb, xb.lo, sh.batch, B_MN, box))) return GD_ERR_UNSUPPORTED;
+        memo->ready = true;
+    }
     if (pair) return ns_launch_pair<A_MN, B_MN, MODE, TOUT>(be, maps, sh, pairs);
     if constexpr (!B_MN) {
         if (slim) return ns_launch_single<A_MN, B_MN, MODE, TOUT, 32>(be, maps, sh, narrow);
@@ -1017,10 +1060,11 @@ gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, n
     return ns_launch_single<A_MN, B_MN, MODE, TOUT, 64>(be, maps, sh, wide);
 }
 
-// Where the parts of the scratch lie: the iterate's high halves (two, used in turn), its low halves, A, P, the sums of squares.
+// Where the parts of the scratch lie: the iterate's high halves (two, used in turn), its low halves, A's and P's, the sums of squares.
 struct ns_layout {
     size_t small, pitch, small_pitch;
-    size_t hi[2], lo, gram, poly, norm, total;
+    uint32_t parts;
+    size_t hi[2], lo[2], gram, gram_lo, poly, poly_lo, norm, total;
 };
 bool ns_plan(const gdb200_orthogonalize_args *a, ns_layout *l)
 {
@@ -1031,13 +1075,23 @@ bool ns_plan(const gdb200_orthogonalize_args *a, ns_layout *l)
     // (the products count tiles of a batch in 32 bits)
     if ((a->rows / 128U + 1U) * (a->cols / 64U + 1U) * (a->batch + 1U) > 0x7fffffffU) return false;
     const size_t x = (a->batch * a->rows * l->pitch * 2U + 255U) & ~(size_t)255U, s = (a->batch * l->small * l->small_pitch * 2U + 255U) & ~(size_t)255U;
-    l->hi[0] = 0U;
-    l->hi[1] = x;
-    l->lo = 2U * x;
-    l->gram = 3U * x;
-    l->poly = 3U * x + s;
-    l->norm = 3U * x + 2U * s;
-    l->total = l->norm + a->batch * NS_NORM_BLOCKS * sizeof(double);
+    l->parts = l->small <= NS_FINE ? 3U : 1U;
+    const size_t s_lo = l->parts > 1U ? s : 0U;
+    size_t at = 0U;
+    const auto next = [&](size_t *where, size_t bytes) {
+        *where = at;
+        at += bytes;
+    };
+    next(&l->hi[0], x);
+    next(&l->hi[1], x);
+    next(&l->lo[0], x);
+    if (l->parts > 1U) next(&l->lo[1], x); else l->lo[1] = l->lo[0];   // (an operand of other CTAs' products too, or read and written in place)
+    next(&l->gram, s);
+    next(&l->gram_lo, s_lo);
+    next(&l->poly, s);
+    next(&l->poly_lo, s_lo);
+    next(&l->norm, a->batch * NS_NORM_BLOCKS * sizeof(double));
+    l->total = at;
     return true;
 }
 
@@ -1095,29 +1149,36 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
         return half_out ? ns_launch_tile<float, __half>(be, xp, op, a) : ns_launch_tile<float, __nv_bfloat16>(be, xp, op, a);
     }
     const bool tall = rows > cols;
-    const ns_tensor hi[2] = {{(__half *)(sp + l.hi[0]), rows, cols, l.pitch}, {(__half *)(sp + l.hi[1]), rows, cols, l.pitch}};
-    const ns_tensor lo = {(__half *)(sp + l.lo), rows, cols, l.pitch}, gram = {(__half *)(sp + l.gram), m, m, l.small_pitch}, poly = {(__half *)(sp + l.poly), m, m, l.small_pitch};
+    const auto half_at = [&](size_t at) { return (__half *)(sp + at); };
+    const ns_tensor xs[2] = {{half_at(l.hi[0]), half_at(l.lo[0]), rows, cols, l.pitch}, {half_at(l.hi[1]), half_at(l.lo[1]), rows, cols, l.pitch}};
+    const ns_tensor gram = {half_at(l.gram), half_at(l.gram_lo), m, m, l.small_pitch}, poly = {half_at(l.poly), half_at(l.poly_lo), m, m, l.small_pitch};
+    ns_memo grams[2], polys, updates[2];
+    for (ns_memo *p : {&grams[0], &grams[1], &polys, &updates[0], &updates[1]}) p->ready = false;
     double *norm = (double *)(sp + l.norm);
-    gd_status st = x->dtype == GDB_DTYPE_F16    ? first_iterate<__half>(be, xp, norm, hi[0].p, lo.p, a, l.pitch)
-                   : x->dtype == GDB_DTYPE_BF16 ? first_iterate<__nv_bfloat16>(be, xp, norm, hi[0].p, lo.p, a, l.pitch)
-                                                : first_iterate<float>(be, xp, norm, hi[0].p, lo.p, a, l.pitch);
+    gd_status st = x->dtype == GDB_DTYPE_F16    ? first_iterate<__half>(be, xp, norm, xs[0].p, xs[0].lo, a, l.pitch)
+                   : x->dtype == GDB_DTYPE_BF16 ? first_iterate<__nv_bfloat16>(be, xp, norm, xs[0].p, xs[0].lo, a, l.pitch)
+                                                : first_iterate<float>(be, xp, norm, xs[0].p, xs[0].lo, a, l.pitch);
     for (uint32_t k = 0; k < a->steps && st == GD_OK; ++k) {
-        const ns_tensor &x0 = hi[k & 1U], &x1 = hi[(k & 1U) ^ 1U];
+        const ns_tensor &x0 = xs[k & 1U], &x1 = xs[(k & 1U) ^ 1U];
         ns_shape square = {};
+        square.parts = out->dtype == GDB_DTYPE_F16 ? l.parts : 1U;
         square.M = square.N = (uint32_t)m;
         square.K = (uint32_t)(tall ? rows : cols);
         square.batch = (uint32_t)a->batch;
         square.alpha = NS_DOWN * NS_DOWN;
         square.pitch = (uint32_t)l.small_pitch;
         square.out = gram.p;
-        st = tall ? ns_product<true, true, NS_GRAM>(be, x0, x0, square) : ns_product<false, false, NS_GRAM>(be, x0, x0, square);
+        square.out_lo = gram.lo;
+        st = tall ? ns_product<true, true, NS_GRAM>(be, x0, x0, square, &grams[k & 1U]) : ns_product<false, false, NS_GRAM>(be, x0, x0, square, &grams[k & 1U]);
         if (st != GD_OK) break;
         square.K = (uint32_t)m;
         square.alpha = a->c;
         square.beta = a->b;
         square.in = gram.p;
+        square.in_lo = gram.lo;
         square.out = poly.p;
-        st = ns_product<false, false, NS_POLY>(be, gram, gram, square);
+        square.out_lo = poly.lo;
+        st = ns_product<false, false, NS_POLY>(be, gram, gram, square, &polys);
         if (st != GD_OK) break;
         ns_shape full = square;
         full.M = (uint32_t)rows;
@@ -1126,15 +1187,16 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
         full.alpha = 1.0f;
         full.beta = a->a;
         full.in = x0.p;
-        full.lo = lo.p;
+        full.in_lo = x0.lo;
         if (k + 1U < a->steps) {
             full.out = x1.p;
-            st = tall ? ns_product<false, false, NS_UPDATE>(be, x0, poly, full) : ns_product<false, true, NS_UPDATE>(be, poly, x0, full);
+            full.out_lo = x1.lo;
+            st = tall ? ns_product<false, false, NS_UPDATE>(be, x0, poly, full, &updates[k & 1U]) : ns_product<false, true, NS_UPDATE>(be, poly, x0, full, &updates[k & 1U]);
         } else {
             full.out = op;
             full.wide_out = cols % 16U == 0U && (uintptr_t)op % 32U == 0U;
-            if (out->dtype == GDB_DTYPE_F16) st = tall ? ns_product<false, false, NS_LAST, __half>(be, x0, poly, full) : ns_product<false, true, NS_LAST, __half>(be, poly, x0, full);
-            else st = tall ? ns_product<false, false, NS_LAST, __nv_bfloat16>(be, x0, poly, full) : ns_product<false, true, NS_LAST, __nv_bfloat16>(be, poly, x0, full);
+            if (out->dtype == GDB_DTYPE_F16) st = tall ? ns_product<false, false, NS_LAST, __half>(be, x0, poly, full, &updates[k & 1U]) : ns_product<false, true, NS_LAST, __half>(be, poly, x0, full, &updates[k & 1U]);
+            else st = tall ? ns_product<false, false, NS_LAST, __nv_bfloat16>(be, x0, poly, full, &updates[k & 1U]) : ns_product<false, true, NS_LAST, __nv_bfloat16>(be, poly, x0, full, &updates[k & 1U]);
         }
     }
     return st;

@@ -354,6 +354,18 @@ def test_orthogonalize(step, batch, rows, cols, kind):
         ns_check(ns_call(step, g, dtype, out_dtype), ns_reference(g, 5, 1e-7), out_dtype, g=g)
 
 
+@pytest.mark.parametrize("kind", ["noise", "strong"])
+@pytest.mark.parametrize("batch,rows,cols", [(2, 16, 300), (1, 64, 64), (3, 128, 256), (2, 1000, 100), (1, 64, 4000), (2, 129, 140), (1, 300, 1000), (2, 1003, 257), (1, 448, 448), (40, 260, 300)])
+def test_orthogonalize_small_sides_keep_fp16_precision(step, batch, rows, cols, kind):
+    """Where the smaller side is at most 448, an FP16 result is off by its rounding (U) and little else: operands are sums of two FP16 numbers,
+    2^-21 off with the product of the two low halves left out, three operands in each of five steps; near their limit an iterate's errors
+    grow by at most a^2 + ... < 64 on the way to the result. One FP16 number an operand gives 1e-3 to 2e-3 on noise."""
+    g = ns_matrix(batch, rows, cols, kind, rows + cols).astype(np.float32)
+    got, want = ns_call(step, g, F32, F16), ns_reference(g, 5, 1e-7)
+    for k in range(batch):
+        assert np.linalg.norm(got[k] - want[k]) <= (U[F16] + 15 * 64 * 2.0 ** -21) * np.linalg.norm(want[k]), k
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 8])
 def test_orthogonalize_steps_and_other_coefficients(step, steps):
     g = ns_matrix(2, 100, 180, "noise", 6).astype(np.float32)
