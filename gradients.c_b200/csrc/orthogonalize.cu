@@ -132,7 +132,7 @@ enum { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
 // are close together (rounding errors of the diagonals add up), 3e-4 where a few stand out; with three products what is left is the
 // result's own rounding, 2e-4. Time of a call, one product and three: 129 x 140 55 and 86 us, 129 x 1000 72 and 118, 300 x 300 69 and 123,
 // 400 x 420 80 and 141: small matrices wait for launches more than for products. Larger ones would pay three times the products and keep
-// one; so do BF16 results, whose rounding is 1.7e-3 (but where one launch does all, below, three take 6 us more of 25 to 60).
+// one; so do BF16 results, whose rounding is 1.7e-3 (but where one launch does all, below, three take 6 to 13 us more of 25 to 60).
 constexpr uint64_t NS_FINE = 448;
 
 struct ns_maps {

@@ -570,9 +570,10 @@ gd_status gdb200_embedding_sorted_backward(gd_backend *backend, const gd_backend
  * AdamW only, src/optim/adamw.c): X = x / (|x|_F + eps), then `steps` times A = X X^T (on the smaller side), X <- a X + (b A + c A^2) X,
  * out = X. x F16, BF16 or F32, out F16 or BF16. The products' operands are FP16 numbers with FP32 sums: sums of two each where the
  * smaller side is at most 128, and up to 448 for an F16 out (the result is then off by its own rounding), one each elsewhere (off by up to
- * 0.2 % in the 2-norm, 0.03 % where a few singular values stand out); the iterate is always carried in two. out may be x. The iterates have to stay below 64 in magnitude, as they do
- * for coefficients whose polynomial maps [0, 1.3] into itself. A matrix of zeros gives zeros (eps > 0). `scratch`: U8, 256-byte aligned, of
- * gdb200_orthogonalize_scratch_bytes(args) bytes (0: a shape that is not taken), not to be shared with a call on another stream. */
+ * 0.2 % in the 2-norm, 0.03 % where a few singular values stand out); the iterate is always carried in two. out may be x (the same
+ * tensor). The iterates have to stay below 64 in magnitude, as they do for coefficients whose polynomial maps [0, 1.3] into itself. A
+ * matrix of zeros gives zeros (eps > 0). `scratch`: U8, 256-byte aligned, of gdb200_orthogonalize_scratch_bytes(args) bytes (0: a shape
+ * that is not taken), not to be shared with a call on another stream. */
 typedef struct gdb200_orthogonalize_args {
     uint64_t batch, rows, cols;
     uint32_t steps;
