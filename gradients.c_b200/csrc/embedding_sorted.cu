@@ -9,10 +9,12 @@
 // 1. es_sort_kernel: a stable counting sort of the positions in one launch without communication between blocks. A block owns a slice
 //    of the vocabulary and reads ALL ids (they lie in L2: 4 bytes each against 2 dim for the gradient's row), so it knows by itself how
 //    many ids lie below its slice. It also clears the rows of its slice that no id names.
-// 2. es_reduce_kernel: equal pieces of the sorted list, whatever the frequencies: a warp adds a few dozen rows for 32 vectors of
+// 2. es_reduce_kernel: equal pieces of the sorted list, whatever the frequencies: a warp adds a few rows up to a few dozen for 32 vectors of
 //    columns, runs that begin and end within a piece are written, the others go to FP32 partial sums.
 // 3. es_merge_kernel: adds the partial sums of the runs that cross pieces, in order.
-// Every sum is FP32 in an order that depends on the ids alone.
+// Every sum is FP32 in an order that depends on the ids, the sizes and the number of SMs alone.
+// 16384 ids, 32768 x 2048 BF16: lookup 19.5 us (6.2 TB/s), 1. 23.5 (14 of them clear 80 MB), 2. 24 (5 TB/s), 3. 5.5; 18432 ids, 2048 x 512 FP16:
+// 6, 9, 8, 5.5, where the launches count.
 #include "common.cuh"
 
 #include <type_traits>

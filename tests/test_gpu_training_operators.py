@@ -157,6 +157,23 @@ def test_layer_norm_views_at_odd_offsets_and_in_place(step):
     assert (around[:3] == 7.0).all() and (around[3 + rows * cols:] == 7.0).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(5, 40), (5, 41), (6000, 512), (4801, 515), (7, 9000)])
+def test_layer_norm_backward_over_the_upstream_gradient_and_without_an_input_gradient(step, rows, cols):
+    """grad_x in grad_out's place gives the same three gradients; accumulating without a grad_x is not accumulating."""
+    ctx = step
+    x, w, b, g = ln_data(rows, cols, F32, rows)
+    want = ln_call(ctx, x, w, b, g, F32)
+    xt, wt, gt, stats = dev(ctx, x, F32), dev(ctx, w, F32), dev(ctx, g, F32), ctx.scratch_empty(F32, (rows, 2))
+    out, dw, db = ctx.scratch_empty(F32, (rows, cols)), ctx.scratch_empty(F32, (cols,)), ctx.scratch_empty(F32, (cols,))
+    args = byref(abi.LayerNormArgs(rows, cols, 1e-5, 0))
+    ctx.check(ctx.lib.gdb200_layer_norm_forward(ctx.backend, xt.ref(), wt.ref(), None, out.ref(), stats.ref(), args), "forward")
+    for grad_x, accumulate in ((None, 1), (gt.ref(), 0)):
+        ctx.check(ctx.lib.gdb200_layer_norm_backward(ctx.backend, xt.ref(), wt.ref(), stats.ref(), gt.ref(), grad_x, accumulate, dw.ref(), db.ref(), args), "backward")
+        np.testing.assert_array_equal(host(dw), want["dw"].reshape(-1))
+        np.testing.assert_array_equal(host(db), want["db"].reshape(-1))
+        np.testing.assert_array_equal(host(gt), g if grad_x is None else want["dx"])
+
+
 def test_layer_norm_empty_and_repeatable(step):
     ctx = step
     x, w, b, g = ln_data(5000, 512, BF16, 2)
@@ -262,6 +279,18 @@ def test_embedding_sorted_backward_frequent_tokens(step, n, vocab, kind):
     got = emb_backward(step, g, ids, vocab, F32, 1.0)
     within(got, want, F32, slack, "d_table")
     np.testing.assert_array_equal(got, emb_backward(step, g, ids, vocab, F32, 1.0))
+
+
+@pytest.mark.parametrize("dim", [8, 5])
+@pytest.mark.parametrize("kind", ["half", "any"])
+def test_embedding_sorted_backward_long_lists(step, dim, kind):
+    """More entries of the sorted list for a warp than it looks at together."""
+    n, vocab = 200001, 700
+    rng = np.random.default_rng(dim)
+    ids = emb_ids(kind, n, vocab, rng).astype(np.int32)
+    g = rnd_np(rng.standard_normal((n, dim)).astype(np.float32), F16)
+    want, slack = emb_reference(g, ids, vocab, 0.5)
+    within(emb_backward(step, g, ids, vocab, F16, 0.5), want, F16, slack, "d_table")
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=ids_of)
@@ -399,3 +428,49 @@ def test_orthogonalize_is_scale_free_and_repeats(step):
     ref = ns_reference(g, 5, 0.0)
     sv = np.linalg.svd(one[0].astype(np.float64), compute_uv=False)
     np.testing.assert_allclose(sv, np.linalg.svd(ref[0], compute_uv=False), atol=4e-3 * 1.3)
+
+
+# ------------------------------------------------------------------ captured and replayed
+def test_captured_calls_replay_on_new_inputs(step):
+    """The entries recorded into one CUDA graph between eager calls that use the same workspace, replayed twice on other inputs."""
+    import torch
+    ctx = step
+    rows, cols, vocab = 4000, 256, 500
+    x, w, b, g = ln_data(rows, cols, F16, 3)
+    ids = np.random.default_rng(0).integers(0, vocab, rows).astype(np.int32)
+    m = ns_matrix(2, 300, 200, "strong", 4).astype(np.float32)
+    xt, wt, bt, gt, it, mt = dev(ctx, x, F16), dev(ctx, w, F16), dev(ctx, b, F16), dev(ctx, g, F16), dev(ctx, ids, I32), dev(ctx, m, F32)
+    out, dx, table, back = (ctx.scratch_empty(F16, s) for s in ((rows, cols), (rows, cols), (vocab, cols), (rows, cols)))
+    dw, db, o = ctx.scratch_empty(F16, (cols,)), ctx.scratch_empty(F16, (cols,)), ctx.scratch_empty(F16, m.shape)
+    stats = ctx.scratch_empty(F32, (rows, 2))
+    la, ea, oa = abi.LayerNormArgs(rows, cols, 1e-5, 0), abi.EmbeddingArgs(rows, vocab, cols), abi.OrthogonalizeArgs(2, 300, 200, 5, *COEFF, 1e-7)
+    scratch = ctx.scratch_empty(U8, (ctx.lib.gdb200_orthogonalize_scratch_bytes(byref(oa)),))
+
+    def calls():
+        be, lib = ctx.backend, ctx.lib
+        ctx.check(lib.gdb200_layer_norm_forward(be, xt.ref(), wt.ref(), bt.ref(), out.ref(), stats.ref(), byref(la)), "forward")
+        ctx.check(lib.gdb200_layer_norm_backward(be, xt.ref(), wt.ref(), stats.ref(), gt.ref(), dx.ref(), 0, dw.ref(), db.ref(), byref(la)), "backward")
+        ctx.check(lib.gdb200_embedding_sorted_backward(be, dx.ref(), it.ref(), table.ref(), 0, 1.0, byref(ea)), "sorted")
+        ctx.check(lib.gdb200_embedding_scaled_forward(be, table.ref(), it.ref(), back.ref(), 2.0, byref(ea)), "lookup")
+        ctx.check(lib.gdb200_orthogonalize(be, mt.ref(), o.ref(), scratch.ref(), byref(oa)), "orthogonalize")
+    results = lambda: [t.read() for t in (out, stats, dx, dw, db, table, back, o)]  # noqa: E731
+    calls()
+    ctx.flush()
+    stream = torch.cuda.ExternalStream(ctx.lib.gdb200_stream(ctx.backend))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        calls()
+    for k in range(2):
+        rng = np.random.default_rng(50 + k)
+        for t, a in ((xt, x[rng.permutation(rows)]), (gt, g[rng.permutation(rows)]), (it, rng.integers(-1, vocab, rows).astype(np.int32)), (mt, np.roll(m, k + 1, 1))):
+            t.write(a.astype(np.float16) if t.dtype == F16 else a)
+        calls()
+        want = results()
+        for t in (out, dx, table, back, o):
+            ctx.fill(t, 0x3C00)
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.flush()
+        for got, ref in zip(results(), want):
+            np.testing.assert_array_equal(got, ref)
+    del graph
