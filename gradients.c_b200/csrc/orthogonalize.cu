@@ -11,7 +11,7 @@
 // where FP16 loses bits.
 //
 // Large matrices are bound by the tensor cores under the power cap (four 5632 x 2048: 1.77 ms for five steps, 900 TFLOP/s), small ones by
-// the chain of three products a step (three 512 x 512: 90 us, 5.3 a launch), the smallest by the exchanges of a cluster (128 x 1000: 66 us).
+// the chain of three products a step (three 512 x 512: 90 us, 5.3 a launch), the smallest by the exchanges of a cluster (128 x 1000: 67 us).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -927,8 +927,10 @@ gd_status ns_launch_tile(gd_backend *be, const void *g, void *out, const gdb200_
     }
     const uint64_t n = std::max(a->rows, a->cols);
     unsigned ctas = 1;
+    // Enough CTAs for the columns, and more, down to 64 columns each, while all matrices' CTAs run at once: the rows of A that each adds up
+    // and sends get fewer (16 x 300: two CTAs 72 us, four 64, eight 60; 128 x 1400: eight 74, sixteen 72).
     if (n > NT_W_ALONE) {
-        while (ctas * NT_W < n) ctas *= 2U;
+        while (ctas * NT_W < n || (ctas < NT_MAX_CTAS && ctas * 64U < n && 2U * ctas * a->batch <= (uint64_t)be->sm_count)) ctas *= 2U;
     }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
