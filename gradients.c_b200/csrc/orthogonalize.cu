@@ -10,8 +10,8 @@
 // times), with the pair 0.02-0.2 %; where small matrices leave the time, A, P and the operand X are pairs too. X is kept times 2^10, which takes its elements (about 1 / sqrt(rows * cols)) out of the range
 // where FP16 loses bits.
 //
-// Large matrices are bound by the tensor cores under the power cap (four 5632 x 2048: 1.77 ms for five steps, 900 TFLOP/s), small ones by
-// the chain of three products a step (three 512 x 512: 90 us, 5.3 a launch), the smallest by the exchanges of a cluster (128 x 1000: 67 us).
+// Large matrices are bound by the tensor cores under the power cap (four 5632 x 2048: 1.72 to 1.80 ms for five steps, 880 to 920 TFLOP/s), small ones by
+// the chain of three products a step (three 512 x 512: 88 us, 5.2 a launch), the smallest by the exchanges of a cluster (128 x 1000: 67 us).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -105,22 +105,40 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
                 unsigned octets, float eps, bool vec)
 {
     gdb_pdl_sync();
-    // (every warp adds the partial sums in the same order)
+    const T *m = g + (size_t)blockIdx.y * rows * cols;
+    uint4 *h = reinterpret_cast<uint4 *>(hi) + (size_t)blockIdx.y * rows * octets, *l = reinterpret_cast<uint4 *>(lo) + (size_t)blockIdx.y * rows * octets;
+    const size_t n = (size_t)rows * octets, stride = (size_t)gridDim.x * blockDim.x;
+    size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const auto load = [&](size_t k, float (&v)[8]) {
+        const unsigned r = n < 0xffffffffU ? (unsigned)k / octets : (unsigned)(k / octets), c = (unsigned)(k - (size_t)r * octets) * 8U;
+        ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
+    };
+    // (the first elements are on their way while the partial sums are added, by every warp in the same order)
+    float v[2][8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        if (i + u * stride < n) load(i + u * stride, v[u]);
+    }
     const int lane = threadIdx.x & 31;
-    double s = 0.0;
-    for (int k = lane; k < parts; k += 32) s += __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + k]);
+    double part[NS_NORM_BLOCKS / 32], s = 0.0;
+#pragma unroll
+    for (int k = 0; k < NS_NORM_BLOCKS / 32; ++k) part[k] = lane + 32 * k < parts ? __ldg(&partial[(size_t)blockIdx.y * NS_NORM_BLOCKS + lane + 32 * k]) : 0.0;
+#pragma unroll
+    for (int k = 0; k < NS_NORM_BLOCKS / 32; ++k) s += part[k];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffU, s, o);
     const double f = (double)NS_UP / (sqrt(s) + (double)eps);
-    const T *m = g + (size_t)blockIdx.y * rows * cols;
-    uint4 *h = reinterpret_cast<uint4 *>(hi) + (size_t)blockIdx.y * rows * octets, *l = reinterpret_cast<uint4 *>(lo) + (size_t)blockIdx.y * rows * octets;
-    const size_t n = (size_t)rows * octets;
-#pragma unroll 2
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
-        const unsigned r = n < 0xffffffffU ? (unsigned)i / octets : (unsigned)(i / octets), c = (unsigned)(i - (size_t)r * octets) * 8U;
-        float v[8];
-        ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
-        ns_halves(v, f, (float)f, h[i], l[i]);
+    for (; i < n; i += 2U * stride) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const size_t k = i + u * stride;
+            if (k >= n) break;
+            uint4 a, b;
+            ns_halves(v[u], f, (float)f, a, b);
+            h[k] = a;
+            l[k] = b;
+            if (k + 2U * stride < n) load(k + 2U * stride, v[u]);
+        }
     }
 }
 
@@ -1111,7 +1129,9 @@ gd_status first_iterate(gd_backend *be, const void *g, double *partial, __half *
     gdb_launch(ns_norm_kernel<T>, dim3((unsigned)parts, (unsigned)a->batch), 256, 0, be->stream, (const T *)g, partial, count, even && (a->batch == 1U || count % 8U == 0U));
     gd_status st = gdb_launched(be, "orthogonalize norm");
     if (st != GD_OK) return st;
-    gdb_launch(ns_split_kernel<T>, dim3(gdb_grid_for(a->rows * (pitch / 8U), 256, be, 8), (unsigned)a->batch), 256, 0, be->stream, (const T *)g, (const double *)partial, (int)parts, hi, lo,
+    // (one wave of blocks, at six an SM, over all matrices)
+    const unsigned split_most = (unsigned)(((uint64_t)be->sm_count * 6U + a->batch - 1U) / a->batch), split_want = gdb_grid_for(a->rows * (pitch / 8U), 256, be, 6);
+    gdb_launch(ns_split_kernel<T>, dim3(split_want < split_most ? split_want : split_most, (unsigned)a->batch), 256, 0, be->stream, (const T *)g, (const double *)partial, (int)parts, hi, lo,
                (unsigned)a->rows, (unsigned)a->cols, (unsigned)(pitch / 8U), a->eps, even && a->cols % 8U == 0U);
     return gdb_launched(be, "orthogonalize split");
 }
