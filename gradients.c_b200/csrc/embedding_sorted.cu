@@ -10,11 +10,11 @@
 //    of the vocabulary and reads ALL ids (they lie in L2: 4 bytes each against 2 dim for the gradient's row), so it knows by itself how
 //    many ids lie below its slice. It also clears the rows of its slice that no id names.
 // 2. es_reduce_kernel: equal pieces of the sorted list, whatever the frequencies: a warp adds a few rows up to a few dozen for 32 vectors of
-//    columns, runs that begin and end within a piece are written, the others go to FP32 partial sums.
-// 3. es_merge_kernel: adds the partial sums of the runs that cross pieces, in order.
+//    columns, runs that begin and end within a piece are written, the others go to FP32 partial sums, which the block of the piece where
+//    the run ends adds up in order.
 // Every sum is FP32 in an order that depends on the ids, the sizes and the number of SMs alone.
-// 16384 ids, 32768 x 2048 BF16: lookup 19.5 us (6.2 TB/s), 1. 23.5 (14 of them clear 80 MB), 2. 24 (5 TB/s), 3. 5.5; 18432 ids, 2048 x 512 FP16:
-// 6, 9, 8, 5.5, where the launches count.
+// 16384 ids, 32768 x 2048 BF16: lookup 19.5 us (6.2 TB/s), 1. 24 (14 of them clear 80 MB), 2. 25.5 (4.7 TB/s); 18432 ids, 2048 x 512 FP16: 6, 9.5,
+// 13, where launches and the waits between pieces count.
 #include "common.cuh"
 
 #include <type_traits>
@@ -23,7 +23,8 @@ namespace {
 
 constexpr int ES_SORT_WARPS = 32, ES_AHEAD = 8;   // (ids on their way, a lane)
 constexpr unsigned ES_MAX_WIDTH = 1536, ES_ZEROS = 4096, ES_SORT_SMEM = 220 * 1024;   // tokens of a slice (32 x 1536 counters fill 192 KB), bytes
-constexpr int ES_WARPS = 8, ES_BLOCKS = 4;   // of a reducing block; blocks on an SM
+constexpr int ES_WARPS = 8, ES_BLOCKS = 4;   // of a summing block; blocks on an SM
+constexpr unsigned ES_POLLS = 1U << 21;      // of a flag, a second or two, before a wait gives up
 
 template <typename T, int VE> struct es_vec {
     T v[VE];
@@ -98,7 +99,7 @@ es_lookup_kernel(const V *__restrict__ table, const int *__restrict__ ids, V *__
 template <typename V>
 __global__ void __launch_bounds__(ES_SORT_WARPS * 32)
 es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned width, unsigned notes, unsigned *__restrict__ order, int *__restrict__ token,
-               unsigned *__restrict__ count, V *__restrict__ clear, size_t row_vecs)
+               unsigned *__restrict__ count, unsigned *__restrict__ flags, unsigned n_flags, V *__restrict__ clear, size_t row_vecs)
 {
     gdb_pdl_sync();
     constexpr bool BULK = sizeof(V) == 16U;
@@ -110,6 +111,7 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
     uint2 *note = sort_smem + (size_t)warp * notes;
     unsigned *counters = reinterpret_cast<unsigned *>(sort_smem + (size_t)ES_SORT_WARPS * notes), *mine = counters + (size_t)warp * width;
     for (unsigned k = threadIdx.x; k < ES_SORT_WARPS * width; k += blockDim.x) counters[k] = 0U;
+    for (unsigned k = blockIdx.x * blockDim.x + threadIdx.x; k < n_flags; k += gridDim.x * blockDim.x) flags[k] = 0U;
     if constexpr (BULK) {
         if (threadIdx.x < ES_ZEROS / 16U) zeros[threadIdx.x] = make_uint4(0U, 0U, 0U, 0U);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -184,7 +186,10 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
         __syncthreads();
     }
     if constexpr (BULK) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) count[0] = base;
+    if (blockIdx.x == gridDim.x - 1U && threadIdx.x == 0) {
+        count[0] = base;
+        count[1] = 0U;   // the summing blocks' turns
+    }
     // every id of the slice to its place, equal ids of a warp's 32 in lane order
     const auto put = [&](bool in, unsigned pos, unsigned k) {
         // lanes with the same token, a bit of it at a time (a match instruction took three times as long)
@@ -252,12 +257,22 @@ __device__ __forceinline__ void es_store(T *p, const float *s, float scale, bool
     *reinterpret_cast<vec *>(p) = v;
 }
 
-// Block (c, s): sorted entries [c * piece, (c + 1) * piece), a warp an eighth of them, columns [s * 32 * VE * NV, ...).
-// partial[c, 0] = sum of the run that began in an earlier piece, partial[c, 1] = of the one that begins here and goes on behind.
+__device__ __forceinline__ unsigned es_load_acquire(const unsigned *p)
+{
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
+// Piece c, slab s: sorted entries [c * piece, (c + 1) * piece), a warp an eighth of them, columns [s * 32 * VE * NV, ...). The piece in which
+// a run ends adds up its parts: partial[b, 1] of the piece b where it begins, partial[k, 0] of those that it fills, its own. Blocks take
+// their pieces in the order in which they start, so a block waits only for ones that run already (a launch of its own for the parts, 18432 ids
+// of 2048 x 512 FP16 26.9 instead of 27.4 us, 5003 of 20011 x 321 FP32 27.4 instead of 25.5, 16384 of 32768 x 2048 BF16 69.0 instead of 66.5);
+// flags[c, s]: the parts of piece c are in memory.
 template <typename T, int VE, int NV>
 __global__ void __launch_bounds__(ES_WARPS * 32, ES_BLOCKS)
-es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table,
-                 float *__restrict__ partial, unsigned n, unsigned piece, size_t dim, float scale, bool add)
+es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, const int *__restrict__ token, unsigned *count, T *__restrict__ table, float *partial,
+                 unsigned *flags, unsigned n, unsigned piece, unsigned slabs, size_t dim, float scale, bool add, int *err_flag)
 {
     gdb_pdl_sync();
     typedef es_vec<T, VE> vec;
@@ -275,16 +290,20 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
     __shared__ int first_token[ES_WARPS];
     __shared__ unsigned ends[ES_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned e0 = blockIdx.x * piece, per = piece / ES_WARPS, a = e0 + warp * per;
+    static_assert(COLS <= ES_WARPS * 32, "a thread per column");
+    __shared__ unsigned turn;
+    if (threadIdx.x == 0) turn = atomicAdd(&count[1], 1U);
+    __syncthreads();
+    const unsigned chunk = turn / slabs, slab = turn - chunk * slabs, e0 = chunk * piece, per = piece / ES_WARPS, a = e0 + warp * per;
     // (all n places of the lists may be read; those behind the ids inside the table hold nothing that is used)
     unsigned mine = a + lane < n ? __ldg(&order[a + lane]) : 0U;
     int mine_token = a + lane < n ? __ldg(&token[a + lane]) : -1;
     const int token_before = a > 0U && a <= n ? __ldg(&token[a - 1U]) : -1, token_after = a + per < n ? __ldg(&token[a + per]) : -1;
-    const unsigned total = count[0];
+    const unsigned total = __ldcg(count);
     if (e0 >= total) return;
     const unsigned e1 = min(total, e0 + piece), b = min(e1, a + per);
     const bool some = a < b;
-    const size_t col0 = (size_t)blockIdx.y * COLS;
+    const size_t col0 = (size_t)slab * COLS;
     float acc[NV][VE];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -387,76 +406,69 @@ es_reduce_kernel(const T *__restrict__ g, const unsigned *__restrict__ order, co
     }
     __syncthreads();
     // runs that cross the warps of the block, a thread per column, warps in order
-    for (int c = threadIdx.x; c < COLS; c += ES_WARPS * 32) {
-        if (col0 + c >= dim) break;
-        float sum = 0.0f;
-        bool from_before = true, open = false;   // the run being added began in an earlier piece; goes on behind the last warp
+    const unsigned c = min((unsigned)threadIdx.x, (unsigned)COLS - 1U);
+    const bool column = threadIdx.x < COLS && col0 + c < dim;
+    float sum = 0.0f, first = 0.0f;                            // of the run being added; of the one that began in an earlier piece
+    bool from_before = true, open = false, closes = false;     // sum is still that one's; goes on behind the last warp; that one ends here
 #pragma unroll
-        for (int k = 0; k < ES_WARPS; ++k) {
-            const unsigned f = ends[k];
-            if (f & 8U) continue;
-            open = (f & 2U) != 0U;
-            if (f & 1U) {
-                sum += head[k][c];
-                if (!(f & 4U)) {
-                    if (from_before) {
-                        partial[(size_t)blockIdx.x * 2U * dim + col0 + c] = sum;
-                    } else {
-                        es_store<T, 1>(table + (size_t)first_token[k] * dim + col0 + c, &sum, scale, add);
-                    }
-                    sum = 0.0f;
-                }
-            }
+    for (int k = 0; k < ES_WARPS; ++k) {
+        const unsigned f = ends[k];
+        if (f & 8U) continue;
+        open = (f & 2U) != 0U;
+        if (f & 1U) {
+            sum += head[k][c];
             if (!(f & 4U)) {
-                from_before = false;
-                if (f & 2U) sum = tail(k)[c];
+                if (from_before) {
+                    closes = true;
+                    first = sum;
+                } else if (column) {
+                    es_store<T, 1>(table + (size_t)first_token[k] * dim + col0 + c, &sum, scale, add);
+                }
+                sum = 0.0f;
             }
         }
-        if (open) partial[((size_t)blockIdx.x * 2U + (from_before ? 0U : 1U)) * dim + col0 + c] = sum;
+        if (!(f & 4U)) {
+            from_before = false;
+            if (f & 2U) sum = tail(k)[c];
+        }
     }
-}
-
-// Block (c, s): the run that begins in piece c and goes on in the next ones, if there is one; a warp adds every eighth of its parts, 128
-// columns at a time.
-template <typename T>
-__global__ void __launch_bounds__(256)
-es_merge_kernel(const float *__restrict__ partial, const int *__restrict__ token, const unsigned *__restrict__ count, T *__restrict__ table, unsigned n, unsigned piece,
-                size_t dim, float scale, bool add)
-{
-    gdb_pdl_sync();
-    __shared__ float sh[8][128];
-    const unsigned c = blockIdx.x, e0 = c * piece, e1 = e0 + piece, e2 = e1 + piece;   // (e1 < n)
-    const int k = __ldg(&token[e1]), last = __ldg(&token[e1 - 1]), before = e0 > 0U ? __ldg(&token[e0 - 1]) : -1, next = e2 < n && e2 > e1 ? __ldg(&token[e2]) : -1;
-    const unsigned total = count[0];
-    if (e1 >= total || last != k || before == k) return;   // nothing behind this piece, complete, or begun earlier
-    // last piece whose first entry has this token (most runs end in the next one)
-    unsigned lo = c + 1U, hi = e2 < total && next == k ? (total - 1U) / piece : lo;
-    while (lo < hi) {
-        const unsigned mid = (lo + hi + 1U) / 2U;
-        if (token[(size_t)mid * piece] == k) lo = mid; else hi = mid - 1U;
+    if (open) {
+        if (column) __stcg(&partial[((size_t)chunk * 2U + (from_before ? 0U : 1U)) * dim + col0 + c], sum);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            __threadfence();
+            atomicExch(&flags[(size_t)chunk * slabs + slab], 1U);
+        }
     }
-    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const unsigned parts = min(8U, lo - c + 1U);
-    for (size_t col0 = (size_t)blockIdx.y * 128U; col0 < dim; col0 += (size_t)gridDim.y * 128U) {
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-        for (unsigned j = c + (unsigned)part; j <= lo; j += 8U) {
-            const float *row = partial + ((size_t)j * 2U + (j == c ? 1U : 0U)) * dim + col0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (col0 + lane + 32 * e < dim) s[e] += __ldcg(&row[lane + 32 * e]);
+    if (!closes) return;
+    // the piece in which the run begins: the one in front of the first piece whose preceding entry has the token
+    const int tok = first_token[0];
+    unsigned begins = chunk, full;   // (32 pieces looked at together, by every warp)
+    do {
+        const bool same = begins > (unsigned)lane + 1U && __ldg(&token[(size_t)(begins - 1U - lane) * piece - 1U]) == tok;
+        const unsigned apart = ~__ballot_sync(0xffffffffU, same);
+        full = apart != 0U ? (unsigned)__ffs((int)apart) - 1U : 32U;
+        begins -= full;
+    } while (full == 32U);
+    begins -= 1U;
+    for (unsigned k = begins + threadIdx.x; k < chunk; k += ES_WARPS * 32) {
+        const unsigned *flag = &flags[(size_t)k * slabs + slab];
+        unsigned polls = 0;
+        while (es_load_acquire(flag) == 0U) {
+            if (++polls == ES_POLLS) {
+                atomicExch(err_flag, 611);
+                break;
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sh[part][lane + 32 * e] = s[e];
-        __syncthreads();
-        if (threadIdx.x < 128U && col0 + threadIdx.x < dim) {
-            float v = 0.0f;
-            for (unsigned p = 0; p < parts; ++p) v += sh[p][threadIdx.x];
-            es_store<T, 1>(table + (size_t)k * dim + col0 + threadIdx.x, &v, scale, add);
-        }
-        __syncthreads();
     }
+    __syncthreads();
+    if (!column) return;
+    const float *part = partial + col0 + c;
+    sum = __ldcg(part + ((size_t)begins * 2U + 1U) * dim);
+#pragma unroll 16
+    for (unsigned k = begins + 1U; k < chunk; ++k) sum += __ldcg(part + (size_t)k * 2U * dim);
+    sum += first;
+    es_store<T, 1>(table + (size_t)tok * dim + col0 + c, &sum, scale, add);
 }
 
 template <typename T, typename V>
@@ -472,19 +484,12 @@ gd_status lookup(gd_backend *be, const void *table, const int *ids, void *out, c
 }
 
 template <typename T, int VE, int NV>
-gd_status reduce(gd_backend *be, const void *g, const unsigned *order, const int *token, const unsigned *count, void *table, float *partial, unsigned n, unsigned piece,
-                 unsigned pieces, size_t dim, float scale, bool add)
+gd_status reduce(gd_backend *be, const void *g, const unsigned *order, const int *token, unsigned *count, void *table, float *partial, unsigned *flags, unsigned n, unsigned piece,
+                 unsigned pieces, unsigned slabs, size_t dim, float scale, bool add)
 {
-    const size_t slabs = (dim + 32U * VE * NV - 1U) / (32U * VE * NV);
-    if (slabs > 65535U) return GD_ERR_UNSUPPORTED;
-    gdb_launch(es_reduce_kernel<T, VE, NV>, dim3(pieces, (unsigned)slabs), ES_WARPS * 32, 0, be->stream, (const T *)g, order, token, count, (T *)table, partial, n, piece, dim, scale,
-               add);
-    gd_status st = gdb_launched(be, "embedding_sorted_backward sums");
-    if (st != GD_OK || pieces == 1U) return st;
-    const size_t col_blocks = (dim + 127U) / 128U;
-    gdb_launch(es_merge_kernel<T>, dim3(pieces - 1U, (unsigned)(col_blocks < 4U ? col_blocks : 4U)), 256, 0, be->stream, (const float *)partial, token, count, (T *)table, n, piece, dim,
-               scale, add);
-    return gdb_launched(be, "embedding_sorted_backward merge");
+    gdb_launch(es_reduce_kernel<T, VE, NV>, pieces * slabs, ES_WARPS * 32, 0, be->stream, (const T *)g, order, token, count, (T *)table, partial, flags, n, piece, slabs, dim, scale, add,
+               be->err_flag);
+    return gdb_launched(be, "embedding_sorted_backward sums");
 }
 
 template <typename T>
@@ -495,14 +500,14 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     const size_t dim = a->dim, row_bytes = dim * sizeof(T);
     const bool vec = dim % VE == 0U && (((uintptr_t)g | (uintptr_t)table) % 16U) == 0U;
     const size_t slabs = vec ? (dim + 32U * VE - 1U) / (32U * VE) : (dim + 255U) / 256U;
-    // order, token, count, partial sums
+    // order, token, count and turns, partial sums, flags
     const size_t list = ((size_t)n * 4U + 255U) & ~(size_t)255U;
-    if (2U * list + 256U + 2U * dim * sizeof(float) > be->ws_bytes) return GD_ERR_OUT_OF_MEMORY;
+    if (2U * list + 256U + 2U * dim * sizeof(float) + slabs * sizeof(unsigned) > be->ws_bytes) return GD_ERR_OUT_OF_MEMORY;
     unsigned *order = reinterpret_cast<unsigned *>(be->ws);
     int *token = reinterpret_cast<int *>(be->ws + list);
     unsigned *count = reinterpret_cast<unsigned *>(be->ws + 2U * list);
     float *partial = reinterpret_cast<float *>(be->ws + 2U * list + 256U);
-    const size_t fit = (be->ws_bytes - 2U * list - 256U) / (2U * dim * sizeof(float));
+    const size_t fit = (be->ws_bytes - 2U * list - 256U) / (2U * dim * sizeof(float) + slabs * sizeof(unsigned));
     // entries of a warp: what gives every place on the GPU one block, 8 at least (rows on their way); more where the partial sums would not
     // fit the workspace
     size_t per = ((size_t)n * slabs + (size_t)be->sm_count * ES_BLOCKS * ES_WARPS - 1U) / ((size_t)be->sm_count * ES_BLOCKS * ES_WARPS);
@@ -510,6 +515,9 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     if (per > 4096U) per = 4096U;
     while (((size_t)n + per * ES_WARPS - 1U) / (per * ES_WARPS) > fit) per *= 2U;
     const size_t piece = per * ES_WARPS, pieces = ((size_t)n + piece - 1U) / piece;
+    if (pieces * slabs > 0x7fffffffU) return GD_ERR_UNSUPPORTED;
+    unsigned *flags = reinterpret_cast<unsigned *>(partial + pieces * 2U * dim);
+    const unsigned n_flags = (unsigned)(pieces * slabs);
     // a slice of the vocabulary per block, two blocks' worth of SMs at most where the counters allow it
     unsigned width = (vocab + (unsigned)be->sm_count - 1U) / (unsigned)be->sm_count;
     if (width > ES_MAX_WIDTH) width = ES_MAX_WIDTH;
@@ -528,14 +536,14 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
         ready = true;
     }
     if (vec) {
-        gdb_launch(es_sort_kernel<uint4>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, notes, order, token, count, add ? (uint4 *)nullptr : (uint4 *)table, row_bytes / 16U);
+        gdb_launch(es_sort_kernel<uint4>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, notes, order, token, count, flags, n_flags, add ? (uint4 *)nullptr : (uint4 *)table, row_bytes / 16U);
     } else {
-        gdb_launch(es_sort_kernel<T>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, notes, order, token, count, add ? (T *)nullptr : (T *)table, dim);
+        gdb_launch(es_sort_kernel<T>, slices, ES_SORT_WARPS * 32, smem, be->stream, ids, n, vocab, width, notes, order, token, count, flags, n_flags, add ? (T *)nullptr : (T *)table, dim);
     }
     gd_status st = gdb_launched(be, "embedding_sorted_backward sort");
     if (st != GD_OK) return st;
-    return vec ? reduce<T, VE, 1>(be, g, order, token, count, table, partial, n, (unsigned)piece, (unsigned)pieces, dim, scale, add)
-               : reduce<T, 1, 8>(be, g, order, token, count, table, partial, n, (unsigned)piece, (unsigned)pieces, dim, scale, add);
+    return vec ? reduce<T, VE, 1>(be, g, order, token, count, table, partial, flags, n, (unsigned)piece, (unsigned)pieces, (unsigned)slabs, dim, scale, add)
+               : reduce<T, 1, 8>(be, g, order, token, count, table, partial, flags, n, (unsigned)piece, (unsigned)pieces, (unsigned)slabs, dim, scale, add);
 }
 
 bool es_args_ok(const gd_backend_tensor_view *rows, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *table, const gd_backend_embedding_args *a)
