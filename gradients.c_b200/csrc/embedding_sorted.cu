@@ -232,11 +232,22 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
     if constexpr (BULK) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (clear != nullptr) {
-        const V zero = {};
-        for (unsigned k = warp; k < w; k += ES_SORT_WARPS) {
-            if (((absent[k / 32U] >> (k & 31U)) & 1U) == 0U) continue;
-            V *row = clear + (size_t)(v0 + k) * row_vecs;
-            for (size_t c = lane; c < row_vecs; c += 32U) row[c] = zero;
+        // neighbouring rows together, whole vectors in the middle; 32 tokens a warp, or several warps where there are fewer
+        const unsigned words = (w + 31U) / 32U, share = words < ES_SORT_WARPS ? ES_SORT_WARPS / words : 1U;
+        for (unsigned unit = warp; unit < words * share; unit += ES_SORT_WARPS) {
+            const unsigned k0 = unit % words * 32U, part = unit / words;
+            unsigned bits = absent[k0 / 32U];
+            while (bits != 0U) {
+                const unsigned r = __ffs((int)bits) - 1U, stop = ~(bits >> r), rows = stop != 0U ? __ffs((int)stop) - 1U : 32U;
+                bits &= r + rows < 32U ? 0xffffffffU << (r + rows) : 0U;
+                V *p = clear + (size_t)(v0 + k0 + r) * row_vecs;
+                const size_t n_all = (size_t)rows * row_vecs, lead = (16U - (uintptr_t)p % 16U) % 16U / sizeof(V), n_lead = lead < n_all ? lead : n_all;
+                const size_t n_wide = (n_all - n_lead) / (16U / sizeof(V)), behind = n_lead + n_wide * (16U / sizeof(V));
+                const V zero = {};
+                for (size_t c = part * 32U + lane; c < n_wide; c += share * 32U) reinterpret_cast<uint4 *>(p + n_lead)[c] = make_uint4(0U, 0U, 0U, 0U);
+                if (part == 0U && lane < n_lead) p[lane] = zero;
+                if (part == 0U && behind + lane < n_all) p[behind + lane] = zero;
+            }
         }
     }
 }
