@@ -209,25 +209,38 @@ es_sort_kernel(const int *__restrict__ ids, unsigned n, unsigned vocab, unsigned
             token[at] = (int)(v0 + k);
         }
     };
-    if (found <= notes) {
-        for (unsigned j = 0; j < found; j += 32U) {
-            const bool in = j + lane < found;
+    const auto put_notes = [&](unsigned held) {
+        __syncwarp();
+        for (unsigned j = 0; j < held; j += 32U) {
+            const bool in = j + lane < held;
             const uint2 e = in ? note[j + lane] : make_uint2(0U, 0U);
             put(in, e.x, e.y);
         }
+        __syncwarp();
+    };
+    if (found <= notes) {
+        put_notes(found);
     } else {
+        // noted again, and put down whenever the notes are full (the few of every 32 ids by themselves: 300000 ids, 32000 tokens, 232 instead of 138 us)
+        unsigned held = 0U;
         for (unsigned i = i0; i < i1; i += 32U * ES_AHEAD) {
             unsigned id[ES_AHEAD];
 #pragma unroll
             for (int u = 0; u < ES_AHEAD; ++u) id[u] = i + 32U * u + lane < i1 ? (unsigned)__ldg(&ids[i + 32U * u + lane]) : 0xffffffffU;
 #pragma unroll 1
             for (int u = 0; u < ES_AHEAD; ++u) {
-                unsigned k = id[0] - v0;   // (the array moves on: its places are registers)
+                const unsigned k = id[0] - v0, here = __ballot_sync(0xffffffffU, k < w);   // (the array moves on: its places are registers)
 #pragma unroll
                 for (int m = 1; m < ES_AHEAD; ++m) id[m - 1] = id[m];
-                if (__ballot_sync(0xffffffffU, k < w) != 0U) put(k < w, i + 32U * u + lane, k);
+                if (k < w) note[held + __popc(here & lower)] = make_uint2(i + 32U * u + lane, k);
+                held += __popc(here);
+                if (held + 32U > notes) {
+                    put_notes(held);
+                    held = 0U;
+                }
             }
         }
+        put_notes(held);
     }
     if constexpr (BULK) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
