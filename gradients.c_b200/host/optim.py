@@ -292,20 +292,26 @@ class Muon(AdamW):
     def _update(self, active: Sequence[int], lr: float, found_buf, found_off: int) -> None:
         chosen = set(self.matrices)
         rest = [i for i in active if i not in chosen]
-        super()._update(rest, lr, found_buf, found_off)
         groups: dict[tuple, list[int]] = {}
         for i in active:
             if i in chosen:
                 groups.setdefault(self.slots[i].param.shape, []).append(i)
         if not groups:
+            super()._update(rest, lr, found_buf, found_off)
             return
         ctx, lib, cfg, descs = self.ctx, self.ctx.lib, self.muon, self._muon_descs
         mark, count, work = ctx.scratch.top, 0, []
-        for shape, members in groups.items():
-            full = (len(members),) + shape
-            direction = ctx.scratch_empty(F32, full, "muon_direction")
-            update = ctx.scratch_empty(F16, full, "muon_update")
-            work.append((full, direction, update))
+        try:   # all that the step lends, before anything is updated
+            for shape, members in groups.items():
+                full = (len(members),) + shape
+                work.append((full, ctx.scratch_empty(F32, full, "muon_direction"), ctx.scratch_empty(F16, full, "muon_update")))
+            # one scratch for all groups: their calls follow one another on the stream
+            lent = ctx.scratch_empty(U8, (max(self._scratch_bytes(ctx, full) for full, _, _ in work),), "muon_scratch")
+        except MemoryError:
+            ctx.scratch.top = mark
+            raise
+        super()._update(rest, lr, found_buf, found_off)
+        for (shape, members), (full, direction, update) in zip(groups.items(), work):
             for i, d_i, u_i in ((i, direction.rows(k, 1), update.rows(k, 1)) for k, i in enumerate(members)):
                 s, d = self.slots[i], descs[count]
                 p, g = s.param, s.param.grad
@@ -325,9 +331,6 @@ class Muon(AdamW):
                 count += 1
         ctx.check(lib.gdb200_muon_momentum_batch(ctx.backend, descs, count), "muon_momentum_batch")
         for full, direction, update in work:
-            top = ctx.scratch.top     # one scratch for all groups: their calls follow one another on the stream
-            lent = ctx.scratch_empty(U8, (self._scratch_bytes(ctx, full),), "muon_scratch")
             ctx.check(lib.gdb200_orthogonalize(ctx.backend, direction.ref(), update.ref(), lent.ref(), byref(self._args(full))), "orthogonalize")
-            ctx.scratch.top = top
         ctx.check(lib.gdb200_muon_apply_batch(ctx.backend, descs, count), "muon_apply_batch")
         ctx.scratch.top = mark

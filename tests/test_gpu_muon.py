@@ -216,6 +216,21 @@ def test_optimizer_overflow_and_missing_gradients():
         assert opt.step_count() == 2
 
 
+def test_optimizer_without_room_updates_nothing():
+    with pkg.runtime.Context(params_bytes=1 << 22, state_bytes=1 << 23, scratch_bytes=1 << 20) as ctx:
+        ps = [ctx.from_numpy(ctx.params, F16, np.full(s, 0.5, np.float32)) for s in ((300, 200), (33,))]
+        opt, sc = optim.Muon(ctx, ps, optim.MuonConfig(), optim.AdamwConfig()), optim.AmpScaler(ctx)
+        ctx.begin_step()
+        gradients(ctx, ps, [np.ones(p.shape, np.float32) for p in ps])
+        top = ctx.scratch.top
+        with pytest.raises(MemoryError):
+            opt.step_amp_clip_lr(sc, 0.01, 1.0)
+        assert ctx.scratch.top == top and opt.step_count() == 0
+        for p in ps:
+            assert (host(p) == 0.5).all()
+        ctx.end_step()
+
+
 # ------------------------------------------------------------------ all of them in one training step
 VOCAB, DIM, HIDDEN, TOKENS = 200, 96, 320, 170
 
