@@ -376,7 +376,8 @@ ns_single_kernel(const __grid_constant__ ns_maps maps, const ns_shape sh, int *e
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tcgen05_fence_before();
-    __syncthreads();
+    __syncwarp();
+    if (SPLIT) cluster_sync_all(); else __syncthreads();   // (the peer runs before its memory is written; under the end of the launch before)
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int quad = warp & 3, part = (warp - 2) >> 2;   // (epilogue warps: tensor-memory quadrant, columns)
