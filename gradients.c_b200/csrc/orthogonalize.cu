@@ -111,7 +111,13 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
     size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
     const auto load = [&](size_t k, float (&v)[8]) {
         const unsigned r = n < 0xffffffffU ? (unsigned)k / octets : (unsigned)(k / octets), c = (unsigned)(k - (size_t)r * octets) * 8U;
-        ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
+        if (c < cols) {
+            ns_load8(m + (size_t)r * cols + c, cols - c, vec, v);
+        } else {
+            // (rows of the scratch are a multiple of 16 elements: the last octet may lie behind the matrix's row as a whole)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        }
     };
     // (the first elements are on their way while the partial sums are added, by every warp in the same order)
     float v[2][8];

@@ -419,6 +419,31 @@ def test_orthogonalize_extreme_and_empty_matrices(step):
     assert ns_call(step, g[:0], F32, F16).size == 0 and ns_call(step, g[:, :0], F32, F16).size == 0
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=ids_of)
+@pytest.mark.parametrize("batch,rows,cols", [(1, 130, 1201), (2, 131, 136), (1, 150, 1208), (2, 1201, 129), (1, 137, 143), (1, 130, 144)])
+def test_orthogonalize_reads_nothing_behind_a_row(step, dtype, batch, rows, cols):
+    """The scratch keeps rows of a multiple of 16 elements. What is behind a row's end there is zeros: neither the next row nor what lies
+    behind the tensor (NaN here) was read. One step leaves the first iterate, both its halves, at the beginning of the scratch."""
+    ctx = step
+    g = rnd_np((64 * ns_matrix(batch, rows, cols, "noise", rows + cols)).astype(np.float32), dtype)
+    whole = dev(ctx, np.concatenate([g.reshape(-1), np.full(64, np.nan, np.float32)]), dtype)
+    x = pkg.runtime.Tensor(ctx, ctx.scratch, whole.offset, dtype, g.shape)
+    args, out = abi.OrthogonalizeArgs(batch, rows, cols, 1, *COEFF, 1e-7), ctx.scratch_empty(F16, g.shape)
+    scratch = ctx.scratch_empty(U8, (ctx.lib.gdb200_orthogonalize_scratch_bytes(byref(args)),))
+    scratch.write(np.full(scratch.count, 0xFF, dtype=np.uint8))
+    ctx.check(ctx.lib.gdb200_orthogonalize(ctx.backend, x.ref(), out.ref(), scratch.ref(), byref(args)), "orthogonalize")
+    ns_check(host(out), ns_reference(g, 1, 1e-7), F16, steps=1)
+    pitch = (cols + 15) // 16 * 16
+    buffer = (batch * rows * pitch * 2 + 255) // 256 * 256
+    want = g.astype(np.float64)
+    want = 1024 * want / (np.sqrt((want * want).sum((1, 2), keepdims=True)) + float(np.float32(1e-7)))
+    hi, lo = (pkg.runtime.Tensor(ctx, ctx.scratch, scratch.offset + at * buffer, F16, (batch, rows, pitch)).read() for at in (0, 2))
+    assert (hi[:, :, cols:] == 0).all() and (lo[:, :, cols:] == 0).all()
+    # an FP32 product (two roundings: the factor's and its own) as two FP16 numbers, whose second is rounded again
+    err = np.abs(hi[:, :, :cols].astype(np.float64) + lo[:, :, :cols].astype(np.float64) - want)
+    assert (err <= (2 * E24 + 2.0 ** -22) * np.abs(want) * (1 + 2.0 ** -8) + TINY[F16]).all()
+
+
 def test_orthogonalize_is_scale_free_and_repeats(step):
     """Powers of two change nothing (the products see the same numbers), and a call repeats bit for bit."""
     g = ns_matrix(2, 200, 333, "strong", 3).astype(np.float32)
