@@ -274,7 +274,7 @@ class GptLm:
             def reshape_backward():
                 if attn_flat.grad is not None:
                     ctx.accumulate_grad(attn, attn_flat.grad.reshape(attn.shape))
-            ctx.record(reshape_backward)
+            ctx.record(reshape_backward, attn_flat)
         proj = ops.gd_linear_transposed_weight(ctx, attn_flat, p[pre + "attn_proj.weight"], p[pre + "attn_proj.bias"])
         resid = ops.gd_dropout_add(ctx, x, proj, cfg.dropout_p, self.training, self._site_seed(GPT_DROPOUT_ATTN, i, step))
         normed2 = ops.gd_rms_norm(ctx, resid, p[pre + "mlp_norm_w"], cfg.rms_eps)

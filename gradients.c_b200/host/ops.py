@@ -60,7 +60,7 @@ def gd_embedding(ctx: Context, table: Tensor, ids: Tensor) -> Tensor:
             ctx.check(ctx.lib.gd_backend_embedding_backward(ctx.backend, _tvp(out.grad), _tvp(ids), _tvp(dtable),
                                                             _tvp(scratch), byref(args)), "embedding_backward")
             ctx.accumulate_grad(table, dtable)
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -76,13 +76,13 @@ def gd_embedding_scaled(ctx: Context, table: Tensor, ids: Tensor, scale: float =
         def backward():
             if out.grad is None:
                 return
-            into = table.grad is not None
+            into = table.grad is not None and ctx.may_add_into_grad(table)
             dtable = table.grad if into else ctx.scratch_empty(table.dtype, table.shape, "d_table")
             ctx.check(ctx.lib.gdb200_embedding_sorted_backward(ctx.backend, _tvp(out.grad), _tvp(ids), _tvp(dtable), 1 if into else 0, scale, byref(args)),
                       "embedding_sorted_backward")
             if not into:
                 ctx.accumulate_grad(table, dtable)
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -108,7 +108,7 @@ def gd_dropout(ctx: Context, x: Tensor, p: float, training: bool, seed: int) -> 
         def backward():
             if y.grad is not None:
                 ctx.accumulate_grad(x, _dropout_backward_mask(ctx, mask, y.grad, scale))
-        ctx.record(backward)
+        ctx.record(backward, y)
     return y
 
 
@@ -131,7 +131,7 @@ def gd_add(ctx: Context, x: Tensor, y: Tensor) -> Tensor:
                     mv, vv = out.grad.mv(rows, cols), dy.vv()
                     ctx.check(ctx.lib.gd_backend_reduce_rows(ctx.backend, byref(mv), byref(vv)), "reduce_rows")
                     ctx.accumulate_grad(y, dy)
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -154,7 +154,7 @@ def gd_dropout_add(ctx: Context, residual: Tensor, x: Tensor, p: float, training
             if x.requires_grad:
                 ctx.accumulate_grad(x, _dropout_backward_mask(ctx, mask, y.grad, scale))
             ctx.accumulate_grad(residual, y.grad)
-        ctx.record(backward)
+        ctx.record(backward, y)
     return y
 
 
@@ -184,7 +184,8 @@ def gd_rms_norm(ctx: Context, x: Tensor, weight: Tensor, eps: float) -> Tensor:
             if out.grad is None:
                 return
             if ONE_PASS_BACKWARD and x.requires_grad and weight.requires_grad:
-                mark, into = ctx.scratch.top, x.grad is not None      # a gradient that is there is added to in the same launch
+                # a gradient that is there, and x's alone, is added to in the same launch
+                mark, into = ctx.scratch.top, x.grad is not None and ctx.may_add_into_grad(x)
                 dx = x.grad if into else ctx.scratch_empty(x.dtype, x.shape, "d_rms_x")
                 dw = ctx.scratch_empty(weight.dtype, weight.shape, "d_rms_w")
                 partial = ctx.scratch_empty(F32, (max(args.row_blocks, RMS_ONE_PASS_ROWS), cols), "rms_partial")
@@ -206,7 +207,7 @@ def gd_rms_norm(ctx: Context, x: Tensor, weight: Tensor, eps: float) -> Tensor:
                 partial = ctx.scratch_empty(F32, (args.row_blocks, cols), "rms_partial")
                 ctx.check(ctx.lib.gd_backend_rms_norm_weight_backward_stats(ctx.backend, _tvp(x), _tvp(inv), _tvp(out.grad), _tvp(dw), _tvp(partial), byref(args)), "rms_norm_weight_backward_stats")
                 ctx.accumulate_grad(weight, dw)
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -226,8 +227,8 @@ def gd_layer_norm(ctx: Context, x: Tensor, weight: Optional[Tensor], bias: Optio
         def backward():
             if out.grad is None:
                 return
-            # (a residual connection may have given x the very tensor that is out's gradient)
-            into = x.requires_grad and x.grad is not None and x.grad is not out.grad
+            # (a residual connection may have given x the very tensor that is out's gradient, or another's)
+            into = x.requires_grad and x.grad is not None and ctx.may_add_into_grad(x)
             dx = None
             if x.requires_grad:
                 dx = x.grad if into else ctx.scratch_empty(x.dtype, x.shape, "d_layer_norm_x")
@@ -241,7 +242,7 @@ def gd_layer_norm(ctx: Context, x: Tensor, weight: Optional[Tensor], bias: Optio
                 ctx.accumulate_grad(weight, dw)
             if db is not None:
                 ctx.accumulate_grad(bias, db)
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -301,7 +302,7 @@ def gd_linear_transposed_weight(ctx: Context, x: Tensor, w: Tensor, bias: Option
                 ctx.accumulate_grad(w, dw)
             if bias is not None and bias.requires_grad:
                 ctx.accumulate_grad(bias, _reduce_rows(ctx, g, m, n, bias))
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -350,7 +351,7 @@ def gd_linear(ctx: Context, x: Tensor, w: Tensor, bias: Optional[Tensor]) -> Ten
                 ctx.accumulate_grad(w, dw)
             if db is not None:
                 ctx.accumulate_grad(bias, db)
-        ctx.record(backward)
+        ctx.record(backward, y)
     return y
 
 
@@ -365,7 +366,7 @@ def gd_swiglu_split(ctx: Context, x12: Tensor) -> Tensor:
         def backward():
             if out.grad is not None:
                 ctx.accumulate_grad(x12, _swiglu_split_backward(ctx, x12, out.grad))
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -408,7 +409,7 @@ def gd_swiglu_split_linear(ctx: Context, x12: Tensor, w: Tensor, bias: Optional[
             if x12.requires_grad:
                 dact, _, _ = gd_linear_backward(ctx, act, w, bias, g, True, False, False)
                 ctx.accumulate_grad(x12, _swiglu_split_backward(ctx, x12, dact))
-        ctx.record(backward)
+        ctx.record(backward, y)
     return y
 
 
@@ -436,7 +437,7 @@ def gd_qkv_split_rope(ctx: Context, qkv: Tensor, positions: Tensor, n_heads: int
             ctx.check(ctx.lib.gd_backend_qkv_split_rope_backward(ctx.backend, _tvp(gs[0]), _tvp(gs[1]), _tvp(gs[2]), _tvp(positions),
                                                                  _tvp(dqkv), n_heads, head_dim, byref(args)), "qkv_split_rope_backward")
             ctx.accumulate_grad(qkv, dqkv)
-        ctx.record(backward)
+        ctx.record(backward, q, k, v)
     return q, k, v
 
 
@@ -475,7 +476,7 @@ def gd_sdpa_varlen(ctx: Context, q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Te
             ctx.accumulate_grad(q, dq)
             ctx.accumulate_grad(k, dk)
             ctx.accumulate_grad(v, dv)
-        ctx.record(backward)
+        ctx.record(backward, out)
     return out
 
 
@@ -608,5 +609,5 @@ def gd_lm_cross_entropy_softcapped_bias_ignore(ctx: Context, hidden: Tensor, wei
                 ctx.accumulate_grad(weight, dw)
             if db is not None:
                 ctx.accumulate_grad(bias, db)
-        ctx.record(backward)
+        ctx.record(backward, loss)
     return loss

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import weakref
 from typing import Callable, Optional, Sequence
 
 import numpy as np
@@ -210,7 +211,8 @@ class Context:
         self.state = Arena(self, "state", state_bytes)
         self.scratch = Arena(self, "scratch", scratch_bytes)
         self._make_data_slot(data_bytes)
-        self.tape: list[Callable[[], None]] = []
+        self.tape: list[tuple[Callable[[], None], tuple[Tensor, ...]]] = []
+        self._held: dict[tuple[Arena, int], list[weakref.ref]] = {}   # place of a gradient: the tensors that have it
         self.grad_enabled = True
         self._fences: list[abi.Fence] = []
         self.run_ahead = 0
@@ -275,6 +277,7 @@ class Context:
         self._data_before, self._data_base = (self._data_base, self.data.top), 0   # range of the data slot the step before uses
         self.data.reset()
         self.tape.clear()
+        self._held = {place: ts for place, ts in getattr(self, "_held", {}).items() if place[0] is not self.scratch}
         self.check(self.lib.gd_backend_scope_begin(self.backend), "scope_begin")
         self.in_step = True
 
@@ -335,23 +338,60 @@ class Context:
         return ts
 
     # ---- tape (reference gd_autograd_record + reverse walk) ----
-    def record(self, backward: Callable[[], None]) -> None:
+    def record(self, backward: Callable[[], None], *outputs: Tensor) -> None:
+        """`outputs`: what the operation gave. Their gradients are `backward`'s to read; behind it nothing of the walk reads them."""
         if self.grad_enabled:
-            self.tape.append(backward)
+            self.tape.append((backward, outputs))
 
     def accumulate_grad(self, t: Tensor, g: Tensor) -> None:
         """First contribution is adopted, later ones are added with gd_backend_accumulate
-        (16-bit storage rounds after every add), as src/autograd/autograd.c:517-685 does."""
+        (16-bit storage rounds after every add), as src/autograd/autograd.c:517-685 does. A sum
+        hands one gradient to both its terms: while another tensor holds it too, the later
+        contribution gives a new gradient (the same rounding of the same two numbers)."""
         if not t.requires_grad:
             return
         if t.grad is None:
             t.grad = g
         else:
-            assert t.grad.count == g.count and t.grad.dtype == g.dtype
-            self.check(self.lib.gd_backend_accumulate(self.backend, t.grad.buffer, t.grad.offset, g.buffer, g.offset,
-                                                      g.count, g.dtype), "accumulate")
+            old = t.grad
+            assert old.count == g.count and old.dtype == g.dtype
+            if self.may_add_into_grad(t):
+                self.check(self.lib.gd_backend_accumulate(self.backend, old.buffer, old.offset, g.buffer, g.offset,
+                                                          g.count, g.dtype), "accumulate")
+                return
+            flat = lambda a: C.byref(a.arena.view(a.offset, a.dtype, (a.count,), a.count))  # noqa: E731
+            t.grad = self.scratch_empty(old.dtype, old.shape, "grad_sum")
+            self.check(self.lib.gd_backend_add(self.backend, flat(old), flat(g), flat(t.grad)), "add(gradients)")
+        self._hold(t)
+
+    def may_add_into_grad(self, t: Tensor) -> bool:
+        """Whether t's gradient may be changed in place: no other tensor holds the same memory as a gradient that is still to be read (by
+        the walk, or, for a leaf, by whoever asked for it)."""
+        g = t.grad
+        for r in self._held.get((g.arena, g.offset), ()):
+            h = r()
+            if h is not None and h is not t and h.grad is not None and h.grad.arena is g.arena and h.grad.offset == g.offset:
+                return False
+        return True
+
+    def _hold(self, t: Tensor) -> None:
+        place, r = (t.grad.arena, t.grad.offset), weakref.ref(t)
+        holders = self._held.get(place)
+        if holders is None:
+            self._held[place] = [r]
+        elif r not in holders:
+            holders[:] = [h for h in holders if h() is not None]
+            holders.append(r)
 
     def run_backward(self) -> None:
-        for fn in reversed(self.tape):
+        for fn, outputs in reversed(self.tape):
+            for o in outputs:
+                if o.grad is not None:
+                    self._hold(o)
             fn()
+            for o in outputs:
+                if o.grad is not None:
+                    holders, r = self._held.get((o.grad.arena, o.grad.offset), ()), weakref.ref(o)
+                    if r in holders:
+                        holders.remove(r)
         self.tape.clear()
