@@ -177,6 +177,13 @@ class AdamW:
     def step_amp_clip_lr(self, scaler: AmpScaler, lr: float, max_grad_norm: float, inv_scale_override: Optional[Tensor] = None) -> None:
         """gd_optimizer_step_amp_clip_lr: unscale + global norm + clip factor in one pass over the
         gradients, then the AdamW update (skipped on overflow), then the scaler update."""
+        try:
+            self._step(scaler, lr, max_grad_norm, inv_scale_override)
+        except BaseException:
+            scaler.step_begun = False   # given up: the next step begins anew, with no overflow found
+            raise
+
+    def _step(self, scaler: AmpScaler, lr: float, max_grad_norm: float, inv_scale_override: Optional[Tensor]) -> None:
         ctx, lib = self.ctx, self.ctx.lib
         scaler.begin_step()
         inv_buf = scaler.scale_state.buffer
@@ -299,17 +306,22 @@ class Muon(AdamW):
         if not groups:
             super()._update(rest, lr, found_buf, found_off)
             return
+        mark = self.ctx.scratch.top
+        try:
+            self._update_with_matrices(rest, groups, lr, found_buf, found_off)
+        finally:
+            self.ctx.scratch.top = mark
+
+    def _update_with_matrices(self, rest: Sequence[int], groups: dict[tuple, list[int]], lr: float, found_buf, found_off: int) -> None:
+        """The update of the matrices `groups` (by shape) and of the slots `rest` beside them. What it lends from the scratch arena is the caller's to give back."""
         ctx, lib, cfg, descs = self.ctx, self.ctx.lib, self.muon, self._muon_descs
-        mark, count, work = ctx.scratch.top, 0, []
-        try:   # all that the step lends, before anything is updated
-            for shape, members in groups.items():
-                full = (len(members),) + shape
-                work.append((full, ctx.scratch_empty(F32, full, "muon_direction"), ctx.scratch_empty(F16, full, "muon_update")))
-            # one scratch for all groups: their calls follow one another on the stream
-            lent = ctx.scratch_empty(U8, (max(self._scratch_bytes(ctx, full) for full, _, _ in work),), "muon_scratch")
-        except MemoryError:
-            ctx.scratch.top = mark
-            raise
+        count, work = 0, []
+        # all that the step lends, before anything is updated
+        for shape, members in groups.items():
+            full = (len(members),) + shape
+            work.append((full, ctx.scratch_empty(F32, full, "muon_direction"), ctx.scratch_empty(F16, full, "muon_update")))
+        # one scratch for all groups: their calls follow one another on the stream
+        lent = ctx.scratch_empty(U8, (max(self._scratch_bytes(ctx, full) for full, _, _ in work),), "muon_scratch")
         super()._update(rest, lr, found_buf, found_off)
         for (shape, members), (full, direction, update) in zip(groups.items(), work):
             for i, d_i, u_i in ((i, direction.rows(k, 1), update.rows(k, 1)) for k, i in enumerate(members)):
@@ -333,4 +345,3 @@ class Muon(AdamW):
         for full, direction, update in work:
             ctx.check(lib.gdb200_orthogonalize(ctx.backend, direction.ref(), update.ref(), lent.ref(), byref(self._args(full))), "orthogonalize")
         ctx.check(lib.gdb200_muon_apply_batch(ctx.backend, descs, count), "muon_apply_batch")
-        ctx.scratch.top = mark

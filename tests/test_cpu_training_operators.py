@@ -165,3 +165,54 @@ def test_muon_takes_matrices_only():
 def test_native_trainer_refuses_muon():
     with pytest.raises(ValueError):
         pkg.gpt_lm.NativeTrainer(None, pkg.gpt_lm.TrainConfig(muon=optim.MuonConfig()))
+
+
+@pytest.mark.parametrize("error", [MemoryError, ValueError, abi.BackendError])
+def test_a_step_that_fails_gives_everything_back(error):
+    """No room, a group of matrices that is not taken, an entry that refuses: the scaler is not left within a step (the next one clears the
+    overflow flag), and the scratch arena is as it was."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *args: calls.append(name) or 0
+
+        @staticmethod
+        def gdb200_orthogonalize_scratch_bytes(args):
+            return 0 if error is ValueError and args._obj.batch > 1 else 256
+    arena = lambda at, size: type("Arena", (), dict(buffer=at, top=0, high_water=0, capacity=size, alloc=pkg.runtime.Arena.alloc, view=pkg.runtime.Arena.view, _views={}, name=str(at)))()  # noqa: E731
+    ctx = type("Ctx", (pkg.runtime.Context,), {"destroy": lambda self: None})
+    ctx = ctx.__new__(ctx)
+    ctx.lib, ctx.backend = Lib(), None
+    ctx.params, ctx.state, ctx.scratch = arena(1, 1 << 20), arena(2, 1 << 22), arena(3, 1 << 20)
+    ctx.last_error = lambda: ""
+    params = [ctx.empty(ctx.params, F32, s) for s in ((40, 24), (40, 24), (33,))]
+    opt, scaler = optim.Muon(ctx, params, optim.MuonConfig(), optim.AdamwConfig()), optim.AmpScaler(ctx)
+
+    def gradients():
+        for p in params:
+            p.grad = ctx.empty(ctx.scratch, p.dtype, p.shape)
+    gradients()
+    top, room = ctx.scratch.top, ctx.scratch.capacity
+    if error is MemoryError:
+        ctx.scratch.capacity = top + 6000    # the directions fit, the updates do not
+    check = ctx.check
+    if error is abi.BackendError:
+        def refuse(status, what):
+            if what == "orthogonalize":
+                raise abi.BackendError(BAD, what, "")
+        ctx.check = refuse
+    scaler.begin_step()                      # (as the backward pass does for the seed)
+    del calls[:]
+    with pytest.raises(error):
+        opt.step_amp_clip_lr(scaler, 0.01, 1.0)
+    assert not scaler.step_begun and ctx.scratch.top == top
+    assert "gd_backend_amp_finish_step" not in calls and ("gd_backend_adamw_batch" in calls) == (error is abi.BackendError)
+    if error is ValueError:
+        return
+    ctx.scratch.capacity, ctx.check = room, check
+    del calls[:]
+    opt.step_amp_clip_lr(scaler, 0.01, 1.0)
+    assert calls == ["gd_backend_amp_begin_step", "gd_backend_grad_clip_scale", "gd_backend_adamw_batch", "gdb200_muon_momentum_batch", "gdb200_orthogonalize",
+                     "gdb200_muon_apply_batch", "gd_backend_amp_finish_step"]
+    assert not scaler.step_begun and ctx.scratch.top == top

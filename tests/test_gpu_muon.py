@@ -231,6 +231,31 @@ def test_optimizer_without_room_updates_nothing():
         ctx.end_step()
 
 
+def test_step_after_one_without_room():
+    """A step that overflowed and found no room is forgotten: the next one, with both, updates and leaves the loss scale."""
+    with pkg.runtime.Context(params_bytes=1 << 22, state_bytes=1 << 23, scratch_bytes=1 << 22) as ctx:
+        ps = [ctx.from_numpy(ctx.params, F16, np.full(s, 0.5, np.float32)) for s in ((300, 200), (33,))]
+        opt, sc = optim.Muon(ctx, ps, optim.MuonConfig(), optim.AdamwConfig()), optim.AmpScaler(ctx, optim.AmpConfig(init_scale=64.0))
+        for bad in (True, False):
+            ctx.begin_step()
+            seed = ctx.scratch_empty(F32, (1,))
+            sc.fill_scale(seed)   # (the backward pass begins the scaler's step)
+            gradients(ctx, ps, [np.full(p.shape, np.inf if bad else 1.0, np.float32) for p in ps])
+            room = ctx.scratch.capacity
+            if bad:
+                ctx.scratch.capacity = ctx.scratch.top + 4096
+                with pytest.raises(MemoryError):
+                    opt.step_amp_clip_lr(sc, 0.01, 1.0)
+                ctx.scratch.capacity = room
+            else:
+                opt.step_amp_clip_lr(sc, 0.01, 1.0)
+            ctx.end_step()
+        assert opt.state_i32.read().tolist() == [1, 1, 1]
+        assert all((host(p) != 0.5).all() and np.isfinite(host(p)).all() for p in ps)
+        state = sc.sync()
+        assert state["scale"] == 64.0 and state["last_found_inf"] == 0 and state["growth_tracker"] == 1
+
+
 # ------------------------------------------------------------------ all of them in one training step
 VOCAB, DIM, HIDDEN, TOKENS = 200, 96, 320, 170
 
