@@ -1193,7 +1193,7 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
     for (uint32_t k = 0; k < a->steps && st == GD_OK; ++k) {
         const ns_tensor &x0 = xs[k & 1U], &x1 = xs[(k & 1U) ^ 1U];
         ns_shape square = {};
-        square.parts = out->dtype == GDB_DTYPE_F16 ? l.parts : 1U;
+        square.parts = out->dtype == GDB_DTYPE_F16 || m <= (uint64_t)NT_M ? l.parts : 1U;   // (up to NT_M as in the one launch of shorter matrices)
         square.M = square.N = (uint32_t)m;
         square.K = (uint32_t)(tall ? rows : cols);
         square.batch = (uint32_t)a->batch;

@@ -395,6 +395,16 @@ def test_orthogonalize_small_sides_keep_fp16_precision(step, batch, rows, cols, 
         assert np.linalg.norm(got[k] - want[k]) <= (U[F16] + 15 * 64 * 2.0 ** -21) * np.linalg.norm(want[k]), k
 
 
+@pytest.mark.parametrize("kind", ["noise", "strong"])
+@pytest.mark.parametrize("batch,rows,cols", [(1, 128, 4097), (2, 3500, 100), (1, 17, 3080), (2, 100, 500), (1, 128, 128)])
+def test_orthogonalize_smallest_sides_have_one_precision(step, batch, rows, cols, kind):
+    """Up to a smaller side of 128 the products' operands are sums of two FP16 numbers whatever the result's type is and the longer side: a
+    BF16 and an FP16 result are two roundings of the same numbers."""
+    g = ns_matrix(batch, rows, cols, kind, rows + cols).astype(np.float32)
+    fine, coarse = (ns_call(step, g, F32, t).astype(np.float64) for t in (F16, BF16))
+    assert (np.abs(fine - coarse) <= (U[F16] + U[BF16]) * np.abs(fine) * (1 + 2.0 ** -7) + TINY[F16]).all()
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 8])
 def test_orthogonalize_steps_and_other_coefficients(step, steps):
     g = ns_matrix(2, 100, 180, "noise", 6).astype(np.float32)
