@@ -187,6 +187,9 @@ static inline bool gdb_is_float_dtype(uint32_t dt)
     return dt == GDB_DTYPE_F16 || dt == GDB_DTYPE_BF16 || dt == GDB_DTYPE_F32;
 }
 
+// SMs for a kernel whose blocks take an SM each and stay: those that a concurrent collective was promised are not among them.
+static inline unsigned gdb_usable_sms(const gd_backend *be) { return (unsigned)(be->sm_count - be->sm_reserve); }
+
 static inline unsigned gdb_grid_for(size_t work_items, unsigned threads, const gd_backend *be, unsigned waves)
 {
     size_t blocks = (work_items + threads - 1U) / threads;

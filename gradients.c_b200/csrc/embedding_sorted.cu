@@ -534,7 +534,8 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     const size_t fit = (be->ws_bytes - 2U * list - 256U) / (2U * dim * sizeof(float) + slabs * sizeof(unsigned));
     // entries of a warp: what gives every place on the GPU one block, 8 at least (rows on their way); more where the partial sums would not
     // fit the workspace
-    size_t per = ((size_t)n * slabs + (size_t)be->sm_count * ES_BLOCKS * ES_WARPS - 1U) / ((size_t)be->sm_count * ES_BLOCKS * ES_WARPS);
+    const unsigned sms = gdb_usable_sms(be);
+    size_t per = ((size_t)n * slabs + (size_t)sms * ES_BLOCKS * ES_WARPS - 1U) / ((size_t)sms * ES_BLOCKS * ES_WARPS);
     if (per < 8U) per = 8U;
     if (per > 4096U) per = 4096U;
     while (((size_t)n + per * ES_WARPS - 1U) / (per * ES_WARPS) > fit) per *= 2U;
@@ -543,7 +544,7 @@ gd_status backward(gd_backend *be, const void *g, const int *ids, void *table, c
     unsigned *flags = reinterpret_cast<unsigned *>(partial + pieces * 2U * dim);
     const unsigned n_flags = (unsigned)(pieces * slabs);
     // a slice of the vocabulary per block, two blocks' worth of SMs at most where the counters allow it
-    unsigned width = (vocab + (unsigned)be->sm_count - 1U) / (unsigned)be->sm_count;
+    unsigned width = (vocab + sms - 1U) / sms;
     if (width > ES_MAX_WIDTH) width = ES_MAX_WIDTH;
     const unsigned slices = (vocab + width - 1U) / width;
     // (more than half of an SM's shared memory: blocks that start while the preceding kernel drains would pair up on the SMs it left first)

@@ -671,11 +671,11 @@ bool ln_tiles(const gd_backend *be, const ln_call &a, int streams, ln_stream *st
     while (r * a.cols * sizeof(T) % 16U != 0U || (r < 8U * GROUPS && 2U * r * a.cols * sizeof(T) <= 16384U)) r *= 2U;
     const size_t bytes = r * a.cols * sizeof(T), slot = (bytes + 127U) & ~(size_t)127U;
     const size_t stages = LN_RING_BYTES / (slot * streams), tiles = (a.rows + r - 1U) / r;
-    if (LN_RING_BYTES / (slot * counted) < 3U || tiles < 2U * (size_t)be->sm_count) return false;
+    if (LN_RING_BYTES / (slot * counted) < 3U || tiles < 2U * (size_t)gdb_usable_sms(be)) return false;
     st->tile_rows = (unsigned)r;
     st->tile_bytes = (unsigned)bytes;
     st->stages = (unsigned)(stages < LN_MAX_STAGES ? stages : LN_MAX_STAGES);
-    *blocks = (unsigned)(tiles < (size_t)be->sm_count ? tiles : (size_t)be->sm_count);
+    *blocks = gdb_usable_sms(be);   // (fewer than tiles)
     return true;
 }
 template <typename T, int TPR, int VE, int EPT, int BWD>
@@ -731,7 +731,9 @@ gd_status fwd_go(gd_backend *be, const ln_call &a)
         if (e != cudaSuccess) return gdb_fail(be, e, "layer_norm_forward smem attribute");
         ready = true;
     }
-    gdb_launch(layer_norm_fwd_kernel<T, TPR, VE>, gdb_grid_for(a.rows, PER, be, ln_fwd_blocks(TPR, VE)), THREADS, smem, be->stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.out,
+    // (one wave: blocks stay and walk over the rows)
+    const size_t most = (size_t)gdb_usable_sms(be) * ln_fwd_blocks(TPR, VE), need = (a.rows + PER - 1U) / PER;
+    gdb_launch(layer_norm_fwd_kernel<T, TPR, VE>, (unsigned)(need < most ? need : most), THREADS, smem, be->stream, (const T *)a.x, (const T *)a.w, (const T *)a.b, (T *)a.out,
                a.stats, a.rows, (unsigned)a.cols, a.eps);
     return gdb_launched(be, "layer_norm_forward");
 }
@@ -807,9 +809,9 @@ gd_status bwd_typed(gd_backend *be, const ln_call &a)
         }
         st = GD_OK;
     } else {
-        const unsigned most = (unsigned)(!sums || fit > (size_t)be->sm_count ? (size_t)be->sm_count : fit);
+        const unsigned sms = gdb_usable_sms(be), most = !sums || fit > sms ? sms : (unsigned)fit;
         const bool vec = a.cols % VE == 0U && (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.g | (uintptr_t)a.dx) % 16U) == 0U;
-        st = most < (unsigned)be->sm_count ? GD_ERR_UNSUPPORTED
+        st = most < sms                    ? GD_ERR_UNSUPPORTED
              : a.add_to_dx                 ? (vec ? stream_typed<T, VE, 2>(be, a, partial, &blocks) : stream_typed<T, 1, 2>(be, a, partial, &blocks))
                                            : (vec ? stream_typed<T, VE, 1>(be, a, partial, &blocks) : stream_typed<T, 1, 1>(be, a, partial, &blocks));
         if (st == GD_ERR_UNSUPPORTED) {

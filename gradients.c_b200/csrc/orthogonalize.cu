@@ -955,7 +955,7 @@ gd_status ns_launch_tile(gd_backend *be, const void *g, void *out, const gdb200_
     // Enough CTAs for the columns, and more, down to 64 columns each, while all matrices' CTAs run at once: the rows of A that each adds up
     // and sends get fewer (16 x 300: two CTAs 72 us, four 64, eight 60; 128 x 1400: eight 74, sixteen 72).
     if (n > NT_W_ALONE) {
-        while (ctas * NT_W < n || (ctas < NT_MAX_CTAS && ctas * 64U < n && 2U * ctas * a->batch <= (uint64_t)be->sm_count)) ctas *= 2U;
+        while (ctas * NT_W < n || (ctas < NT_MAX_CTAS && ctas * 64U < n && 2U * ctas * a->batch <= gdb_usable_sms(be))) ctas *= 2U;
     }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -1035,7 +1035,7 @@ gd_status ns_launch_pair(gd_backend *be, const ns_maps &maps, const ns_shape &sh
         if (e != cudaSuccess) return gdb_fail(be, e, "orthogonalize smem attribute");
         ready = true;
     }
-    const uint32_t most = (uint32_t)be->sm_count / 2U;
+    const uint32_t most = gdb_usable_sms(be) / 2U;
     return ns_launch_clusters(be, kern, dim3(2U * (units < most ? units : most)), 32U * (2 + NS2_WARPS), NS2_SMEM, maps, sh);
 }
 
@@ -1044,7 +1044,7 @@ template <bool A_MN, bool B_MN, int MODE, typename TOUT = __half>
 gd_status ns_product(gd_backend *be, const ns_tensor &xa, const ns_tensor &xb, ns_shape sh, ns_memo *memo)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    const uint64_t sms = (uint64_t)be->sm_count, clusters = sms / 2U;
+    const uint64_t sms = gdb_usable_sms(be), clusters = sms / 2U;
     const uint32_t p_m = (sh.M + 255U) / 256U, p_n = (sh.N + 255U) / 256U, s_m = (sh.M + 127U) / 128U;
     const uint32_t pairs = (SYM ? p_n * (p_n + 1U) / 2U : p_m * p_n) * sh.batch;
     auto singles = [&](uint32_t bn) {
