@@ -7,8 +7,8 @@
 // matrices with a few strong directions), sums FP32. The iterate is carried as the sum of two FP16 numbers, X = hi + lo: the product
 // takes hi, the linear term a X takes both. With hi alone the rounding of the strong directions, spread over all directions and
 // amplified a-fold per step as the weak ones are, is 0.8 % of the result for strong directions 20 times the others (3 % for 200
-// times), with the pair 0.02-0.2 %; where small matrices leave the time, A, P and the operand X are pairs too. X is kept times 2^10, which takes its elements (about 1 / sqrt(rows * cols)) out of the range
-// where FP16 loses bits.
+// times), with the pair 0.02-0.2 %. For small matrices, and for all where the caller asks for it, A, P and the operand X are pairs too. X is
+// kept times 2^10, which takes its elements (about 1 / sqrt(rows * cols)) out of the range where FP16 loses bits.
 //
 // Large matrices are bound by the tensor cores under the power cap (four 5632 x 2048: 1.72 to 1.80 ms for five steps, 880 to 920 TFLOP/s), small ones by
 // the chain of three products a step (three 512 x 512: 88 us, 5.2 a launch), the smallest by the exchanges of a cluster (128 x 1000: 67 us).
@@ -154,12 +154,14 @@ ns_split_kernel(const T *__restrict__ g, const double *__restrict__ partial, int
 // either order of the product's operands does.
 enum { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
 
-// Smaller sides up to which an FP16 result gets its full precision: operands as sums of two FP16 numbers, hi hi + hi lo + lo hi of three
-// products in one accumulator. Rounded to one FP16 number each, A and P cost the result up to 2e-3 in the 2-norm where its singular values
-// are close together (rounding errors of the diagonals add up), 3e-4 where a few stand out; with three products what is left is the
-// result's own rounding, 2e-4. Time of a call, one product and three: 129 x 140 55 and 86 us, 129 x 1000 72 and 118, 300 x 300 69 and 123,
-// 400 x 420 80 and 141: small matrices wait for launches more than for products. Larger ones would pay three times the products and keep
-// one; so do BF16 results, whose rounding is 1.7e-3 (but where one launch does all, below, three take 6 to 13 us more of 25 to 60).
+// Smaller sides up to which an FP16 result gets its full precision without being asked for it: operands as sums of two FP16 numbers, hi hi +
+// hi lo + lo hi of three products in one accumulator. Rounded to one FP16 number each, A and P cost the result up to 1.7e-3 in the 2-norm
+// where its singular values are close together (rounding errors of the diagonals add up), 3e-4 where a few stand out; with three products
+// what is left is the result's own rounding, 2.1e-4. What they cost grows with the size and has no turn; the cut is where it is three
+// quarters of a call. One product and three, one square matrix: 129 54 and 84 us (1.54 times), 256 63 and 106 (1.68), 448 81 and 140 (1.73),
+// 480 83 and 147 (1.78), 512 87 and 152 (1.76), 640 94 and 173 (1.84), 896 117 and 233 (2.0); four of 5632 x 2048 1500 and 4010 (2.7). BF16
+// results, whose own rounding is 1.7e-3 (2.1e-3 to 2.4e-3 with one product), keep one product unless asked (but where one launch does all,
+// below, three take 6 to 13 us more of 25 to 60).
 constexpr uint64_t NS_FINE = 448;
 
 struct ns_maps {
@@ -1098,14 +1100,14 @@ struct ns_layout {
 };
 bool ns_plan(const gdb200_orthogonalize_args *a, ns_layout *l)
 {
-    if (a == NULL || a->rows >= (1U << 24) || a->cols >= (1U << 24) || a->batch > 65535U) return false;
+    if (a == NULL || a->rows >= (1U << 24) || a->cols >= (1U << 24) || a->batch > 65535U || a->pairs > 1U) return false;
     l->small = a->rows < a->cols ? a->rows : a->cols;
     l->pitch = (a->cols + 15U) & ~(uint64_t)15U;   // (32 bytes: one access of the epilogue)
     l->small_pitch = (l->small + 15U) & ~(size_t)15U;
     // (the products count tiles of a batch in 32 bits)
     if ((a->rows / 128U + 1U) * (a->cols / 64U + 1U) * (a->batch + 1U) > 0x7fffffffU) return false;
     const size_t x = (a->batch * a->rows * l->pitch * 2U + 255U) & ~(size_t)255U, s = (a->batch * l->small * l->small_pitch * 2U + 255U) & ~(size_t)255U;
-    l->parts = l->small <= NS_FINE ? 3U : 1U;
+    l->parts = a->pairs != 0U || l->small <= NS_FINE ? 3U : 1U;
     const size_t s_lo = l->parts > 1U ? s : 0U;
     size_t at = 0U;
     const auto next = [&](size_t *where, size_t bytes) {
@@ -1156,7 +1158,7 @@ size_t gdb200_orthogonalize_scratch_bytes(const gdb200_orthogonalize_args *args)
 gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, const gd_backend_tensor_view *out, const gd_backend_tensor_view *scratch,
                                const gdb200_orthogonalize_args *a)
 {
-    if (be == NULL || x == NULL || out == NULL || scratch == NULL || a == NULL || a->steps == 0U || !(a->eps >= 0.0f)) {
+    if (be == NULL || x == NULL || out == NULL || scratch == NULL || a == NULL || a->steps == 0U || !(a->eps >= 0.0f) || a->pairs > 1U) {
         return GD_ERR_INVALID_ARGUMENT;
     }
     ns_layout l;
@@ -1193,7 +1195,7 @@ gd_status gdb200_orthogonalize(gd_backend *be, const gd_backend_tensor_view *x, 
     for (uint32_t k = 0; k < a->steps && st == GD_OK; ++k) {
         const ns_tensor &x0 = xs[k & 1U], &x1 = xs[(k & 1U) ^ 1U];
         ns_shape square = {};
-        square.parts = out->dtype == GDB_DTYPE_F16 || m <= (uint64_t)NT_M ? l.parts : 1U;   // (up to NT_M as in the one launch of shorter matrices)
+        square.parts = out->dtype == GDB_DTYPE_F16 || a->pairs != 0U || m <= (uint64_t)NT_M ? l.parts : 1U;   // (up to NT_M as in the one launch of shorter matrices)
         square.M = square.N = (uint32_t)m;
         square.K = (uint32_t)(tall ? rows : cols);
         square.batch = (uint32_t)a->batch;

@@ -126,7 +126,7 @@ class LayerNormArgs(C.Structure):
 
 
 class OrthogonalizeArgs(C.Structure):
-    _fields_ = [("batch", U64), ("rows", U64), ("cols", U64), ("steps", U32), ("a", F), ("b", F), ("c", F), ("eps", F)]
+    _fields_ = [("batch", U64), ("rows", U64), ("cols", U64), ("steps", U32), ("a", F), ("b", F), ("c", F), ("eps", F), ("pairs", U32)]
 
 
 class MuonDesc(C.Structure):

@@ -49,13 +49,15 @@ class AdamwConfig:  # gd_adamw_config_default, src/optim/adamw.c:1087-1097
 class MuonConfig:
     """Muon: matrices step along the orthogonalised momentum of their gradients, W <- W - lr * update_rms * sqrt(max(rows, cols)) * O - lr *
     weight_decay * W. The factor gives a step of any matrix the root mean square lr * update_rms, about that of an AdamW step, so that both
-    share a learning rate; the three coefficients are those of the Newton-Schulz polynomial a x + b x^3 + c x^5."""
+    share a learning rate; the three coefficients are those of the Newton-Schulz polynomial a x + b x^3 + c x^5. `pairs`: products of sums of
+    two FP16 numbers for matrices of every size, three times the work (gdb200_orthogonalize)."""
     momentum: float = 0.95
     nesterov: bool = True
     steps: int = 5
     coefficients: tuple = (3.4445, -4.7750, 2.0315)
     eps: float = 1.0e-7
     update_rms: float = 0.2
+    pairs: bool = False
 
 
 def gd_lr_scheduler_value(max_lr: float, min_lr: float, warmup_steps: int, total_steps: int, step: int) -> float:
@@ -286,7 +288,7 @@ class Muon(AdamW):
 
     def _args(self, shape: tuple) -> abi.OrthogonalizeArgs:
         c = self.muon
-        return abi.OrthogonalizeArgs(*shape, c.steps, *c.coefficients, c.eps)
+        return abi.OrthogonalizeArgs(*shape, c.steps, *c.coefficients, c.eps, 1 if c.pairs else 0)
 
     def _scratch_bytes(self, ctx: Context, shape: tuple) -> int:
         need = self.scratch_need.get(shape)

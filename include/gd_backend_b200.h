@@ -569,8 +569,9 @@ gd_status gdb200_embedding_sorted_backward(gd_backend *backend, const gd_backend
 /* Orthogonalisation of `batch` matrices [rows, cols] by Newton-Schulz products (what the Muon optimizer steps along; the reference has
  * AdamW only, src/optim/adamw.c): X = x / (|x|_F + eps), then `steps` times A = X X^T (on the smaller side), X <- a X + (b A + c A^2) X,
  * out = X. x F16, BF16 or F32, out F16 or BF16. The products' operands are FP16 numbers with FP32 sums: sums of two each where the
- * smaller side is at most 128, and up to 448 for an F16 out (the result is then off by its own rounding), one each elsewhere (off by up to
- * 0.2 % in the 2-norm, 0.03 % where a few singular values stand out); the iterate is always carried in two. out may be x (the same
+ * smaller side is at most 128, up to 448 for an F16 out, and wherever `pairs` asks for it (the result is then off by its own rounding), one
+ * each elsewhere (off by up to 0.2 % in the 2-norm, 0.03 % where a few singular values stand out, beside the rounding); pairs take 1.5 to
+ * 2.7 times as long, from small matrices to large ones. The iterate is always carried in two. out may be x (the same
  * tensor). The iterates have to stay below 64 in magnitude, as they do for coefficients whose polynomial maps [0, 1.3] into itself. A
  * matrix of zeros gives zeros (eps > 0). `scratch`: U8, 256-byte aligned, of gdb200_orthogonalize_scratch_bytes(args) bytes (0: a shape
  * that is not taken), not to be shared with a call on another stream. */
@@ -578,6 +579,7 @@ typedef struct gdb200_orthogonalize_args {
     uint64_t batch, rows, cols;
     uint32_t steps;
     float a, b, c, eps;
+    uint32_t pairs;   /* 1: operands as sums of two whatever the size and the type of out; 0: as above */
 } gdb200_orthogonalize_args;
 size_t gdb200_orthogonalize_scratch_bytes(const gdb200_orthogonalize_args *args);
 gd_status gdb200_orthogonalize(gd_backend *backend, const gd_backend_tensor_view *x, const gd_backend_tensor_view *out, const gd_backend_tensor_view *scratch,

@@ -216,3 +216,16 @@ def test_a_step_that_fails_gives_everything_back(error):
     assert calls == ["gd_backend_amp_begin_step", "gd_backend_grad_clip_scale", "gd_backend_adamw_batch", "gdb200_muon_momentum_batch", "gdb200_orthogonalize",
                      "gdb200_muon_apply_batch", "gd_backend_amp_finish_step"]
     assert not scaler.step_begun and ctx.scratch.top == top
+
+
+def test_orthogonalize_pairs(fake):
+    """More scratch where pairs are asked for beyond the sizes that have them anyway; no other value."""
+    lib, be, b = fake
+    b.nbytes = 1 << 26
+    with_pairs = lambda value, rows, cols: abi.OrthogonalizeArgs(1, rows, cols, 5, 3.4445, -4.7750, 2.0315, 1e-7, value)  # noqa: E731
+    need = lambda *a: lib.gdb200_orthogonalize_scratch_bytes(C.byref(with_pairs(*a)))  # noqa: E731
+    assert need(0, 448, 600) == need(1, 448, 600) and 0 < need(0, 449, 600) < need(1, 449, 600)
+    assert need(2, 449, 600) == 0
+    x, out = view(b, F32, 449 * 600), view(b, F16, 449 * 600, 1 << 22)
+    call = lambda value, scratch: lib.gdb200_orthogonalize(be, C.byref(x), C.byref(out), C.byref(view(b, U8, scratch, 1 << 23)), C.byref(with_pairs(value, 449, 600)))  # noqa: E731
+    assert call(2, need(1, 449, 600)) == BAD and call(1, need(0, 449, 600)) == BAD

@@ -231,6 +231,23 @@ def test_optimizer_without_room_updates_nothing():
         ctx.end_step()
 
 
+def test_optimizer_with_pairs():
+    """MuonConfig.pairs reaches the products: the step is off by the update's rounding to FP16 and FP32 roundings alone. (The bound is that of
+    the orthogonalisation's own test; one FP16 number an operand is 1.5e-3 off for this matrix.)"""
+    shape, lr = (600, 520), 0.02
+    with pkg.runtime.Context(params_bytes=1 << 22, state_bytes=1 << 24, scratch_bytes=1 << 26) as ctx:
+        p = ctx.from_numpy(ctx.params, F32, np.zeros(shape, np.float32))
+        cfg = optim.MuonConfig(nesterov=False, pairs=True)
+        opt, sc = optim.Muon(ctx, [p], cfg, optim.AdamwConfig(), [0.0]), optim.AmpScaler(ctx, optim.AmpConfig(init_scale=1.0))
+        ctx.begin_step()
+        a = 1e3 * ns_matrix(1, *shape, "noise", 4)[0].astype(np.float32)
+        gradients(ctx, [p], [a])
+        opt.step_amp_clip_lr(sc, lr, 1e9)
+        want = -f32(lr * cfg.update_rms * math.sqrt(max(shape))) * ns_reference(a[None], cfg.steps, cfg.eps, cfg.coefficients)[0]
+        assert np.linalg.norm(host(p) - want) <= (U[F16] + 15 * 64 * 2.0 ** -21 + 4 * E24) * np.linalg.norm(want)
+        ctx.end_step()
+
+
 def test_step_after_one_without_room():
     """A step that overflowed and found no room is forgotten: the next one, with both, updates and leaves the loss scale."""
     with pkg.runtime.Context(params_bytes=1 << 22, state_bytes=1 << 23, scratch_bytes=1 << 22) as ctx:
