@@ -12,9 +12,10 @@
 // 2. es_reduce_kernel: equal pieces of the sorted list, whatever the frequencies: a warp adds a few rows up to a few dozen for 32 vectors of
 //    columns, runs that begin and end within a piece are written, the others go to FP32 partial sums, which the block of the piece where
 //    the run ends adds up in order.
-// Every sum is FP32 in an order that depends on the ids, the sizes and the number of SMs alone.
+// Every sum is FP32 in an order that depends on the ids, the sizes, the number of SMs and the workspace alone.
 // 16384 ids, 32768 x 2048 BF16: lookup 19.5 us (6.2 TB/s), 1. 24 (14 of them clear 80 MB), 2. 25.5 (4.7 TB/s); 18432 ids, 2048 x 512 FP16: 6, 9.5,
-// 13, where launches and the waits between pieces count.
+// 13, where launches and the waits between pieces count. The scatter next door and this on the same inputs, calls among others: 128 and 46 us,
+// 39 and 20, 5003 ids of 20011 x 321 FP32 37 and 21.
 #include "common.cuh"
 
 #include <type_traits>

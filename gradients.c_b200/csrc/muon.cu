@@ -5,7 +5,7 @@
 //   p <- p - step o - decay p,  param = round(p)                                  muon_apply_kernel
 //
 // Both are bound by HBM: with 16-bit gradients and parameters 14 and 12 bytes an element (momentum, direction and master FP32, the update
-// 16 bits), a flop or two for each: 4 matrices of 2048 x 5632 take 104 us (6.2 TB/s) and 79 us (7.0 TB/s), 12 of 512 x 512 (in L2) 11 and 8 us,
+// 16 bits), a flop or two for each: 4 matrices of 2048 x 5632 take 103 us (6.2 TB/s) and 89 us (6.2 TB/s), 12 of 512 x 512 (in L2) 11 and 8 us,
 // of steps of 1.7 and 0.22 ms. One launch takes up to MUON_BATCH tensors, so that the matrices of a model need a few launches a step;
 // a block has 2048 consecutive elements of one tensor, 8 a thread in 16-byte accesses. The direction is FP32: an unscaled gradient may lie
 // below FP16's range, and what is orthogonalised is scaled by its own norm only afterwards.

@@ -10,8 +10,9 @@
 // times), with the pair 0.02-0.2 %. For small matrices, and for all where the caller asks for it, A, P and the operand X are pairs too. X is
 // kept times 2^10, which takes its elements (about 1 / sqrt(rows * cols)) out of the range where FP16 loses bits.
 //
-// Large matrices are bound by the tensor cores under the power cap (four 5632 x 2048: 1.72 to 1.80 ms for five steps, 880 to 920 TFLOP/s), small ones by
-// the chain of three products a step (three 512 x 512: 88 us, 5.2 a launch), the smallest by the exchanges of a cluster (128 x 1000: 67 us).
+// Large matrices: four 5632 x 2048 take 1.72 ms for five steps (925 TFLOP/s; 1.45 to 1.5 ms of pure noise). By themselves A has the
+// tensor pipe at work 72 % of its cycles, X 74 %, P, with two rounds of short tiles, 51 %. Small ones wait for the chain of three products a
+// step (three 512 x 512: 87 us, 5.2 a launch), the smallest for the exchanges of a cluster (128 x 1000: 67 us).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -179,9 +180,9 @@ struct ns_shape {
 };
 
 // One warp's piece of the result, 32 rows (a lane each) x COLS columns. Inputs and results go between registers and memory directly, 32 bytes a lane
-// and access: the products alone take 125 of the 128 bytes that shared memory moves in a cycle (operands written, read, and read by
-// the peer), so staging tiles there for TMA costs the products their time (four 5632 x 2048 matrices: a step's UPDATE 170 us with staged
-// tiles, 128 us without any epilogue traffic).
+// and access, beside the products' operands in shared memory, not through it: with tiles staged there for TMA a step's UPDATE of four 5632 x
+// 2048 matrices took 170 us, without any epilogue traffic 128, and takes 153 so (tensor pipe 74 % busy, its reads of shared memory 34 % of
+// what that delivers).
 constexpr int NS_PIECE = 32, NS_STAGE_ROW = 80, NS_WARP_STAGE = NS_PIECE * NS_STAGE_ROW;   // rows of 64 bytes, 16 apart in the banks
 template <int COLS> struct ns_row {
     uint32_t w[COLS / 2];

@@ -542,8 +542,9 @@ uint64_t gdb200_embedding_backward_static_max_elems(void);
  * type), any cols, sums FP32, one rounding. rows may be 0.
  * Backward: grad_x (accumulate != 0: added into grad_x: round, add, round, as gd_backend_accumulate after the entry would), grad_weight =
  * sum over rows of grad_out * (x - mean) / sqrt(var + eps), grad_bias = sum over rows of grad_out; each may be NULL, not all three. The two
- * sums are FP32 in an order that depends on the shape alone, through partial sums in the backend's workspace (GD_ERR_UNSUPPORTED where one
- * row of them, 8 * cols bytes, does not fit it). grad_x may be grad_out where it is not accumulated into. */
+ * sums are FP32 in a fixed order, without atomics: a call repeats bit for bit. Which order depends on the shape, on whether x, grad_out and
+ * grad_x lie on 16 bytes, on the number of SMs and on the size of the backend's workspace, in which partial sums lie (GD_ERR_UNSUPPORTED
+ * where one row of them, 8 * cols bytes, does not fit). grad_x may be grad_out where it is not accumulated into. */
 typedef struct gdb200_layer_norm_args {
     uint64_t rows, cols;
     float eps;
@@ -557,8 +558,8 @@ gd_status gdb200_layer_norm_backward(gd_backend *backend, const gd_backend_tenso
 
 /* Embedding lookup with a scale, out[i] = round(scale * table[ids[i]]), NaN rows for ids outside the table as gd_backend_embedding_forward
  * gives; and its gradient grad_table[v] = round(scale * sum of grad_out[i] over the i with ids[i] = v), ids outside the table skipped.
- * Against gd_backend_embedding_backward: the rows are summed in FP32 in the order of the ids, so a call repeats bit for bit, no FP32
- * table is lent, and accumulate != 0 adds into grad_table (round, add, round, as gd_backend_accumulate after the plain call would)
+ * Against gd_backend_embedding_backward: the rows of a token are summed in FP32 in a fixed order (of the ids, in pieces whose size depends
+ * on the sizes, the number of SMs and the workspace), so a call repeats bit for bit, no FP32 table is lent, and accumulate != 0 adds into grad_table (round, add, round, as gd_backend_accumulate after the plain call would)
  * touching only the rows that the ids name (a tied head's gradient). F16, BF16, F32, any dim; up to 2^31 - 1 ids and table rows. The sorted
  * order (8 bytes an id) and partial sums lie in the backend's workspace; GD_ERR_OUT_OF_MEMORY where they do not fit. */
 gd_status gdb200_embedding_scaled_forward(gd_backend *backend, const gd_backend_tensor_view *table, const gd_backend_tensor_view *ids, const gd_backend_tensor_view *out, float scale,
