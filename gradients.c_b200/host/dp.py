@@ -93,10 +93,14 @@ class DataParallel:
         the ranks always issue the same collectives), and of the loss share. With the loss normalised by the
         global row count (shard_share) the sum IS the gradient of the global mean loss: no division by world."""
         ctx, lib = self.ctx, self.ctx.lib
+        reduced = set()   # (two parameters of one sum have one gradient)
         for slot in optimizer.slots:
             if slot.param.grad is None:
                 slot.param.grad = ctx.zeros(ctx.scratch, slot.param.dtype, slot.param.shape, "zero_grad")
             g = slot.param.grad
+            if (g.arena, g.offset) in reduced:
+                continue
+            reduced.add((g.arena, g.offset))
             ctx.check(lib.gdb200_dp_all_reduce(ctx.backend, g.buffer, g.offset, g.count, g.dtype), "dp_all_reduce")
         if loss is not None:
             ctx.check(lib.gdb200_dp_all_reduce(ctx.backend, loss.buffer, loss.offset, 1, F32), "dp_all_reduce(loss)")

@@ -129,3 +129,20 @@ def test_a_sum_of_a_tensor_with_itself(ctx):
     np.testing.assert_array_equal(read, [[2.0, 8.0]])
     np.testing.assert_array_equal(values_of(x.grad), [6.0, 24.0])
     np.testing.assert_array_equal(values_of(out.grad), [1.0, 4.0])
+
+
+def test_a_shared_gradient_is_reduced_once(ctx):
+    """Two parameters with one gradient in a data-parallel step: the sum over the ranks is taken once (on every rank, whose graphs are alike)."""
+    from types import SimpleNamespace
+    p, q, r = tensor(ctx, [1.0, 2.0]), tensor(ctx, [3.0, 4.0]), tensor(ctx, [5.0])
+    out = ops.gd_add(ctx, p, q)
+    out.grad = tensor(ctx, [1.0, 1.0], False)
+    ctx.run_backward()
+    reduced = []
+    ctx.lib.gdb200_dp_all_reduce = lambda be, buffer, offset, count, dtype: reduced.append((offset, count)) or 0
+    ctx.lib.gdb200_dp_join = lambda be: 0
+    ctx.zeros = lambda arena, dtype, shape, name="": ctx.scratch_empty(dtype, shape)
+    dp = pkg.dp.DataParallel.__new__(pkg.dp.DataParallel)
+    dp.ctx = ctx
+    dp.reduce_gradients(SimpleNamespace(slots=[SimpleNamespace(param=t) for t in (p, q, r)]))
+    assert reduced == [(p.grad.offset, 2), (r.grad.offset, 1)]
